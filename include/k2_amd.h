@@ -31,7 +31,8 @@ enum k2amd_status {
   K2AMD_ERR_SCRATCH_LIMIT = 6     /* k2amd_mi_forward_noalloc: shape beyond its static scratch array */
 };
 
-enum k2amd_dtype { K2AMD_F32 = 0, K2AMD_F64 = 1, K2AMD_F16 = 2 /* lattice scores only */ };
+enum k2amd_dtype { K2AMD_F32 = 0, K2AMD_F64 = 1, K2AMD_F16 = 2, K2AMD_BF16 = 3 };
+/* K2AMD_F16: lattice scores and rows of output logits; K2AMD_BF16: rows of output logits */
 
 /* rnnt_type of k2/python/k2/rnnt_loss.py:70 ("regular" | "modified" | "constrained") */
 enum k2amd_rnnt_type { K2AMD_REGULAR = 0, K2AMD_MODIFIED = 1, K2AMD_CONSTRAINED = 2 };
@@ -429,6 +430,58 @@ K2AMD_API int k2amd_lattice_fill(const int32_t *ranges, const int32_t *frames,
                                  const int32_t *arc_base, const int32_t *arc_local,
                                  int32_t *arc_splits, void *arcs, int32_t *arc_map, int B, int T,
                                  int R, int S, int C, int dtype, void *stream);
+
+/* ------------------------------------------------------------------ rows of output logits
+ *
+ * No counterpart in the reference.  `logits`: `rows` rows of C elements (dtype K2AMD_F32, K2AMD_F16 or K2AMD_BF16), row r
+ * at element r * row_stride, any alignment of the element type; p = softmax(x / temperature) of a row x, temperature > 0.
+ * `mask` [rows] (one byte a row, 0: the row does not count and is not read) or NULL.  Sums are held in 32 bits or more;
+ * results do not depend on the order in which workgroups run.  Served up to 2^24 - 1 rows a call.
+ *
+ * Log-probs of n given tokens a row (tokens [rows][n] int64; a negative one counts as absent and has log-prob 0, one past
+ * the vocabulary gives NaN), the entropy (or NULL) and the k largest logits in falling order, the lower index first where
+ * they are equal: top_logprobs [rows][k], top_tokens [rows][k] int64 (-inf and -1 past the C-th).  n and k <= 64.
+ * Rows that do not count get 0, 0, -inf and -1.  A row of nothing but -inf has p = 0, entropy 0 and log-probs -inf.
+ * stats [rows][2] (or NULL) and entropy are what the backward call reads.
+ *
+ * Backward: logits_grad [rows][C] (dense, of the logits' type) from what reaches the three results (each may be NULL).
+ * A token listed twice takes both gradients. */
+K2AMD_API int k2amd_token_logprobs_forward(const void *logits, long long row_stride, const int64_t *tokens,
+                                           const uint8_t *mask, float *logprobs, float *entropy, float *top_logprobs,
+                                           int64_t *top_tokens, float *stats, long long rows, int C, int n, int k,
+                                           float temperature, int dtype, void *stream);
+K2AMD_API int k2amd_token_logprobs_backward(const void *logits, long long row_stride, const int64_t *tokens,
+                                            const uint8_t *mask, const float *stats, const float *entropy,
+                                            const int64_t *top_tokens, const float *logprobs_grad,
+                                            const float *entropy_grad, const float *top_grad, void *logits_grad,
+                                            long long rows, int C, int n, int k, float temperature, int dtype, void *stream);
+
+/* Distillation from a teacher's list of K <= 256 tokens a row: top_tokens [rows][K] int64 (negative: no entry; past the
+ * vocabulary: the row's loss is NaN), top_logprobs [rows][K].  rest == 0: the list is renormalised (q = softmax of its
+ * log-probs); rest != 0: q = exp(log-probs) and what they leave of 1 is one more outcome, the student's counterpart of
+ * which is everything that is not listed (a row without any student mass there has no such outcome).
+ * row_losses [rows] = KL(q || p); 0 for rows that do not count or have no list.  records [rows][4] (or NULL): for the
+ * backward call, which writes logits_grad [rows][C] for loss_grad[r / rows_per_loss] * factor * inverse_count[0] (or 1
+ * where NULL) reaching row r's loss.
+ * _sum: sums[i] = factor * (sum of rows_per_sum row losses), divided by the number of rows that count where mean != 0;
+ * inverse_count [num_sums] (or NULL) = 1 / max(that number, 1); scratch as the query says. */
+K2AMD_API int k2amd_distillation_forward(const void *logits, long long row_stride, const float *top_logprobs,
+                                         const int64_t *top_tokens, const uint8_t *mask, float *row_losses, float *records,
+                                         long long rows, int C, int K, int rest, float temperature, int dtype, void *stream);
+K2AMD_API int k2amd_distillation_backward(const void *logits, long long row_stride, const float *top_logprobs,
+                                          const int64_t *top_tokens, const float *records, const float *loss_grad,
+                                          long long rows_per_loss, const float *inverse_count, float factor,
+                                          void *logits_grad, long long rows, int C, int K, int rest, float temperature,
+                                          int dtype, void *stream);
+K2AMD_API size_t k2amd_distillation_sum_scratch_bytes(long long num_sums, long long rows_per_sum);
+K2AMD_API int k2amd_distillation_sum(const float *row_losses, const uint8_t *mask, float *sums, float *inverse_count,
+                                     long long num_sums, long long rows_per_sum, int mean, float factor, void *scratch,
+                                     size_t scratch_bytes, void *stream);
+
+/* mask [B][T][R] = 1 where row (b, t, k) of a pruned lattice lies in its sequence's box: boundary[b][1] <= t <
+ * boundary[b][3] and boundary[b][0] <= ranges[b][t][k] <= boundary[b][2], else 0. */
+K2AMD_API int k2amd_rnnt_pruned_mask(const int64_t *ranges, const int64_t *boundary, uint8_t *mask, int B, int T, int R,
+                                     void *stream);
 
 #ifdef __cplusplus
 }

@@ -21,6 +21,8 @@ RNNT_TYPES = {"regular": REGULAR, "modified": MODIFIED, "constrained": CONSTRAIN
 _vp = ctypes.c_void_p
 _ci = ctypes.c_int
 _sz = ctypes.c_size_t
+_ll = ctypes.c_longlong
+_cf = ctypes.c_float
 
 _SIGNATURES = {
     "k2amd_version": ([], _ci),
@@ -71,6 +73,13 @@ _SIGNATURES = {
     "k2amd_rnnt_prune_gather_backward": ([_vp] * 3 + [_ci] * 6 + [_vp], _ci),
     "k2amd_lattice_count": ([_vp] * 6 + [_ci] * 3 + [_vp], _ci),
     "k2amd_lattice_fill": ([_vp] * 11 + [_ci] * 6 + [_vp], _ci),
+    "k2amd_token_logprobs_forward": ([_vp, _ll] + [_vp] * 7 + [_ll] + [_ci] * 3 + [_cf, _ci, _vp], _ci),
+    "k2amd_token_logprobs_backward": ([_vp, _ll] + [_vp] * 9 + [_ll] + [_ci] * 3 + [_cf, _ci, _vp], _ci),
+    "k2amd_distillation_forward": ([_vp, _ll] + [_vp] * 5 + [_ll] + [_ci] * 3 + [_cf, _ci, _vp], _ci),
+    "k2amd_distillation_backward": ([_vp, _ll] + [_vp] * 4 + [_ll, _vp, _cf, _vp, _ll] + [_ci] * 3 + [_cf, _ci, _vp], _ci),
+    "k2amd_distillation_sum_scratch_bytes": ([_ll] * 2, _sz),
+    "k2amd_distillation_sum": ([_vp] * 4 + [_ll] * 2 + [_ci, _cf, _vp, _sz, _vp], _ci),
+    "k2amd_rnnt_pruned_mask": ([_vp] * 3 + [_ci] * 3 + [_vp], _ci),
 }
 
 
@@ -774,3 +783,169 @@ def pruned_ranges_to_lattice(ranges, frames, symbols, logits):
                                        ptr(arc_local), ptr(arc_splits), ptr(arcs), ptr(arc_map), B, T,
                                        R, S, C, code, stream_ptr(dev)))
     return state_splits, arc_splits, arcs, arc_map
+
+
+# ---- rows of output logits -------------------------------------------------------------------
+
+BF16 = 3
+MAX_TOKENS, MAX_TOP, MAX_TEACHER = 64, 64, 256
+_LOGITS_DTYPES = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
+
+
+def _logits_rows(logits):
+    """(logits, rows, row stride, C, dtype code) of logits [..., C]: as they are where their rows lie at one distance from
+    each other, else a dense copy."""
+    if not isinstance(logits, torch.Tensor) or logits.dtype not in _LOGITS_DTYPES:
+        raise RuntimeError("k2_amd: logits must be a float32, float16 or bfloat16 tensor")
+    if not _on_device(logits):
+        raise RuntimeError(f"k2_amd runs on MI355X only: logits are on {logits.device} (there is no CPU path)")
+    if logits.dim() < 1 or logits.shape[-1] < 1:
+        raise RuntimeError(f"k2_amd: logits must be [..., C] with C >= 1, got {list(logits.shape)}")
+    C = logits.shape[-1]
+    rows = logits.numel() // C
+    if logits.is_contiguous():
+        return logits, rows, C, C, _LOGITS_DTYPES[logits.dtype]
+    stride, expected = C, None
+    uniform = logits.stride(-1) == 1 or C == 1
+    for d in range(logits.dim() - 2, -1, -1):
+        if logits.shape[d] == 1:
+            continue
+        if expected is None:
+            stride = logits.stride(d)
+        elif logits.stride(d) != expected:
+            uniform = False
+        expected = logits.stride(d) * logits.shape[d]
+    if not uniform:
+        logits, stride = logits.contiguous(), C
+    return logits, rows, stride, C, _LOGITS_DTYPES[logits.dtype]
+
+
+def _token_rows(logits, tokens):
+    """Number of tokens a row: tokens has the rows' shape, or one more dimension."""
+    if tokens is None:
+        return 0
+    lead = tuple(logits.shape[:-1])
+    if tuple(tokens.shape) != lead and tuple(tokens.shape[:-1]) != lead:
+        raise RuntimeError(f"k2_amd: tokens {list(tokens.shape)} do not belong to logits {list(logits.shape)}")
+    expect(tokens, "tokens", torch.int64, logits.device, tokens.shape)
+    return 1 if tuple(tokens.shape) == lead else tokens.shape[-1]
+
+
+def token_logprobs_forward(logits, tokens, mask, temperature, num_top, return_entropy, keep):
+    """Returns (logprobs, entropy, top_logprobs, top_tokens, stats), None where not asked for; ``keep``: whether to return
+    what the backward call reads."""
+    lead, dev = tuple(logits.shape[:-1]), logits.device
+    x, rows, stride, C, dt = _logits_rows(logits)
+    n = _token_rows(logits, tokens)
+    expect_optional(mask, "mask", torch.bool, dev, lead)
+    if num_top < 0:
+        raise RuntimeError("k2_amd: num_top must not be negative")
+    logprobs = None if tokens is None else torch.empty(tokens.shape, dtype=torch.float32, device=dev)
+    entropy = torch.empty(lead, dtype=torch.float32, device=dev) if return_entropy else None
+    top_logprobs = torch.empty(lead + (num_top,), dtype=torch.float32, device=dev) if num_top else None
+    top_tokens = torch.empty(lead + (num_top,), dtype=torch.int64, device=dev) if num_top else None
+    stats = torch.empty(lead + (2,), dtype=torch.float32, device=dev) if keep else None
+    with torch.cuda.device(dev):
+        check(lib().k2amd_token_logprobs_forward(
+            x.data_ptr(), stride, ptr(tokens), ptr(mask), ptr(logprobs), ptr(entropy), ptr(top_logprobs), ptr(top_tokens),
+            ptr(stats), rows, C, n, num_top, temperature, dt, stream_ptr(dev)))
+    return logprobs, entropy, top_logprobs, top_tokens, stats
+
+
+def token_logprobs_backward(logits, tokens, mask, stats, entropy, top_tokens, logprobs_grad, entropy_grad, top_grad,
+                            temperature):
+    """logits_grad, dense; each of the three gradients may be None."""
+    lead, dev = tuple(logits.shape[:-1]), logits.device
+    x, rows, stride, C, dt = _logits_rows(logits)
+    n = _token_rows(logits, tokens)
+    k = 0 if top_tokens is None else top_tokens.shape[-1]
+    expect_optional(mask, "mask", torch.bool, dev, lead)
+    expect(stats, "stats", torch.float32, dev, lead + (2,))
+    expect_optional(entropy, "entropy", torch.float32, dev, lead)
+    expect_optional(top_tokens, "top_tokens", torch.int64, dev, lead + (k,))
+    if logprobs_grad is not None and tokens is None or entropy_grad is not None and entropy is None or \
+            top_grad is not None and top_tokens is None:
+        raise RuntimeError("k2_amd: a gradient of a result that the forward call did not return")
+    expect_optional(logprobs_grad, "logprobs_grad", torch.float32, dev, () if tokens is None else tokens.shape)
+    expect_optional(entropy_grad, "entropy_grad", torch.float32, dev, lead)
+    expect_optional(top_grad, "top_grad", torch.float32, dev, lead + (k,))
+    grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+    with torch.cuda.device(dev):
+        check(lib().k2amd_token_logprobs_backward(
+            x.data_ptr(), stride, ptr(tokens), ptr(mask), ptr(stats), ptr(entropy), ptr(top_tokens), ptr(logprobs_grad),
+            ptr(entropy_grad), ptr(top_grad), ptr(grad), rows, C, n, k, temperature, dt, stream_ptr(dev)))
+    return grad
+
+
+def _teacher_list(logits, top_logprobs, top_tokens):
+    lead, dev = tuple(logits.shape[:-1]), logits.device
+    if top_tokens.dim() < 1:
+        raise RuntimeError("k2_amd: top_tokens must be [..., K]")
+    K = top_tokens.shape[-1]
+    expect(top_tokens, "top_tokens", torch.int64, dev, lead + (K,))
+    expect(top_logprobs, "top_logprobs", torch.float32, dev, lead + (K,))
+    return K
+
+
+def distillation_forward(logits, top_logprobs, top_tokens, mask, temperature, bucket, keep):
+    """(row losses of the rows' shape, records for the backward call or None)."""
+    lead, dev = tuple(logits.shape[:-1]), logits.device
+    x, rows, stride, C, dt = _logits_rows(logits)
+    K = _teacher_list(logits, top_logprobs, top_tokens)
+    expect_optional(mask, "mask", torch.bool, dev, lead)
+    losses = torch.empty(lead, dtype=torch.float32, device=dev)
+    records = torch.empty(lead + (4,), dtype=torch.float32, device=dev) if keep else None
+    with torch.cuda.device(dev):
+        check(lib().k2amd_distillation_forward(x.data_ptr(), stride, ptr(top_logprobs), ptr(top_tokens), ptr(mask),
+                                               ptr(losses), ptr(records), rows, C, K, int(bucket), temperature, dt,
+                                               stream_ptr(dev)))
+    return losses, records
+
+
+def distillation_sum(losses, mask, sums, mean, factor):
+    """(sums [sums], 1 / number of rows that count [sums] or None): ``sums`` equal shares of the row losses."""
+    dev = losses.device
+    expect(losses, "row losses", torch.float32, dev, losses.shape)
+    expect_optional(mask, "mask", torch.bool, dev, losses.shape)
+    if sums < 0 or (sums == 0 and losses.numel() > 0) or (sums > 0 and losses.numel() % sums != 0):
+        raise RuntimeError(f"k2_amd: {losses.numel()} row losses cannot be cut into {sums} sums")
+    per_sum = losses.numel() // max(sums, 1)
+    out = torch.empty(sums, dtype=torch.float32, device=dev)
+    inverse_count = torch.empty(sums, dtype=torch.float32, device=dev) if mean else None
+    nbytes = lib().k2amd_distillation_sum_scratch_bytes(sums, per_sum)
+    scratch = torch.empty(max(nbytes, 8), dtype=torch.uint8, device=dev)
+    with torch.cuda.device(dev):
+        check(lib().k2amd_distillation_sum(ptr(losses), ptr(mask), ptr(out), ptr(inverse_count), sums, per_sum, int(mean),
+                                           factor, ptr(scratch), scratch.numel(), stream_ptr(dev)))
+    return out, inverse_count
+
+
+def distillation_backward(logits, top_logprobs, top_tokens, records, loss_grad, inverse_count, factor, temperature, bucket):
+    """logits_grad, dense.  loss_grad: one value for every equal share of the rows."""
+    lead, dev = tuple(logits.shape[:-1]), logits.device
+    x, rows, stride, C, dt = _logits_rows(logits)
+    K = _teacher_list(logits, top_logprobs, top_tokens)
+    expect(records, "records", torch.float32, dev, lead + (4,))
+    expect(loss_grad, "loss_grad", torch.float32, dev, loss_grad.shape)
+    losses = loss_grad.numel()
+    if rows > 0 and (losses < 1 or rows % losses != 0):
+        raise RuntimeError(f"k2_amd: {losses} loss gradients for {rows} rows")
+    expect_optional(inverse_count, "inverse_count", torch.float32, dev, (1,))
+    grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+    with torch.cuda.device(dev):
+        check(lib().k2amd_distillation_backward(x.data_ptr(), stride, ptr(top_logprobs), ptr(top_tokens), ptr(records),
+                                                ptr(loss_grad), max(rows // max(losses, 1), 1), ptr(inverse_count), factor,
+                                                ptr(grad), rows, C, K, int(bucket), temperature, dt, stream_ptr(dev)))
+    return grad
+
+
+def pruned_mask(ranges, boundary):
+    """bool [B][T][R]: the rows of a pruned lattice inside their sequence's box."""
+    B, T, R = _dims(ranges, "ranges", 3)
+    dev = ranges.device
+    expect(ranges, "ranges", torch.int64, dev, (B, T, R))
+    expect(boundary, "boundary", torch.int64, dev, (B, 4))
+    mask = torch.empty(B, T, R, dtype=torch.bool, device=dev)
+    with torch.cuda.device(dev):
+        check(lib().k2amd_rnnt_pruned_mask(ptr(ranges), ptr(boundary), ptr(mask), B, T, R, stream_ptr(dev)))
+    return mask

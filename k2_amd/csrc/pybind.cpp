@@ -859,6 +859,240 @@ class BoundaryRead {
   at::cuda::CUDAEvent event_;
 };
 
+namespace {
+
+// ---------------------------------------------------------------------------------------------
+// Rows of output logits (k2_amd/token_loss.py); no counterpart in the reference.
+
+typedef torch::optional<torch::Tensor> OptionalTensor;
+
+// logits [..., C] as rows: as they are where their rows lie at one distance from each other, else a dense copy
+struct LogitsRows {
+  torch::Tensor x;
+  int64_t rows, stride, C;
+  int dtype;
+  std::vector<int64_t> lead;
+
+  explicit LogitsRows(const torch::Tensor &logits) : x(logits) {
+    TORCH_CHECK(logits.is_cuda(), "k2_amd runs on MI355X only: logits are on ", logits.device(), " (there is no CPU path)");
+    const auto type = logits.scalar_type();
+    TORCH_CHECK(type == torch::kFloat || type == torch::kHalf || type == torch::kBFloat16,
+                "k2_amd: logits must be a float32, float16 or bfloat16 tensor");
+    dtype = type == torch::kFloat ? K2AMD_F32 : type == torch::kHalf ? K2AMD_F16 : K2AMD_BF16;
+    TORCH_CHECK(logits.dim() >= 1 && logits.size(-1) >= 1, "k2_amd: logits must be [..., C] with C >= 1, got ",
+                logits.sizes());
+    C = logits.size(-1);
+    rows = logits.numel() / C;
+    lead.assign(logits.sizes().begin(), logits.sizes().end() - 1);
+    stride = C;
+    if (logits.is_contiguous()) return;
+    bool uniform = logits.stride(-1) == 1 || C == 1;
+    int64_t expected = -1;
+    for (int64_t d = logits.dim() - 2; d >= 0; --d) {
+      if (logits.size(d) == 1) continue;
+      if (expected < 0) stride = logits.stride(d);
+      else if (logits.stride(d) != expected) uniform = false;
+      expected = logits.stride(d) * logits.size(d);
+    }
+    if (!uniform) {
+      x = logits.contiguous();
+      stride = C;
+    }
+  }
+  std::vector<int64_t> Shape(int64_t last) const {
+    std::vector<int64_t> shape = lead;
+    shape.push_back(last);
+    return shape;
+  }
+  torch::TensorOptions Floats() const { return x.options().dtype(torch::kFloat); }
+};
+
+bool Same(const torch::Tensor &t, torch::IntArrayRef shape) { return t.sizes() == shape; }
+void ExpectShape(const torch::Tensor &t, const char *name, c10::ScalarType dtype, const torch::Device &dev,
+                 torch::IntArrayRef shape) {
+  RequireDevice(t, name);
+  TORCH_CHECK(t.scalar_type() == dtype && t.device() == dev && Same(t, shape), "k2_amd: ", name, " must be ", dtype, " ", shape,
+              " on ", dev, ", got ", t.scalar_type(), " ", t.sizes(), " on ", t.device());
+}
+void ExpectShape(const OptionalTensor &t, const char *name, c10::ScalarType dtype, const torch::Device &dev,
+                 torch::IntArrayRef shape) {
+  if (Given(t)) ExpectShape(*t, name, dtype, dev, shape);
+}
+const uint8_t *MaskPtr(const OptionalTensor &mask) {
+  return Given(mask) ? static_cast<const uint8_t *>(mask->data_ptr()) : nullptr;
+}
+float *FloatPtr(const OptionalTensor &t) { return Given(t) ? t->data_ptr<float>() : nullptr; }
+
+// how many tokens a row: tokens has the rows' shape, or one more dimension
+int64_t TokensOfRow(const LogitsRows &r, const OptionalTensor &tokens) {
+  if (!Given(tokens)) return 0;
+  const auto sizes = tokens->sizes();
+  const bool one = Same(*tokens, r.lead);
+  TORCH_CHECK(one || (sizes.size() == r.lead.size() + 1 && sizes.slice(0, r.lead.size()) == torch::IntArrayRef(r.lead)),
+              "k2_amd: tokens ", sizes, " do not belong to these logits");
+  ExpectShape(tokens, "tokens", torch::kLong, r.x.device(), sizes);
+  return one ? 1 : sizes.back();
+}
+int Int(int64_t v) {
+  TORCH_CHECK(v >= 0 && v < (int64_t(1) << 31), "k2_amd: size ", v, " out of range");
+  return static_cast<int>(v);
+}
+
+std::tuple<OptionalTensor, OptionalTensor, OptionalTensor, OptionalTensor, OptionalTensor> TokenLogprobsForward(
+    torch::Tensor logits, OptionalTensor tokens, OptionalTensor mask, double temperature, int64_t num_top,
+    bool return_entropy, bool keep) {
+  const LogitsRows r(logits);
+  const auto dev = logits.device();
+  const int64_t n = TokensOfRow(r, tokens);
+  ExpectShape(mask, "mask", torch::kBool, dev, r.lead);
+  c10::hip::HIPGuardMasqueradingAsCUDA guard(dev);
+  OptionalTensor logprobs, entropy, top_logprobs, top_tokens, stats;
+  if (Given(tokens)) logprobs = torch::empty(tokens->sizes(), r.Floats());
+  if (return_entropy) entropy = torch::empty(r.lead, r.Floats());
+  if (num_top != 0) {
+    top_logprobs = torch::empty(r.Shape(Int(num_top)), r.Floats());
+    top_tokens = torch::empty(r.Shape(num_top), r.Floats().dtype(torch::kLong));
+  }
+  if (keep) stats = torch::empty(r.Shape(2), r.Floats());
+  void *stream = StreamOf(logits);
+  {
+    pybind11::gil_scoped_release release;
+    Check(k2amd_token_logprobs_forward(r.x.data_ptr(), r.stride, I64(tokens), MaskPtr(mask), FloatPtr(logprobs),
+                                       FloatPtr(entropy), FloatPtr(top_logprobs),
+                                       Given(top_tokens) ? top_tokens->data_ptr<int64_t>() : nullptr, FloatPtr(stats), r.rows,
+                                       Int(r.C), Int(n), Int(num_top), static_cast<float>(temperature), r.dtype, stream));
+  }
+  return std::make_tuple(logprobs, entropy, top_logprobs, top_tokens, stats);
+}
+
+torch::Tensor TokenLogprobsBackward(torch::Tensor logits, OptionalTensor tokens, OptionalTensor mask, torch::Tensor stats,
+                                    OptionalTensor entropy, OptionalTensor top_tokens, OptionalTensor logprobs_grad,
+                                    OptionalTensor entropy_grad, OptionalTensor top_grad, double temperature) {
+  const LogitsRows r(logits);
+  const auto dev = logits.device();
+  const int64_t n = TokensOfRow(r, tokens), k = Given(top_tokens) && top_tokens->dim() > 0 ? top_tokens->size(-1) : 0;
+  ExpectShape(mask, "mask", torch::kBool, dev, r.lead);
+  ExpectShape(stats, "stats", torch::kFloat, dev, r.Shape(2));
+  ExpectShape(entropy, "entropy", torch::kFloat, dev, r.lead);
+  ExpectShape(top_tokens, "top_tokens", torch::kLong, dev, r.Shape(k));
+  TORCH_CHECK((!Given(logprobs_grad) || Given(tokens)) && (!Given(entropy_grad) || Given(entropy)) &&
+                  (!Given(top_grad) || Given(top_tokens)),
+              "k2_amd: a gradient of a result that the forward call did not return");
+  if (Given(logprobs_grad)) ExpectShape(logprobs_grad, "logprobs_grad", torch::kFloat, dev, tokens->sizes());
+  ExpectShape(entropy_grad, "entropy_grad", torch::kFloat, dev, r.lead);
+  ExpectShape(top_grad, "top_grad", torch::kFloat, dev, r.Shape(k));
+  c10::hip::HIPGuardMasqueradingAsCUDA guard(dev);
+  torch::Tensor grad = torch::empty(logits.sizes(), r.x.options());
+  void *stream = StreamOf(logits);
+  {
+    pybind11::gil_scoped_release release;
+    Check(k2amd_token_logprobs_backward(r.x.data_ptr(), r.stride, I64(tokens), MaskPtr(mask), stats.data_ptr<float>(),
+                                        FloatPtr(entropy), I64(top_tokens), FloatPtr(logprobs_grad), FloatPtr(entropy_grad),
+                                        FloatPtr(top_grad), grad.data_ptr(), r.rows, Int(r.C), Int(n), Int(k),
+                                        static_cast<float>(temperature), r.dtype, stream));
+  }
+  return grad;
+}
+
+int64_t ExpectTeacher(const LogitsRows &r, const torch::Tensor &top_logprobs, const torch::Tensor &top_tokens) {
+  TORCH_CHECK(top_tokens.dim() >= 1, "k2_amd: top_tokens must be [..., K]");
+  const int64_t K = top_tokens.size(-1);
+  ExpectShape(top_tokens, "top_tokens", torch::kLong, r.x.device(), r.Shape(K));
+  ExpectShape(top_logprobs, "top_logprobs", torch::kFloat, r.x.device(), r.Shape(K));
+  return K;
+}
+
+std::tuple<torch::Tensor, OptionalTensor> DistillationForward(torch::Tensor logits, torch::Tensor top_logprobs,
+                                                              torch::Tensor top_tokens, OptionalTensor mask,
+                                                              double temperature, bool bucket, bool keep) {
+  const LogitsRows r(logits);
+  const int64_t K = ExpectTeacher(r, top_logprobs, top_tokens);
+  ExpectShape(mask, "mask", torch::kBool, logits.device(), r.lead);
+  c10::hip::HIPGuardMasqueradingAsCUDA guard(logits.device());
+  torch::Tensor losses = torch::empty(r.lead, r.Floats());
+  OptionalTensor records;
+  if (keep) records = torch::empty(r.Shape(4), r.Floats());
+  void *stream = StreamOf(logits);
+  {
+    pybind11::gil_scoped_release release;
+    Check(k2amd_distillation_forward(r.x.data_ptr(), r.stride, top_logprobs.data_ptr<float>(), I64(top_tokens), MaskPtr(mask),
+                                     losses.data_ptr<float>(), FloatPtr(records), r.rows, Int(r.C), Int(K), bucket ? 1 : 0,
+                                     static_cast<float>(temperature), r.dtype, stream));
+  }
+  return std::make_tuple(losses, records);
+}
+
+std::tuple<torch::Tensor, OptionalTensor> DistillationSum(torch::Tensor losses, OptionalTensor mask, int64_t sums, bool mean,
+                                                          double factor) {
+  const auto dev = losses.device();
+  ExpectShape(losses, "row losses", torch::kFloat, dev, losses.sizes());
+  ExpectShape(mask, "mask", torch::kBool, dev, losses.sizes());
+  TORCH_CHECK(sums >= 0 && (sums > 0 ? losses.numel() % sums == 0 : losses.numel() == 0), "k2_amd: ", losses.numel(),
+              " row losses cannot be cut into ", sums, " sums");
+  const int64_t per_sum = losses.numel() / std::max<int64_t>(sums, 1);
+  c10::hip::HIPGuardMasqueradingAsCUDA guard(dev);
+  torch::Tensor out = torch::empty({sums}, losses.options());
+  OptionalTensor inverse_count;
+  if (mean) inverse_count = torch::empty({sums}, losses.options());
+  const size_t bytes = k2amd_distillation_sum_scratch_bytes(sums, per_sum);
+  torch::Tensor scratch =
+      torch::empty({static_cast<int64_t>(std::max<size_t>(bytes, 8))}, losses.options().dtype(torch::kUInt8));
+  void *stream = StreamOf(losses);
+  {
+    pybind11::gil_scoped_release release;
+    Check(k2amd_distillation_sum(losses.data_ptr<float>(), MaskPtr(mask), out.data_ptr<float>(), FloatPtr(inverse_count), sums,
+                                 per_sum, mean ? 1 : 0, static_cast<float>(factor), scratch.data_ptr(),
+                                 static_cast<size_t>(scratch.numel()), stream));
+  }
+  return std::make_tuple(out, inverse_count);
+}
+
+torch::Tensor DistillationBackward(torch::Tensor logits, torch::Tensor top_logprobs, torch::Tensor top_tokens,
+                                   torch::Tensor records, torch::Tensor loss_grad, OptionalTensor inverse_count, double factor,
+                                   double temperature, bool bucket) {
+  const LogitsRows r(logits);
+  const auto dev = logits.device();
+  const int64_t K = ExpectTeacher(r, top_logprobs, top_tokens);
+  ExpectShape(records, "records", torch::kFloat, dev, r.Shape(4));
+  ExpectShape(loss_grad, "loss_grad", torch::kFloat, dev, loss_grad.sizes());
+  const int64_t losses = loss_grad.numel();
+  TORCH_CHECK(r.rows == 0 || (losses >= 1 && r.rows % losses == 0), "k2_amd: ", losses, " loss gradients for ", r.rows,
+              " rows");
+  ExpectShape(inverse_count, "inverse_count", torch::kFloat, dev, {1});
+  c10::hip::HIPGuardMasqueradingAsCUDA guard(dev);
+  torch::Tensor grad = torch::empty(logits.sizes(), r.x.options());
+  void *stream = StreamOf(logits);
+  {
+    pybind11::gil_scoped_release release;
+    Check(k2amd_distillation_backward(r.x.data_ptr(), r.stride, top_logprobs.data_ptr<float>(), I64(top_tokens),
+                                      records.data_ptr<float>(), loss_grad.data_ptr<float>(),
+                                      std::max<int64_t>(r.rows / std::max<int64_t>(losses, 1), 1), FloatPtr(inverse_count),
+                                      static_cast<float>(factor), grad.data_ptr(), r.rows, Int(r.C), Int(K), bucket ? 1 : 0,
+                                      static_cast<float>(temperature), r.dtype, stream));
+  }
+  return grad;
+}
+
+torch::Tensor PrunedMask(torch::Tensor ranges, torch::Tensor boundary) {
+  RequireDevice(ranges, "ranges");
+  TORCH_CHECK(ranges.dim() == 3, "k2_amd: ranges must have 3 dimensions, got ", ranges.dim());
+  const auto dev = ranges.device();
+  Expect(ranges, "ranges", torch::kLong, dev, {ranges.size(0), ranges.size(1), ranges.size(2)});
+  Expect(boundary, "boundary", torch::kLong, dev, {ranges.size(0), 4});
+  c10::hip::HIPGuardMasqueradingAsCUDA guard(dev);
+  torch::Tensor mask = torch::empty(ranges.sizes(), ranges.options().dtype(torch::kBool));
+  void *stream = StreamOf(ranges);
+  {
+    pybind11::gil_scoped_release release;
+    Check(k2amd_rnnt_pruned_mask(ranges.data_ptr<int64_t>(), boundary.data_ptr<int64_t>(),
+                                 static_cast<uint8_t *>(mask.data_ptr()), Int(ranges.size(0)), Int(ranges.size(1)),
+                                 Int(ranges.size(2)), stream));
+  }
+  return mask;
+}
+
+}  // namespace
+
 PYBIND11_MODULE(_k2_amd, m) {
   m.doc() = "MI355X host layer of the k2 mutual-information recursion";
   pybind11::class_<BoundaryRead>(m, "BoundaryRead")
@@ -901,4 +1135,10 @@ PYBIND11_MODULE(_k2_amd, m) {
   m.def("prune_gather_backward", &PruneGatherBackward);
   m.def("pruned_ranges_to_lattice", &PrunedRangesToLattice, pybind11::arg("ranges"),
         pybind11::arg("frames"), pybind11::arg("symbols"), pybind11::arg("logits"));
+  m.def("token_logprobs_forward", &TokenLogprobsForward);
+  m.def("token_logprobs_backward", &TokenLogprobsBackward);
+  m.def("distillation_forward", &DistillationForward);
+  m.def("distillation_sum", &DistillationSum);
+  m.def("distillation_backward", &DistillationBackward);
+  m.def("pruned_mask", &PrunedMask);
 }

@@ -307,3 +307,52 @@ def pruned_ranges_to_lattice(ranges, frames, symbols, logits):
         raise RuntimeError("ranges and frames must be int32, symbols int64")
     return capi.pruned_ranges_to_lattice(ranges.contiguous(), frames.contiguous(),
                                          symbols.contiguous(), logits)
+
+
+# ---- rows of output logits (token_loss.py; no counterpart in the reference) ---------------------
+
+MAX_TOKENS, MAX_TOP, MAX_TEACHER = capi.MAX_TOKENS, capi.MAX_TOP, capi.MAX_TEACHER
+
+
+def token_logprobs_forward(logits, tokens, mask, temperature, num_top, return_entropy, keep):
+    _require_device(logits)
+    if _ext is not None:
+        return _ext.token_logprobs_forward(logits, tokens, mask, temperature, num_top, return_entropy, keep)
+    return capi.token_logprobs_forward(logits, tokens, mask, temperature, num_top, return_entropy, keep)
+
+
+def token_logprobs_backward(logits, tokens, mask, stats, entropy, top_tokens, logprobs_grad, entropy_grad, top_grad,
+                            temperature):
+    if _ext is not None:
+        return _ext.token_logprobs_backward(logits, tokens, mask, stats, entropy, top_tokens, logprobs_grad, entropy_grad,
+                                            top_grad, temperature)
+    return capi.token_logprobs_backward(logits, tokens, mask, stats, entropy, top_tokens, logprobs_grad, entropy_grad,
+                                        top_grad, temperature)
+
+
+def distillation_forward(logits, top_logprobs, top_tokens, mask, temperature, bucket, keep):
+    _require_device(logits)
+    if _ext is not None:
+        return _ext.distillation_forward(logits, top_logprobs, top_tokens, mask, temperature, bucket, keep)
+    return capi.distillation_forward(logits, top_logprobs, top_tokens, mask, temperature, bucket, keep)
+
+
+def distillation_sum(losses, mask, sums, mean, factor):
+    if _ext is not None:
+        return _ext.distillation_sum(losses, mask, sums, mean, factor)
+    return capi.distillation_sum(losses, mask, sums, mean, factor)
+
+
+def distillation_backward(logits, top_logprobs, top_tokens, records, loss_grad, inverse_count, factor, temperature, bucket):
+    if _ext is not None:
+        return _ext.distillation_backward(logits, top_logprobs, top_tokens, records, loss_grad, inverse_count, factor,
+                                          temperature, bucket)
+    return capi.distillation_backward(logits, top_logprobs, top_tokens, records, loss_grad, inverse_count, factor,
+                                      temperature, bucket)
+
+
+def pruned_mask(ranges, boundary):
+    _require_device(ranges)
+    if _ext is not None:
+        return _ext.pruned_mask(ranges, boundary)
+    return capi.pruned_mask(ranges, boundary)

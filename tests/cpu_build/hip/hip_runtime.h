@@ -427,6 +427,8 @@ inline T atomicAdd(T *address, T value) { return std::atomic_ref<T>(*address).fe
 template <typename T>
 inline T unsafeAtomicAdd(T *address, T value) { return atomicAdd(address, value); }
 template <typename T>
+inline T atomicOr(T *address, T value) { return std::atomic_ref<T>(*address).fetch_or(value); }
+template <typename T>
 inline T atomicMax(T *address, T value) {
   std::atomic_ref<T> a(*address);
   T old = a.load();
@@ -458,6 +460,19 @@ inline float __half2float(__half h) {
   float f;
   memcpy(&f, &u, 4);
   return f;
+}
+// and the hardware's conversion to it (round to nearest even)
+inline unsigned short hip_threads_to_half(float f) {
+  uint32_t u;
+  memcpy(&u, &f, 4);
+  const uint16_t sign = (uint16_t)((u >> 16) & 0x8000u);
+  const double a = fabs((double)f);
+  if (f != f) return (unsigned short)(sign | 0x7e00u);
+  if (a >= 65520.0) return (unsigned short)(sign | 0x7c00u);  // the midpoint to the next power of two rounds to infinity
+  // steps of the half's last place at this magnitude; nearbyint rounds to even
+  const int exponent = a < 6.103515625e-5 ? -14 : ilogb(a);
+  const double steps = nearbyint(ldexp(a, 10 - exponent));  // below 2048; a carry runs into the exponent as it should
+  return (unsigned short)(sign + (a < 6.103515625e-5 ? (uint16_t)steps : (uint16_t)(((exponent + 15) << 10) + (int)steps - 1024)));
 }
 
 #endif  // K2_AMD_TESTS_CPU_BUILD_HIP_RUNTIME_H_

@@ -44,6 +44,14 @@ FLAGS = ["-std=c++20", "-O1", "-g", "-fPIC", "-pthread", "-ffp-contract=off", f"
 _lib = None
 
 
+# the 16-bit element types of token_rows.h, which the files that include it get in line
+TOKEN_ROWS_EDITS = [
+    ("return static_cast<float>(__builtin_bit_cast(_Float16, u));", "return __half2float(__half{u});", 1),
+    ("return __builtin_bit_cast(unsigned short, static_cast<_Float16>(f));", "return hip_threads_to_half(f);", 1),
+    ("return __builtin_bit_cast(unsigned short, static_cast<__bf16>(f));", "return hip_threads_to_bf16(f);", 1),
+]
+
+
 # Two sources hold lines that the host compiler cannot parse; the host build compiles copies in
 # which exactly these are replaced and not a character else.  (old, new, count): a literal that
 # must be found `count` times (None: at least once); a compiled pattern replaces every match.
@@ -53,6 +61,8 @@ EDITS = {
         ("return __builtin_bit_cast(unsigned short, static_cast<__bf16>(f));", "return hip_threads_to_bf16(f);", 1),
         ("extern __shared__ __attribute__((aligned(16))) unsigned char smem[];", "HIP_DYNAMIC_SHARED(unsigned char, smem)", None),
     ],
+    "token_logprobs": [],
+    "distillation": [],
     "mi_fast": [
         # the first half of a forward chain step (twice: natural and base-2 logarithms)
         ("""  asm volatile(
@@ -98,7 +108,11 @@ EDITS = {
 
 def _edited_source(name):
     text = open(os.path.join(CSRC, name + ".hip")).read()
-    for old, new, count in EDITS[name]:
+    edits = EDITS[name]
+    if '#include "token_rows.h"' in text:
+        text = text.replace('#include "token_rows.h"', open(os.path.join(CSRC, "token_rows.h")).read())
+        edits = edits + TOKEN_ROWS_EDITS
+    for old, new, count in edits:
         if isinstance(old, str):
             found = text.count(old)
             text = text.replace(old, new)
