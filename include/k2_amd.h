@@ -436,20 +436,23 @@ K2AMD_API int k2amd_lattice_fill(const int32_t *ranges, const int32_t *frames,
  * No counterpart in the reference.  `logits`: `rows` rows of C elements (dtype K2AMD_F32, K2AMD_F16 or K2AMD_BF16), row r
  * at element r * row_stride, any alignment of the element type; p = softmax(x / temperature) of a row x, temperature > 0.
  * `mask` [rows] (one byte a row, 0: the row does not count and is not read) or NULL.  Sums are held in 32 bits or more;
- * results do not depend on the order in which workgroups run.  Served up to 2^24 - 1 rows a call.
+ * results do not depend on the order in which workgroups run.  Served: fewer than 2^31 rows of up to 2^22 columns.
  *
  * Log-probs of n given tokens a row (tokens [rows][n] int64; a negative one counts as absent and has log-prob 0, one past
  * the vocabulary gives NaN), the entropy (or NULL) and the k largest logits in falling order, the lower index first where
  * they are equal: top_logprobs [rows][k], top_tokens [rows][k] int64 (-inf and -1 past the C-th).  n and k <= 64.
  * Rows that do not count get 0, 0, -inf and -1.  A row of nothing but -inf has p = 0, entropy 0 and log-probs -inf.
- * stats [rows][2] (or NULL) and entropy are what the backward call reads.
+ * stats [rows][2] (or NULL) and entropy are what the backward call reads.  Rows that a workgroup cannot hold are cut into
+ * parts; scratch: device memory of at least k2amd_token_logprobs_scratch_bytes(...) (0 for most calls, then NULL will do;
+ * nothing in it has to survive the call).
  *
  * Backward: logits_grad [rows][C] (dense, of the logits' type) from what reaches the three results (each may be NULL).
  * A token listed twice takes both gradients. */
+K2AMD_API size_t k2amd_token_logprobs_scratch_bytes(long long rows, int C, int k, int dtype);
 K2AMD_API int k2amd_token_logprobs_forward(const void *logits, long long row_stride, const int64_t *tokens,
                                            const uint8_t *mask, float *logprobs, float *entropy, float *top_logprobs,
                                            int64_t *top_tokens, float *stats, long long rows, int C, int n, int k,
-                                           float temperature, int dtype, void *stream);
+                                           float temperature, int dtype, void *scratch, size_t scratch_bytes, void *stream);
 K2AMD_API int k2amd_token_logprobs_backward(const void *logits, long long row_stride, const int64_t *tokens,
                                             const uint8_t *mask, const float *stats, const float *entropy,
                                             const int64_t *top_tokens, const float *logprobs_grad,

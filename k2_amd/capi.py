@@ -73,7 +73,8 @@ _SIGNATURES = {
     "k2amd_rnnt_prune_gather_backward": ([_vp] * 3 + [_ci] * 6 + [_vp], _ci),
     "k2amd_lattice_count": ([_vp] * 6 + [_ci] * 3 + [_vp], _ci),
     "k2amd_lattice_fill": ([_vp] * 11 + [_ci] * 6 + [_vp], _ci),
-    "k2amd_token_logprobs_forward": ([_vp, _ll] + [_vp] * 7 + [_ll] + [_ci] * 3 + [_cf, _ci, _vp], _ci),
+    "k2amd_token_logprobs_scratch_bytes": ([_ll] + [_ci] * 3, _sz),
+    "k2amd_token_logprobs_forward": ([_vp, _ll] + [_vp] * 7 + [_ll] + [_ci] * 3 + [_cf, _ci, _vp, _sz, _vp], _ci),
     "k2amd_token_logprobs_backward": ([_vp, _ll] + [_vp] * 9 + [_ll] + [_ci] * 3 + [_cf, _ci, _vp], _ci),
     "k2amd_distillation_forward": ([_vp, _ll] + [_vp] * 5 + [_ll] + [_ci] * 3 + [_cf, _ci, _vp], _ci),
     "k2amd_distillation_backward": ([_vp, _ll] + [_vp] * 4 + [_ll, _vp, _cf, _vp, _ll] + [_ci] * 3 + [_cf, _ci, _vp], _ci),
@@ -845,10 +846,12 @@ def token_logprobs_forward(logits, tokens, mask, temperature, num_top, return_en
     top_logprobs = torch.empty(lead + (num_top,), dtype=torch.float32, device=dev) if num_top else None
     top_tokens = torch.empty(lead + (num_top,), dtype=torch.int64, device=dev) if num_top else None
     stats = torch.empty(lead + (2,), dtype=torch.float32, device=dev) if keep else None
+    nbytes = lib().k2amd_token_logprobs_scratch_bytes(rows, C, num_top, dt)
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     with torch.cuda.device(dev):
         check(lib().k2amd_token_logprobs_forward(
             x.data_ptr(), stride, ptr(tokens), ptr(mask), ptr(logprobs), ptr(entropy), ptr(top_logprobs), ptr(top_tokens),
-            ptr(stats), rows, C, n, num_top, temperature, dt, stream_ptr(dev)))
+            ptr(stats), rows, C, n, num_top, temperature, dt, ptr(scratch), nbytes, stream_ptr(dev)))
     return logprobs, entropy, top_logprobs, top_tokens, stats
 
 

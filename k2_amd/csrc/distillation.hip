@@ -306,7 +306,7 @@ int k2amd_distillation_forward(const void *logits, long long row_stride, const f
                                const int64_t *top_tokens, const uint8_t *mask, float *row_losses, float *records,
                                long long rows, int C, int K, int rest, float temperature, int dtype, void *stream) {
   if (!RowsOk(rows, row_stride, C, temperature, dtype) || K < 0) return K2AMD_ERR_INVALID_ARGUMENT;
-  if (!RowsServed(rows) || K > kMaxTeacher) return K2AMD_ERR_UNSUPPORTED;
+  if (!RowsServed(rows, C) || K > kMaxTeacher) return K2AMD_ERR_UNSUPPORTED;
   if (rows == 0) return K2AMD_OK;
   if (logits == nullptr || row_losses == nullptr || (K > 0 && (top_logprobs == nullptr || top_tokens == nullptr)))
     return K2AMD_ERR_INVALID_ARGUMENT;
@@ -323,7 +323,7 @@ int k2amd_distillation_backward(const void *logits, long long row_stride, const 
                                 void *logits_grad, long long rows, int C, int K, int rest, float temperature, int dtype,
                                 void *stream) {
   if (!RowsOk(rows, row_stride, C, temperature, dtype) || K < 0 || rows_per_loss < 1) return K2AMD_ERR_INVALID_ARGUMENT;
-  if (!RowsServed(rows) || K > kMaxTeacher) return K2AMD_ERR_UNSUPPORTED;
+  if (!RowsServed(rows, C) || K > kMaxTeacher) return K2AMD_ERR_UNSUPPORTED;
   if (rows == 0) return K2AMD_OK;
   if (logits == nullptr || records == nullptr || loss_grad == nullptr || logits_grad == nullptr ||
       (K > 0 && (top_logprobs == nullptr || top_tokens == nullptr)))

@@ -954,13 +954,17 @@ std::tuple<OptionalTensor, OptionalTensor, OptionalTensor, OptionalTensor, Optio
     top_tokens = torch::empty(r.Shape(num_top), r.Floats().dtype(torch::kLong));
   }
   if (keep) stats = torch::empty(r.Shape(2), r.Floats());
+  const size_t bytes = k2amd_token_logprobs_scratch_bytes(r.rows, Int(r.C), Int(num_top), r.dtype);
+  torch::Tensor scratch;
+  if (bytes > 0) scratch = torch::empty({static_cast<int64_t>(bytes)}, r.x.options().dtype(torch::kUInt8));
   void *stream = StreamOf(logits);
   {
     pybind11::gil_scoped_release release;
     Check(k2amd_token_logprobs_forward(r.x.data_ptr(), r.stride, I64(tokens), MaskPtr(mask), FloatPtr(logprobs),
                                        FloatPtr(entropy), FloatPtr(top_logprobs),
                                        Given(top_tokens) ? top_tokens->data_ptr<int64_t>() : nullptr, FloatPtr(stats), r.rows,
-                                       Int(r.C), Int(n), Int(num_top), static_cast<float>(temperature), r.dtype, stream));
+                                       Int(r.C), Int(n), Int(num_top), static_cast<float>(temperature), r.dtype,
+                                       bytes > 0 ? scratch.data_ptr() : nullptr, bytes, stream));
   }
   return std::make_tuple(logprobs, entropy, top_logprobs, top_tokens, stats);
 }

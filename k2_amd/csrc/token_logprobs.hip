@@ -10,171 +10,550 @@
 namespace k2amd {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kWaves = kThreads / kWave;
+// ---- alternatives ---------------------------------------------------------------------------------
+//
+// The k largest of the elements that wavefronts hold in registers, without sorting them.  A lane's elements form up to four
+// groups; a bisection over the groups' maxima finds a logit that at least k groups reach, by counting ballots (a comparison
+// and scalar work for each step), so at least k elements reach it, and hardly more in data that is not made of ties: the
+// groups with two of the k largest are few.  These elements go to LDS as whole numbers that carry value and index, and each
+// one's place is the number of larger ones.  Where more than kListed reach the threshold (rows of equal logits, a mask
+// that leaves a handful of tokens in front of thousands of -inf) or a NaN is among them, the wavefront lists its k
+// largest class by class instead: the largest value, all its occurrences in the order of the index, the next value.
+constexpr int kListed = 128;  // elements that a wavefront lists
 
-__device__ __forceinline__ float BlockMax(float v, float *lds) {
-  v = WaveMaxF(v);
-  __syncthreads();
-  if ((threadIdx.x & (kWave - 1)) == 0) lds[threadIdx.x / kWave] = v;
-  __syncthreads();
-  for (int w = 0; w < kWaves; ++w) v = fmaxf(v, lds[w]);
-  return v;
-}
-__device__ __forceinline__ float BlockSum(float v, float *lds) {
-  v = WaveSumF(v);
-  __syncthreads();
-  if ((threadIdx.x & (kWave - 1)) == 0) lds[threadIdx.x / kWave] = v;
-  __syncthreads();
-  v = 0;
-  for (int w = 0; w < kWaves; ++w) v += lds[w];
-  return v;
-}
-__device__ __forceinline__ unsigned long long BlockMaxKey(unsigned long long v, unsigned long long *lds) {
+template <int G>
+__device__ __forceinline__ int GroupsReaching(const float (&group)[G], float v) {
+  int n = 0;
 #pragma unroll
-  for (int off = 32; off > 0; off >>= 1) v = max(v, __shfl_xor(v, off, kWave));
-  __syncthreads();
-  if ((threadIdx.x & (kWave - 1)) == 0) lds[threadIdx.x / kWave] = v;
-  __syncthreads();
-  for (int w = 0; w < kWaves; ++w) v = max(v, lds[w]);
-  return v;
+  for (int g = 0; g < G; ++g) n += __popcll(__ballot(group[g] >= v));
+  return n;
 }
 
-// One workgroup a row: a pass for the maximum, one for the sums, one for each alternative.
-template <typename T>
-__global__ __launch_bounds__(kThreads) void TokenForwardKernel(
-    const T *__restrict__ logits, long long row_stride, const int64_t *__restrict__ tokens,
-    const uint8_t *__restrict__ mask, float *__restrict__ logprobs, float *__restrict__ entropy,
-    float *__restrict__ top_logprobs, int64_t *__restrict__ top_tokens, float *__restrict__ stats, int C, int n, int k,
-    float c, float inv_tau) {
-  __shared__ float lds[kWaves];
-  __shared__ unsigned long long lds_key[kWaves];
-  const size_t row = blockIdx.x;
-  const int tid = threadIdx.x;
-  if (mask != nullptr && mask[row] == 0) {
-    if (tid < n) logprobs[row * n + tid] = 0.0f;
-    if (tid < k) {
-      top_logprobs[row * k + tid] = Real<float>::NegInf();
-      top_tokens[row * k + tid] = -1;
-    }
-    if (tid == 0 && entropy != nullptr) entropy[row] = 0.0f;
-    if (tid == 0 && stats != nullptr) stats[2 * row] = stats[2 * row + 1] = 0.0f;
-    return;
-  }
-  const T *x = logits + row * row_stride;
-  float m = Real<float>::NegInf();
-  for (int i = tid; i < C; i += kThreads) m = fmaxf(m, ToFloat(x[i]));
-  m = BlockMax(m, lds);
-  if (m == Real<float>::NegInf()) m = 0.0f;
-  float s = 0.0f, t = 0.0f;
-  for (int i = tid; i < C; i += kThreads) {
-    const float d = (ToFloat(x[i]) - m) * c, e = Exp2(d);
-    s += e;
-    t += fmaxf(d, kNothing) * e;
-  }
-  s = BlockSum(s, lds);
-  t = BlockSum(t, lds);
-  const float ls = Log2(s);
-  if (tid < n) {
-    const int64_t token = tokens[row * n + tid];
-    float lp = 0.0f;
-    if (token >= C) lp = __uint_as_float(0x7fc00000u);
-    else if (token >= 0) lp = LogProb(ToFloat(x[token]), m, ls, inv_tau);
-    logprobs[row * n + tid] = lp;
-  }
-  if (tid == 0 && entropy != nullptr) entropy[row] = s == 0.0f ? 0.0f : kLn2 * (ls - t / s);
-  if (tid == 0 && stats != nullptr) {
-    stats[2 * row] = m;
-    stats[2 * row + 1] = ls;
-  }
-  unsigned long long last = ~0ull;
-  for (int j = 0; j < k; ++j) {
-    unsigned long long best = 0;
-    for (int i = tid; i < C; i += kThreads) {
-      const unsigned long long key = KeyOf(ToFloat(x[i]), (unsigned)i);
-      if (key < last) best = max(best, key);
-    }
-    last = BlockMaxKey(best, lds_key);
-    if (tid == 0) {
-      const bool some = last != 0;
-      top_logprobs[row * k + j] = some ? LogProb(ToFloat(x[IndexOf(last)]), m, ls, inv_tau) : Real<float>::NegInf();
-      top_tokens[row * k + j] = some ? (int64_t)IndexOf(last) : -1;
+// A value that at least k of the groups' maxima reach (-inf if no larger one was found), the largest of them being `high`;
+// `from`: one that is known to be reached by k.
+template <int G>
+__device__ __forceinline__ float Threshold(const float (&group)[G], float high, int k, float from) {
+  if (GroupsReaching(group, high) >= k) return high;
+  float lo = from, hi = high;
+  if (lo == Real<float>::NegInf()) {
+    // steps of 8, 64, 4096: most rows' k-th largest lies within 8 of the largest
+    lo = high - 8.0f;
+    if (GroupsReaching(group, lo) < k) {
+      hi = lo;
+      lo = high - 64.0f;
+      if (GroupsReaching(group, lo) < k) {
+        hi = lo;
+        lo = high - 4096.0f;
+        if (!(GroupsReaching(group, lo) >= k)) return Real<float>::NegInf();
+      }
     }
   }
-}
-
-// One workgroup a row: the softmax part of every element, then the entries' own elements over it.
-template <typename T>
-__global__ __launch_bounds__(kThreads) void TokenBackwardKernel(
-    const T *__restrict__ logits, long long row_stride, const int64_t *__restrict__ tokens,
-    const uint8_t *__restrict__ mask, const float *__restrict__ stats, const float *__restrict__ entropy,
-    const int64_t *__restrict__ top_tokens, const float *__restrict__ logprobs_grad,
-    const float *__restrict__ entropy_grad, const float *__restrict__ top_grad, T *__restrict__ logits_grad, int C, int n,
-    int k, float c, float inv_tau) {
-  __shared__ int entry[kMaxTokens + kMaxTop];
-  __shared__ float entry_grad[kMaxTokens + kMaxTop];
-  __shared__ float lds[kWaves];
-  const size_t row = blockIdx.x;
-  const int tid = threadIdx.x;
-  T *dx = logits_grad + row * C;
-  if (mask != nullptr && mask[row] == 0) {
-    for (int i = tid; i < C; i += kThreads) FromFloat(0.0f, &dx[i]);
-    return;
-  }
-  const T *x = logits + row * row_stride;
-  const int used = (logprobs_grad != nullptr ? n : 0), both = used + (top_grad != nullptr ? k : 0);
-  float g = 0.0f;
-  if (tid < both) {
-    int64_t token;
-    if (tid < used) {
-      token = tokens[row * n + tid];
-      g = logprobs_grad[row * n + tid];
+  for (int step = 0; step < 24; ++step) {
+    const float mid = 0.5f * (lo + hi);
+    const int n = GroupsReaching(group, mid);
+    if (n >= k) {
+      lo = mid;
+      if (n <= k + (k >> 1) + 2) break;
     } else {
-      token = top_tokens[row * k + (tid - used)];
-      g = top_grad[row * k + (tid - used)];
+      hi = mid;
     }
-    if (token < 0) g = 0.0f;
-    if (token >= C) g = __uint_as_float(0x7fc00000u);
-    entry[tid] = token < 0 || token >= C ? -1 : (int)token;
-    entry_grad[tid] = g;
   }
-  const float sum = BlockSum(g, lds);
-  const float m = stats[2 * row], ls = stats[2 * row + 1];
-  const float h = entropy_grad != nullptr ? entropy[row] : 0.0f, gh = entropy_grad != nullptr ? entropy_grad[row] : 0.0f;
-  const float none = ls == Real<float>::NegInf() ? 0.0f : 1.0f;  // a row without any mass: every p is 0
-  auto softmax_part = [&](float xi) {
-    const float d = fmaxf((xi - m) * c, kNothing) - (none != 0.0f ? ls : 0.0f);
-    const float p = none * Exp2(d);
-    return -p * (sum + gh * (kLn2 * d + h));
-  };
-  for (int i = tid; i < C; i += kThreads) FromFloat(softmax_part(ToFloat(x[i])) * inv_tau, &dx[i]);
-  __syncthreads();
-  if (tid < both && entry[tid] >= 0) {
-    float own = 0.0f;
-    for (int j = 0; j < both; ++j)
-      if (entry[j] == entry[tid]) own += entry_grad[j];
-    FromFloat((softmax_part(ToFloat(x[entry[tid]])) + own) * inv_tau, &dx[entry[tid]]);
+  return lo;
+}
+
+// Lists the wavefront's elements that reach `threshold`; returns how many there are (only kListed of them are listed).
+template <typename T, int U, int W>
+__device__ __forceinline__ int ListReaching(RowPart<T, U, W> &part, int C, int first, int wave, int lane, float threshold,
+                                            unsigned long long *list) {
+  constexpr int kN = Lanes<T>::kN;
+  int count = 0;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const Vec &v = part.Packed(u);
+    float x[kN], high = Real<float>::NegInf();
+#pragma unroll
+    for (int e = 0; e < kN; ++e) {
+      x[e] = ElementOf<T>(v, e);
+      high = fmaxf(high, x[e]);
+    }
+    if (__ballot(high >= threshold) == 0) continue;
+    const int q = part.VectorAnew(u, first, wave, lane), base = VecBase<T>(q, C);
+#pragma unroll
+    for (int e = 0; e < kN; ++e) {
+      if (__ballot(x[e] >= threshold) == 0) continue;
+      const int index = base + e;
+      const bool mine = x[e] >= threshold && index >= q * kN && index < C;  // (the -inf that pads a row is no element of it)
+      const unsigned long long lanes = __ballot(mine);
+      const int at = count + (int)BelowLane(lanes);
+      if (mine && at < kListed) list[at] = KeyOf(x[e], (unsigned)index);
+      count += __popcll(lanes);
+    }
+  }
+  return count;
+}
+
+// Lists the wavefront's k largest elements (k <= kMaxTop) class by class of equal ones; returns how many.
+template <typename T, int U, int W>
+__device__ __forceinline__ int ListByClasses(RowPart<T, U, W> &part, int C, int first, int wave, int lane, int k,
+                                             unsigned long long *list) {
+  constexpr int kN = Lanes<T>::kN;
+  int count = 0;
+  float last = 0.0f;
+  for (int round = 0; count < k; ++round) {
+    // the first class: the NaNs; the second: the largest; then the largest below the last
+    float high = Real<float>::NegInf();
+      if (round > 0) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const Vec &v = part.Packed(u);
+#pragma unroll
+        for (int e = 0; e < kN; ++e) {
+          const float x = ElementOf<T>(v, e);
+          if (round == 1 || x < last) high = fmaxf(high, x);
+        }
+      }
+      high = WaveMaxF(high);
+        }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (count >= k) continue;
+      const int q = part.VectorAnew(u, first, wave, lane), base = VecBase<T>(q, C);
+      const Vec &v = part.Packed(u);
+      unsigned bits = 0;
+#pragma unroll
+      for (int e = 0; e < kN; ++e) {
+        const float x = ElementOf<T>(v, e);
+        if ((round == 0 ? x != x : x == high) && base + e >= q * kN && base + e < C) bits |= 1u << e;
+      }
+      if (__ballot(bits != 0) == 0) continue;
+      unsigned long long total = 0;
+      int at = count, here = 0;
+#pragma unroll
+      for (int e = 0; e < kN; ++e) {  // elements in front of this lane's, in the order of the index
+        const unsigned long long lanes = __ballot((bits >> e & 1u) != 0);
+        at += (int)BelowLane(lanes);
+        total += __popcll(lanes);
+      }
+#pragma unroll
+      for (int e = 0; e < kN; ++e)
+        if (bits >> e & 1u) {
+          if (at + here < k) list[at + here] = KeyOf(ElementOf<T>(v, e), (unsigned)(base + e));
+          ++here;
+        }
+      count = min(k, count + (int)total);
+    }
+    if (round > 0 && high == Real<float>::NegInf()) break;  // nothing is below
+    last = high;
+  }
+  return count;
+}
+
+// ---- forward ----------------------------------------------------------------------------------------
+
+struct ForwardArgs {
+  long long row_stride;
+  const int64_t *tokens;
+  const uint8_t *mask;
+  float *logprobs, *entropy, *top_logprobs;
+  int64_t *top_tokens;
+  float *stats;
+  int C, n, k;
+  float c, inv_tau;
+  // rows in several parts: [rows][parts] sums and [rows][parts][k] keys, the largest first, 0 past the last
+  int parts;
+  float4 *part_sums;
+  unsigned long long *part_keys;
+};
+
+__device__ __forceinline__ void WriteSkippedRow(const ForwardArgs &a, size_t row, int i) {
+  if (i < a.n) a.logprobs[row * a.n + i] = 0.0f;
+  if (i < a.k) {
+    a.top_logprobs[row * a.k + i] = Real<float>::NegInf();
+    a.top_tokens[row * a.k + i] = -1;
+  }
+  if (i == 0 && a.entropy != nullptr) a.entropy[row] = 0.0f;
+  if (i == 0 && a.stats != nullptr) a.stats[2 * row] = a.stats[2 * row + 1] = 0.0f;
+}
+
+// What a row's sums say, by the first 64 work-items; x_token: the logit of work-item i's token.
+__device__ __forceinline__ void WriteRow(const ForwardArgs &a, size_t row, int i, const Sums &sums, int64_t token,
+                                         float x_token) {
+  const float ls = Log2(sums.s);
+  if (i < a.n) {
+    float lp = 0.0f;
+    if (token >= a.C) lp = __uint_as_float(0x7fc00000u);
+    else if (token >= 0) lp = LogProb(x_token, sums.m, ls, a.inv_tau);
+    a.logprobs[row * a.n + i] = lp;
+  }
+  if (i == 0 && a.entropy != nullptr) a.entropy[row] = sums.s == 0.0f ? 0.0f : kLn2 * (ls - sums.t / sums.s);
+  if (i == 0 && a.stats != nullptr) {
+    a.stats[2 * row] = sums.m;
+    a.stats[2 * row + 1] = sums.s;
   }
 }
 
+// W wavefronts a row (or a part of it), W == 1: four rows a workgroup.  kEntropy: whether t is summed up.
+template <typename T, int U, int W, bool kEntropy>
+__global__ __launch_bounds__(W == 1 ? 4 * kWave : W *kWave) void TokenForwardKernel(const T *__restrict__ logits,
+                                                                                   long long row0, long long rows,
+                                                                                   ForwardArgs a) {
+  constexpr int kN = Lanes<T>::kN, kWaves = W == 1 ? 4 : W;
+  __shared__ unsigned long long lists[kWaves][kListed];
+  __shared__ float4 wave_sums[kWaves];      // of W > 1 wavefronts: m, s, t, the threshold that k of its groups reach
+  __shared__ float wave_low[kWaves];        // and the one that its share of k reach
+  __shared__ int listed[kWaves];
+  const int lane = threadIdx.x & (kWave - 1);
+  const int in_block = __builtin_amdgcn_readfirstlane((int)(threadIdx.x / kWave));
+  const int wave = W == 1 ? 0 : in_block;   // of the row
+  const size_t row = row0 + (W == 1 ? (long long)blockIdx.x * 4 + in_block : (long long)blockIdx.x);
+  if (W == 1 && (long long)row >= row0 + rows) return;
+  const int first = W == 1 ? 0 : (int)blockIdx.y * (U * W * kWave);
+  if (a.mask != nullptr && a.mask[row] == 0) {
+    if (wave == 0 && blockIdx.y == 0) WriteSkippedRow(a, row, lane);
+    return;
+  }
+  const T *x = logits + row * a.row_stride;
+  RowPart<T, U, W> part;
+  part.Load(x, a.C, first, wave, lane);
+  int64_t token = -1;
+  float x_token = 0.0f;
+  if (wave == 0 && a.parts == 1 && lane < a.n) {
+    token = a.tokens[row * a.n + lane];
+    if (token >= 0 && token < a.C) x_token = ToFloat(x[token]);
+  }
+
+  // the wavefront's sums
+  constexpr int kGroups = U < 4 ? U : 4;
+  float group[kGroups];
+#pragma unroll
+  for (int g = 0; g < kGroups; ++g) group[g] = Real<float>::NegInf();
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const Vec &v = part.Packed(u);
+#pragma unroll
+    for (int e = 0; e < kN; ++e) group[u % kGroups] = fmaxf(group[u % kGroups], ElementOf<T>(v, e));
+  }
+  float high = group[0];
+#pragma unroll
+  for (int g = 1; g < kGroups; ++g) high = fmaxf(high, group[g]);
+  high = WaveMaxF(high);
+  Sums sums;
+  sums.m = high == Real<float>::NegInf() ? 0.0f : high;
+  float s[4] = {0, 0, 0, 0}, t[4] = {0, 0, 0, 0};
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const Vec &v = part.Packed(u);
+#pragma unroll
+    for (int e = 0; e < kN; ++e) {
+      const float d = (ElementOf<T>(v, e) - sums.m) * a.c, p = Exp2(d);
+      s[e & 3] += p;
+      if (kEntropy) t[e & 3] += fmaxf(d, kNothing) * p;
+    }
+  }
+  sums.s = WaveSumF((s[0] + s[1]) + (s[2] + s[3]));
+  sums.t = kEntropy ? WaveSumF((t[0] + t[1]) + (t[2] + t[3])) : 0.0f;
+
+  const bool odd = sums.s != sums.s;  // a NaN or +inf among them
+  float threshold = Real<float>::NegInf();
+  if (a.k > 0 && !odd) threshold = Threshold<kGroups>(group, high, a.k, threshold);
+  if (W > 1) {
+    const float low = a.k > 0 && !odd ? Threshold<kGroups>(group, high, (a.k + W - 1) / W, threshold) : threshold;
+    if (lane == 0) {
+      wave_sums[wave] = make_float4(sums.m, sums.s, sums.t, threshold);
+      wave_low[wave] = low;
+    }
+    __syncthreads();
+    // k elements of the part reach every wavefront's own threshold, and the lowest of those that k / W reach in each
+    float lowest = wave_low[0];
+    threshold = Real<float>::NegInf();
+    for (int w = 0; w < W; ++w) {
+      threshold = fmaxf(threshold, wave_sums[w].w);
+      lowest = fminf(lowest, wave_low[w]);
+    }
+    threshold = fmaxf(threshold, lowest);
+    sums = Sums{wave_sums[0].x, wave_sums[0].y, wave_sums[0].z};
+    for (int w = 1; w < W; ++w) sums = Join(sums, Sums{wave_sums[w].x, wave_sums[w].y, wave_sums[w].z}, a.c);
+  }
+  if (wave == 0) {
+    if (a.parts == 1) WriteRow(a, row, lane, sums, token, x_token);
+    else if (lane == 0) a.part_sums[row * a.parts + blockIdx.y] = make_float4(sums.m, sums.s, sums.t, 0.0f);
+  }
+  if (a.k == 0) return;
+
+  unsigned long long *own = lists[in_block];
+  int count = odd ? kListed + 1 : ListReaching<T, U, W>(part, a.C, first, wave, lane, threshold, own);
+  if (count > kListed)
+    count = ListByClasses<T, U, W>(part, a.C, first, wave, lane, a.k, own);
+  if (W > 1) {
+    if (lane == 0) listed[wave] = count;
+    __syncthreads();
+  } else {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  }
+  // each listed element's place
+  const float ls = Log2(sums.s);
+  int all = 0;
+  for (int w = 0; w < W; ++w) all += W == 1 ? count : listed[w];
+  for (int i = lane; i < count; i += kWave) {
+    const unsigned long long key = own[i];
+    int place = 0;
+    for (int w = 0; w < W; ++w) {
+      const unsigned long long *other = W == 1 ? own : lists[w];
+      const int n = W == 1 ? count : listed[w];
+      for (int j = 0; j < n; ++j) place += other[j] > key ? 1 : 0;
+    }
+    if (place < a.k) {
+      if (a.parts == 1) {
+        a.top_tokens[row * a.k + place] = IndexOf(key);
+        a.top_logprobs[row * a.k + place] = LogProb(LogitOf(key), sums.m, ls, a.inv_tau);
+      } else {
+        a.part_keys[(row * a.parts + blockIdx.y) * a.k + place] = key;
+      }
+    }
+  }
+  if (wave == 0 && lane < a.k && lane >= all) {  // rows shorter than the list
+    if (a.parts == 1) {
+      a.top_tokens[row * a.k + lane] = -1;
+      a.top_logprobs[row * a.k + lane] = Real<float>::NegInf();
+    } else {
+      a.part_keys[(row * a.parts + blockIdx.y) * a.k + lane] = 0;
+    }
+  }
+}
+
+// Joins the parts of a row: a workgroup a row.  The keys of a part are in order, so a key's place among all is its place in
+// its own part and, in every other part, the number of larger ones, by bisection.
+constexpr int kJoinThreads = 256;
 template <typename T>
-int Forward(const void *logits, long long row_stride, const int64_t *tokens, const uint8_t *mask, float *logprobs,
-            float *entropy, float *top_logprobs, int64_t *top_tokens, float *stats, long long rows, int C, int n, int k,
-            float temperature, hipStream_t stream) {
-  hipLaunchKernelGGL((TokenForwardKernel<T>), dim3((unsigned)rows), dim3(kThreads), 0, stream, (const T *)logits, row_stride,
-                     tokens, mask, logprobs, entropy, top_logprobs, top_tokens, stats, C, n, k,
-                     (float)(kLog2E / (double)temperature), (float)(1.0 / (double)temperature));
+__global__ __launch_bounds__(kJoinThreads) void TokenJoinKernel(const T *__restrict__ logits, long long row0, ForwardArgs a) {
+  HIP_DYNAMIC_SHARED(unsigned long long, keys)
+  const size_t row = row0 + blockIdx.x;
+  if (a.mask != nullptr && a.mask[row] == 0) return;
+  Sums sums{0, 0, 0};
+  for (int p = 0; p < a.parts; ++p) {
+    const float4 v = a.part_sums[row * a.parts + p];
+    sums = p == 0 ? Sums{v.x, v.y, v.z} : Join(sums, Sums{v.x, v.y, v.z}, a.c);
+  }
+  const int i = threadIdx.x;
+  if (i < kWave) {
+    int64_t token = -1;
+    float x_token = 0.0f;
+    if (i < a.n) {
+      token = a.tokens[row * a.n + i];
+      if (token >= 0 && token < a.C) x_token = ToFloat(logits[row * a.row_stride + token]);
+    }
+    WriteRow(a, row, i, sums, token, x_token);
+  }
+  if (a.k == 0) return;
+  const int all = a.parts * a.k;
+  for (int j = i; j < all; j += kJoinThreads) keys[j] = a.part_keys[row * all + j];
+  __syncthreads();
+  const float ls = Log2(sums.s);
+  for (int j = i; j < all; j += kJoinThreads) {
+    const unsigned long long key = keys[j];
+    const int part = j / a.k;
+    int place = j - part * a.k;
+    if (key == 0) {  // past the last of its part: behind every key, in the order of the parts' ends
+      for (int p = 0; p < a.parts; ++p) {
+        if (p == part) continue;
+        int lo = 0, hi = a.k;  // keys of p that are not 0
+        while (lo < hi) {
+          const int mid = (lo + hi) / 2;
+          if (keys[p * a.k + mid] != 0) lo = mid + 1;
+          else hi = mid;
+        }
+        place += p < part ? a.k : lo;
+      }
+      if (place < a.k) {
+        a.top_tokens[row * a.k + place] = -1;
+        a.top_logprobs[row * a.k + place] = Real<float>::NegInf();
+      }
+      continue;
+    }
+    for (int p = 0; p < a.parts; ++p) {
+      if (p == part) continue;
+      int lo = 0, hi = a.k;
+      while (lo < hi) {
+        const int mid = (lo + hi) / 2;
+        if (keys[p * a.k + mid] > key) lo = mid + 1;
+        else hi = mid;
+      }
+      place += lo;
+    }
+    if (place < a.k) {
+      a.top_tokens[row * a.k + place] = IndexOf(key);
+      a.top_logprobs[row * a.k + place] = LogProb(LogitOf(key), sums.m, ls, a.inv_tau);
+    }
+  }
+}
+
+// ---- backward ---------------------------------------------------------------------------------------
+
+struct BackwardArgs {
+  long long row_stride;
+  const int64_t *tokens;
+  const uint8_t *mask;
+  const float *stats, *entropy;
+  const int64_t *top_tokens;
+  const float *logprobs_grad, *entropy_grad, *top_grad;
+  int C, n, k;
+  float c, inv_tau;
+};
+
+// dx of an element that is no entry: -p (G + gH (log p + H)) / tau, with 1 / (s tau) in the coefficients
+struct SoftmaxGrad {
+  float m, c, flat, slope;
+  __device__ __forceinline__ float At(float x) const {
+    const float d = (x - m) * c;
+    return Exp2(d) * (flat + slope * fmaxf(d, kNothing));
+  }
+};
+
+// W wavefronts take U vectors a lane of a row, or of the stretch of it that blockIdx.y counts; W == 1: four rows a
+// workgroup, each in rounds of U.  The softmax part of every element first; then the entries' own elements over it.
+template <typename T, int U, int W>
+__global__ __launch_bounds__(W == 1 ? 4 * kWave : W *kWave) void TokenBackwardKernel(const T *__restrict__ logits,
+                                                                                    T *__restrict__ logits_grad, long long row0,
+                                                                                    long long rows, BackwardArgs a) {
+  constexpr int kN = Lanes<T>::kN, kWaves = W == 1 ? 4 : W;
+  constexpr int kEntries = kMaxTokens + kMaxTop;
+  __shared__ int entry_lds[kWaves][W == 1 ? kEntries : 1];
+  __shared__ float grad_lds[kWaves][W == 1 ? kEntries : 1];
+  __shared__ int block_entry[W == 1 ? 1 : kEntries];
+  __shared__ float block_grad[W == 1 ? 1 : kEntries];
+  const int lane = threadIdx.x & (kWave - 1);
+  const int in_block = __builtin_amdgcn_readfirstlane((int)(threadIdx.x / kWave));
+  const int wave = W == 1 ? 0 : in_block;
+  // the last row first: of a batch larger than the 256 MB memory-side cache it is the tail that the forward pass left there
+  const long long from_last = W == 1 ? (long long)blockIdx.x * 4 + in_block : (long long)blockIdx.x;
+  if (W == 1 && from_last >= rows) return;
+  const size_t row = row0 + rows - 1 - from_last;
+  const int first = W == 1 ? 0 : (int)blockIdx.y * (U * W * kWave);
+  T *dx = logits_grad + row * (size_t)a.C;
+  const int all = VecsOf<T>(a.C);
+  const bool live = a.mask == nullptr || a.mask[row] != 0;
+  const T *x = logits + row * a.row_stride;
+  RowPart<T, U, W> part;
+  SoftmaxGrad f{0.0f, 0.0f, 0.0f, 0.0f};
+  int *entry = W == 1 ? entry_lds[in_block] : block_entry;
+  float *entry_grad = W == 1 ? grad_lds[in_block] : block_grad;
+  const int used = a.logprobs_grad != nullptr ? a.n : 0, both = live ? used + (a.top_grad != nullptr ? a.k : 0) : 0;
+  if (live) {
+    part.Load(x, a.C, first, wave, lane);
+    float sum = 0.0f;
+    for (int i = lane; i < both; i += kWave) {  // (every wavefront of a row: all need the sum)
+      const bool given = i < used;
+      const int64_t token = given ? a.tokens[row * a.n + i] : a.top_tokens[row * a.k + (i - used)];
+      float g = given ? a.logprobs_grad[row * a.n + i] : a.top_grad[row * a.k + (i - used)];
+      if (token < 0) g = 0.0f;
+      if (token >= a.C) g = __uint_as_float(0x7fc00000u);
+      sum += g;
+      if (wave == 0) {
+        entry[i] = token < 0 || token >= a.C ? -1 : (int)token;
+        entry_grad[i] = g;
+      }
+    }
+    sum = both > 0 ? WaveSumF(sum) : 0.0f;
+    const float s = a.stats[2 * row + 1];
+    const float h = a.entropy_grad != nullptr ? a.entropy[row] : 0.0f;
+    const float gh = a.entropy_grad != nullptr ? a.entropy_grad[row] : 0.0f;
+    f.m = a.stats[2 * row];
+    f.c = a.c;
+    if (s != 0.0f) {  // (a row without any mass: every p is 0)
+      const float inv_s = a.inv_tau / s;
+      f.flat = -inv_s * (sum + gh * (h - kLn2 * Log2(s)));
+      f.slope = -inv_s * gh * kLn2;
+    } else if (sum != sum) {
+      f.flat = sum;
+    }
+  }
+  const int whole = a.C / kN;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int q = part.Vector(u, first, wave, lane);
+    if (q >= all) continue;
+    float g[kN];
+#pragma unroll
+    for (int e = 0; e < kN; ++e) g[e] = live ? f.At(ElementOf<T>(part.v[u], e)) : 0.0f;
+    if (q < whole) {
+      StoreVec(dx + (size_t)q * kN, PackOf<T>(g));
+    } else {  // the incomplete last vector, element by element
+      const int base = VecBase<T>(q, a.C);
+#pragma unroll
+      for (int e = 0; e < kN; ++e)
+        if (base + e >= q * kN && base + e < a.C) FromFloat(g[e], &dx[base + e]);
+    }
+  }
+  if (both == 0) return;
+  // (the stores above are before the ones below for every lane of the wavefront or workgroup)
+  if (W == 1) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  else __syncthreads();
+  const int begin = first * kN, end = min((long long)a.C, (long long)(first + U * W * kWave) * kN);
+  for (int i = W == 1 ? lane : (int)threadIdx.x; i < both; i += W * kWave) {
+    const int token = entry[i];
+    if (token < begin || token >= end) continue;
+    float own = 0.0f;  // a token that is listed twice takes both gradients
+    for (int j = 0; j < both; ++j)
+      if (entry[j] == token) own += entry_grad[j];
+    FromFloat(f.At(ToFloat(x[token])) + own * a.inv_tau, &dx[token]);
+  }
+}
+
+// ---- launches ---------------------------------------------------------------------------------------
+
+template <typename T, int U, int W>
+void LaunchForward(const T *logits, long long rows, bool entropy, const ForwardArgs &a, hipStream_t stream) {
+  for (long long row0 = 0; row0 < rows; row0 += kRowsPerLaunch) {
+    const long long n = rows - row0 < kRowsPerLaunch ? rows - row0 : kRowsPerLaunch;
+    const dim3 grid((unsigned)(W == 1 ? (n + 3) / 4 : n), (unsigned)a.parts), block(W == 1 ? 4 * kWave : W * kWave);
+    if (entropy) hipLaunchKernelGGL((TokenForwardKernel<T, U, W, true>), grid, block, 0, stream, logits, row0, n, a);
+    else hipLaunchKernelGGL((TokenForwardKernel<T, U, W, false>), grid, block, 0, stream, logits, row0, n, a);
+    if (a.parts > 1)
+      hipLaunchKernelGGL(TokenJoinKernel<T>, dim3((unsigned)n), dim3(kJoinThreads),
+                         (size_t)a.parts * a.k * sizeof(unsigned long long), stream, logits, row0, a);
+  }
+}
+
+// How many parts a row of C elements is held in: one workgroup of 16 wavefronts with 16 vectors a lane holds 16384 vectors.
+constexpr int kPartVecs = 16 * 16 * kWave;
+int PartsOf(int C, int dtype) {
+  const int vecs = dtype == K2AMD_F32 ? VecsOf<float>(C) : VecsOf<Half>(C);
+  return (vecs + kPartVecs - 1) / kPartVecs;
+}
+
+template <typename T>
+int Forward(const void *logits_v, long long rows, ForwardArgs a, hipStream_t stream) {
+  const T *logits = static_cast<const T *>(logits_v);
+  const int vecs = VecsOf<T>(a.C);
+  const bool entropy = a.entropy != nullptr;
+  if (vecs <= kWave) LaunchForward<T, 1, 1>(logits, rows, entropy, a, stream);
+  else if (vecs <= 2 * kWave) LaunchForward<T, 2, 1>(logits, rows, entropy, a, stream);
+  else if (vecs <= 4 * kWave) LaunchForward<T, 4, 1>(logits, rows, entropy, a, stream);
+  else if (vecs <= 16 * kWave) LaunchForward<T, 4, 4>(logits, rows, entropy, a, stream);
+  else if (vecs <= 64 * kWave) LaunchForward<T, 16, 4>(logits, rows, entropy, a, stream);
+  else LaunchForward<T, 16, 16>(logits, rows, entropy, a, stream);
   return LaunchStatus();
 }
 
+template <typename T, int U, int W>
+void LaunchBackward(const T *logits, T *logits_grad, long long rows, const BackwardArgs &a, hipStream_t stream) {
+  const int stretches = W == 1 ? 1 : (VecsOf<T>(a.C) + U * W * kWave - 1) / (U * W * kWave);
+  for (long long done = 0; done < rows; done += kRowsPerLaunch) {
+    const long long n = rows - done < kRowsPerLaunch ? rows - done : kRowsPerLaunch;
+    const dim3 grid((unsigned)(W == 1 ? (n + 3) / 4 : n), (unsigned)stretches), block(W == 1 ? 4 * kWave : W * kWave);
+    hipLaunchKernelGGL((TokenBackwardKernel<T, U, W>), grid, block, 0, stream, logits, logits_grad, rows - done - n, n, a);
+  }
+}
+
 template <typename T>
-int Backward(const void *logits, long long row_stride, const int64_t *tokens, const uint8_t *mask, const float *stats,
-             const float *entropy, const int64_t *top_tokens, const float *logprobs_grad, const float *entropy_grad,
-             const float *top_grad, void *logits_grad, long long rows, int C, int n, int k, float temperature,
-             hipStream_t stream) {
-  hipLaunchKernelGGL((TokenBackwardKernel<T>), dim3((unsigned)rows), dim3(kThreads), 0, stream, (const T *)logits, row_stride,
-                     tokens, mask, stats, entropy, top_tokens, logprobs_grad, entropy_grad, top_grad, (T *)logits_grad, C, n,
-                     k, (float)(kLog2E / (double)temperature), (float)(1.0 / (double)temperature));
+int Backward(const void *logits_v, void *grad_v, long long rows, const BackwardArgs &a, hipStream_t stream) {
+  const T *logits = static_cast<const T *>(logits_v);
+  T *grad = static_cast<T *>(grad_v);
+  const int vecs = VecsOf<T>(a.C);
+  if (vecs <= kWave) LaunchBackward<T, 1, 1>(logits, grad, rows, a, stream);
+  else if (vecs <= 2 * kWave) LaunchBackward<T, 2, 1>(logits, grad, rows, a, stream);
+  else if (vecs <= 4 * kWave) LaunchBackward<T, 4, 1>(logits, grad, rows, a, stream);
+  else LaunchBackward<T, 4, 4>(logits, grad, rows, a, stream);
   return LaunchStatus();
 }
 
@@ -185,21 +564,33 @@ using namespace k2amd;
 
 extern "C" {
 
+size_t k2amd_token_logprobs_scratch_bytes(long long rows, int C, int k, int dtype) {
+  if (rows < 0 || C < 1 || k < 0 || C > kMaxColumns || k > kMaxTop) return 0;
+  const size_t parts = PartsOf(C, dtype);
+  return parts <= 1 ? 0 : (size_t)rows * parts * (sizeof(float4) + (size_t)k * sizeof(unsigned long long));
+}
+
 int k2amd_token_logprobs_forward(const void *logits, long long row_stride, const int64_t *tokens, const uint8_t *mask,
                                  float *logprobs, float *entropy, float *top_logprobs, int64_t *top_tokens, float *stats,
-                                 long long rows, int C, int n, int k, float temperature, int dtype, void *stream) {
+                                 long long rows, int C, int n, int k, float temperature, int dtype, void *scratch,
+                                 size_t scratch_bytes, void *stream) {
   if (!RowsOk(rows, row_stride, C, temperature, dtype) || n < 0 || k < 0) return K2AMD_ERR_INVALID_ARGUMENT;
-  if (!RowsServed(rows) || n > kMaxTokens || k > kMaxTop) return K2AMD_ERR_UNSUPPORTED;
+  if (!RowsServed(rows, C) || n > kMaxTokens || k > kMaxTop) return K2AMD_ERR_UNSUPPORTED;
   if (rows == 0) return K2AMD_OK;
   if (logits == nullptr || (n > 0 && (tokens == nullptr || logprobs == nullptr)) ||
       (k > 0 && (top_logprobs == nullptr || top_tokens == nullptr)))
     return K2AMD_ERR_INVALID_ARGUMENT;
+  const int parts = PartsOf(C, dtype);
+  if (parts > 1 && (scratch == nullptr || scratch_bytes < k2amd_token_logprobs_scratch_bytes(rows, C, k, dtype)))
+    return K2AMD_ERR_WORKSPACE;
+  float4 *sums = static_cast<float4 *>(scratch);
+  const ForwardArgs a{row_stride, tokens, mask, logprobs, entropy, top_logprobs, top_tokens, stats, C, n, k,
+                      (float)(kLog2E / (double)temperature), (float)(1.0 / (double)temperature), parts, sums,
+                      parts > 1 ? reinterpret_cast<unsigned long long *>(sums + rows * parts) : nullptr};
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (dtype == K2AMD_F32)
-    return Forward<float>(logits, row_stride, tokens, mask, logprobs, entropy, top_logprobs, top_tokens, stats, rows, C, n, k, temperature, st);
-  if (dtype == K2AMD_F16)
-    return Forward<Half>(logits, row_stride, tokens, mask, logprobs, entropy, top_logprobs, top_tokens, stats, rows, C, n, k, temperature, st);
-  return Forward<Bfloat>(logits, row_stride, tokens, mask, logprobs, entropy, top_logprobs, top_tokens, stats, rows, C, n, k, temperature, st);
+  if (dtype == K2AMD_F32) return Forward<float>(logits, rows, a, st);
+  if (dtype == K2AMD_F16) return Forward<Half>(logits, rows, a, st);
+  return Forward<Bfloat>(logits, rows, a, st);
 }
 
 int k2amd_token_logprobs_backward(const void *logits, long long row_stride, const int64_t *tokens, const uint8_t *mask,
@@ -208,17 +599,17 @@ int k2amd_token_logprobs_backward(const void *logits, long long row_stride, cons
                                   void *logits_grad, long long rows, int C, int n, int k, float temperature, int dtype,
                                   void *stream) {
   if (!RowsOk(rows, row_stride, C, temperature, dtype) || n < 0 || k < 0) return K2AMD_ERR_INVALID_ARGUMENT;
-  if (!RowsServed(rows) || n > kMaxTokens || k > kMaxTop) return K2AMD_ERR_UNSUPPORTED;
+  if (!RowsServed(rows, C) || n > kMaxTokens || k > kMaxTop) return K2AMD_ERR_UNSUPPORTED;
   if (rows == 0) return K2AMD_OK;
   if (logits == nullptr || stats == nullptr || logits_grad == nullptr || (n > 0 && logprobs_grad != nullptr && tokens == nullptr) ||
       (k > 0 && top_grad != nullptr && top_tokens == nullptr) || (entropy_grad != nullptr && entropy == nullptr))
     return K2AMD_ERR_INVALID_ARGUMENT;
+  const BackwardArgs a{row_stride, tokens, mask, stats, entropy, top_tokens, logprobs_grad, entropy_grad, top_grad, C, n, k,
+                       (float)(kLog2E / (double)temperature), (float)(1.0 / (double)temperature)};
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (dtype == K2AMD_F32)
-    return Backward<float>(logits, row_stride, tokens, mask, stats, entropy, top_tokens, logprobs_grad, entropy_grad, top_grad, logits_grad, rows, C, n, k, temperature, st);
-  if (dtype == K2AMD_F16)
-    return Backward<Half>(logits, row_stride, tokens, mask, stats, entropy, top_tokens, logprobs_grad, entropy_grad, top_grad, logits_grad, rows, C, n, k, temperature, st);
-  return Backward<Bfloat>(logits, row_stride, tokens, mask, stats, entropy, top_tokens, logprobs_grad, entropy_grad, top_grad, logits_grad, rows, C, n, k, temperature, st);
+  if (dtype == K2AMD_F32) return Backward<float>(logits, logits_grad, rows, a, st);
+  if (dtype == K2AMD_F16) return Backward<Half>(logits, logits_grad, rows, a, st);
+  return Backward<Bfloat>(logits, logits_grad, rows, a, st);
 }
 
 }  // extern "C"

@@ -1,11 +1,17 @@
-// What the operators on rows of output logits share (token_logprobs.hip, distillation.hip): the three element types, and
-// the two numbers that a row's softmax is kept as.
+// What the operators on rows of output logits share (token_logprobs.hip, distillation.hip): the three element types, how a
+// wavefront holds its part of a row, and the two numbers that a row's softmax is kept as.
 //
 // A row of C logits x at temperature tau is kept as its largest logit m and log2 s, s = sum_i 2^d_i with
-// d_i = (x_i - m) c, c = log2(e) / tau; then log p_i = ln2 (d_i - log2 s).  The difference is formed in the logits' own
-// scale, before c multiplies it: it is exact or one rounding off for every pair of logits, and rows that a mask has filled
-// with the type's lowest value stay rows of equal logits (c x alone would overflow).  m is the row's largest logit, or 0
-// where that is -inf (a row that a mask left nothing of): then s = 0 and every p_i is 0.
+// d_i = (x_i - m) c, c = log2(e) / tau; then log p_i = (x_i - m) / tau - ln2 log2 s.  The difference is formed in the
+// logits' own scale, before c multiplies it: it is exact or one rounding off for every pair of logits, and rows that a mask
+// has filled with the type's lowest value stay rows of equal logits (c x alone would overflow).  m is the row's largest
+// logit, or 0 where that is -inf (a row that a mask left nothing of): then s = 0 and every p_i is 0.
+//
+// A row is read once, 16 bytes a lane at a time, and stays in registers: wavefront w of the W that share a row takes, in
+// round u of U, vector (u W + w) 64 + lane.  Rows start at any element: the loads are unaligned ones (a row of odd length
+// in 16 bits moves the start of every other row off the dword), which cost nothing measurable beside aligned ones here.
+// The last vector of a row whose length is no multiple of the vector's is read so that it ends with the row, and what the
+// vector in front of it holds already is set to -inf in it: no byte outside the row is read, without a loop over elements.
 #ifndef K2_AMD_CSRC_TOKEN_ROWS_H_
 #define K2_AMD_CSRC_TOKEN_ROWS_H_
 
@@ -21,6 +27,7 @@ constexpr float kNothing = -1024.0f;
 constexpr int kMaxTokens = 64;        // given tokens of a row
 constexpr int kMaxTop = 64;           // listed alternatives of a row
 constexpr int kMaxTeacher = 256;      // entries of a teacher's list
+constexpr int kMaxColumns = 1 << 22;  // columns of a row: 64 parts of the longest stretch that a workgroup holds
 
 // the bits of one 16-bit element and back (to nearest even)
 struct Half {
@@ -41,27 +48,180 @@ __device__ __forceinline__ unsigned short FloatToBfloat(float f) {
 __device__ __forceinline__ float ToFloat(float x) { return x; }
 __device__ __forceinline__ float ToFloat(Half x) { return HalfToFloat(x.bits); }
 __device__ __forceinline__ float ToFloat(Bfloat x) { return __uint_as_float((unsigned)x.bits << 16); }
+__device__ __forceinline__ unsigned Narrow(float f, const float *) { return __float_as_uint(f); }
+__device__ __forceinline__ unsigned Narrow(float f, const Half *) { return FloatToHalf(f); }
+__device__ __forceinline__ unsigned Narrow(float f, const Bfloat *) { return FloatToBfloat(f); }
 __device__ __forceinline__ void FromFloat(float f, float *x) { *x = f; }
 __device__ __forceinline__ void FromFloat(float f, Half *x) { x->bits = FloatToHalf(f); }
 __device__ __forceinline__ void FromFloat(float f, Bfloat *x) { x->bits = FloatToBfloat(f); }
 
+// 16 bytes of a row: four or eight elements
+struct Vec {
+  unsigned w[4];
+};
+template <typename T>
+struct Lanes {
+  static constexpr int kN = 16 / sizeof(T);
+  static constexpr unsigned kNegInf = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;
+};
+template <>
+struct Lanes<Half> {
+  static constexpr int kN = 8;
+  static constexpr unsigned kNegInf = 0xfc00fc00u;
+};
+__device__ __forceinline__ float Element(const Vec &v, int e, const float *) { return __uint_as_float(v.w[e]); }
+__device__ __forceinline__ float Element(const Vec &v, int e, const Half *) {
+  return HalfToFloat((unsigned short)(e & 1 ? v.w[e >> 1] >> 16 : v.w[e >> 1] & 0xffffu));
+}
+__device__ __forceinline__ float Element(const Vec &v, int e, const Bfloat *) {
+  return __uint_as_float(e & 1 ? v.w[e >> 1] & 0xffff0000u : v.w[e >> 1] << 16);
+}
+template <typename T>
+__device__ __forceinline__ float ElementOf(const Vec &v, int e) { return Element(v, e, static_cast<const T *>(nullptr)); }
+template <typename T>
+__device__ __forceinline__ Vec PackOf(const float *f) {
+  Vec v;
+  if (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v.w[i] = __float_as_uint(f[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      v.w[i] = Narrow(f[2 * i], static_cast<const T *>(nullptr)) | Narrow(f[(2 * i + 1) % Lanes<T>::kN], static_cast<const T *>(nullptr)) << 16;
+  }
+  return v;
+}
+__device__ __forceinline__ Vec LoadVec(const void *p) {
+  Vec v;
+  __builtin_memcpy(&v, p, 16);
+  return v;
+}
+__device__ __forceinline__ void StoreVec(void *p, const Vec &v) { __builtin_memcpy(p, &v, 16); }
+
+// vectors of a row
+template <typename T>
+__host__ __device__ __forceinline__ int VecsOf(int C) { return (C + Lanes<T>::kN - 1) / Lanes<T>::kN; }
+
+// where vector q of a row is read: its first element, or for the row's incomplete last vector what makes it end with the
+// row (rows of less than a vector: 0)
+template <typename T>
+__device__ __forceinline__ int VecBase(int q, int C) {
+  constexpr int kN = Lanes<T>::kN;
+  return max(0, min(q * kN, C - kN));
+}
+
+// Vector q of row x (q < VecsOf(C)), elements that belong to the vector in front of it as -inf.  `ragged`: uniform, whether
+// q may be the incomplete last vector.
+template <typename T>
+__device__ __forceinline__ Vec LoadRowVec(const T *x, int q, int C, bool ragged) {
+  constexpr int kN = Lanes<T>::kN;
+  Vec v;
+  if (!ragged) return LoadVec(x + q * kN);
+  if (C < kN) {
+    float f[kN];
+#pragma unroll
+    for (int e = 0; e < kN; ++e) f[e] = e < C ? ToFloat(x[e < C ? e : 0]) : Real<float>::NegInf();
+    return PackOf<T>(f);
+  }
+  const int base = VecBase<T>(q, C), skip = q * kN - base;
+  v = LoadVec(x + base);
+  if (skip > 0) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (sizeof(T) == 4) {
+        if (i < skip) v.w[i] = Lanes<T>::kNegInf;
+      } else {
+        if (2 * i < skip) v.w[i] = (v.w[i] & 0xffff0000u) | (Lanes<T>::kNegInf & 0xffffu);
+        if (2 * i + 1 < skip) v.w[i] = (v.w[i] & 0xffffu) | (Lanes<T>::kNegInf & 0xffff0000u);
+      }
+    }
+  }
+  return v;
+}
+
+// A wavefront's U vectors of a row (or of the row's part that starts at vector `first`); -inf past the row's end.
+template <typename T, int U, int W>
+struct RowPart {
+  Vec v[U];
+
+  __device__ __forceinline__ static int Vector(int u, int first, int wave, int lane) {
+    return first + (u * W + wave) * kWave + lane;
+  }
+  // Vector u as a pass over the vectors reads it.  The empty statement is a change of it to the compiler, which would
+  // otherwise hold all vectors' elements unpacked from one pass to the next (twice the registers for 16-bit types).
+  __device__ __forceinline__ const Vec &Packed(int u) {
+    asm volatile("" : "+v"(v[u].w[0]), "+v"(v[u].w[1]), "+v"(v[u].w[2]), "+v"(v[u].w[3]));
+    return v[u];
+  }
+  // the same as Vector, and likewise not kept from one pass to the next (nor what is compared with it)
+  __device__ __forceinline__ static int VectorAnew(int u, int first, int wave, int lane) {
+    int q = Vector(u, first, wave, lane);
+    asm volatile("" : "+v"(q));
+    return q;
+  }
+  __device__ __forceinline__ void Load(const T *x, int C, int first, int wave, int lane) {
+    const int whole = C / Lanes<T>::kN, all = VecsOf<T>(C);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int q = Vector(u, first, wave, lane);
+      const int q_last = first + (u * W + wave) * kWave + kWave - 1;  // the same in every lane
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[u].w[i] = Lanes<T>::kNegInf;
+      if (q_last < whole) v[u] = LoadRowVec<T>(x, q, C, false);
+      else if (q < all) v[u] = LoadRowVec<T>(x, q, C, true);
+    }
+  }
+};
+
 __device__ __forceinline__ float Exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float Log2(float x) { return __builtin_amdgcn_logf(x); }
 
+// Reductions over a wavefront: within rows of 16 lanes by DPP moves, across the four rows through scalar registers.  Every
+// lane gets the result.
+template <int kCtrl>
+__device__ __forceinline__ float DppMove(float v) {
+  return __uint_as_float(__builtin_amdgcn_update_dpp(0u, __float_as_uint(v), kCtrl, 0xf, 0xf, false));
+}
+__device__ __forceinline__ float ReadLane(float v, int lane) {
+  return __uint_as_float((unsigned)__builtin_amdgcn_readlane((int)__float_as_uint(v), lane));
+}
 __device__ __forceinline__ float WaveMaxF(float v) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor(v, off, kWave));
-  return v;
+  v = fmaxf(v, DppMove<0xb1>(v));   // neighbours
+  v = fmaxf(v, DppMove<0x4e>(v));   // pairs
+  v = fmaxf(v, DppMove<0x141>(v));  // quads, mirrored within eight lanes
+  v = fmaxf(v, DppMove<0x140>(v));  // eights, mirrored within sixteen
+  return fmaxf(fmaxf(ReadLane(v, 0), ReadLane(v, 16)), fmaxf(ReadLane(v, 32), ReadLane(v, 48)));
 }
 __device__ __forceinline__ float WaveSumF(float v) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, kWave);
-  return v;
+  v += DppMove<0xb1>(v);
+  v += DppMove<0x4e>(v);
+  v += DppMove<0x141>(v);
+  v += DppMove<0x140>(v);
+  return (ReadLane(v, 0) + ReadLane(v, 16)) + (ReadLane(v, 32) + ReadLane(v, 48));
+}
+__device__ __forceinline__ unsigned BelowLane(unsigned long long lanes) {  // how many of `lanes` are below this one
+  return __builtin_amdgcn_mbcnt_hi((unsigned)(lanes >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)lanes, 0u));
 }
 
 // log p of an element with logit x, in the natural logarithm's scale throughout: (x - m) c could overflow where this does not
 __device__ __forceinline__ float LogProb(float x, float m, float ls, float inv_tau) {
   return ls == Real<float>::NegInf() ? Real<float>::NegInf() : (x - m) * inv_tau - kLn2 * ls;
+}
+
+// What is known of a stretch of logits: the largest (0 where that is -inf), s and t = sum of d 2^d for the entropy.
+struct Sums {
+  float m, s, t;
+};
+// the sums of two stretches as one
+__device__ __forceinline__ Sums Join(const Sums &a, const Sums &b, float c) {
+  if (a.s == 0.0f) return b;
+  if (b.s == 0.0f) return a;
+  Sums r;
+  r.m = fmaxf(a.m, b.m);
+  const float da = (a.m - r.m) * c, db = (b.m - r.m) * c, ea = Exp2(da), eb = Exp2(db);
+  r.s = a.s * ea + b.s * eb;
+  r.t = (a.t + fmaxf(da, kNothing) * a.s) * ea + (b.t + fmaxf(db, kNothing) * b.s) * eb;
+  return r;
 }
 
 // The order of alternatives as one whole number: the larger logit first (a NaN before everything, -0 and 0 alike), the
@@ -75,14 +235,20 @@ __device__ __forceinline__ unsigned long long KeyOf(float x, unsigned index) {
   return ((unsigned long long)OrderOf(x) << 32) | (0xffffffffu - index);
 }
 __device__ __forceinline__ unsigned IndexOf(unsigned long long key) { return 0xffffffffu - (unsigned)key; }
+__device__ __forceinline__ float LogitOf(unsigned long long key) {
+  const unsigned order = (unsigned)(key >> 32);
+  return __uint_as_float((order & 0x80000000u) ? (order == 0xffffffffu ? 0x7fc00000u : order & 0x7fffffffu) : ~order);
+}
 
 inline bool RowsOk(long long rows, long long row_stride, int C, float temperature, int dtype) {
   if (rows < 0 || C < 1 || row_stride < 0) return false;
   if (!(temperature > 0.0f) || temperature - temperature != 0.0f) return false;
   return dtype == K2AMD_F32 || dtype == K2AMD_F16 || dtype == K2AMD_BF16;
 }
-// one workgroup of up to 256 work-items a row: a launch holds fewer than 2^32 work-items
-inline bool RowsServed(long long rows) { return rows < (1ll << 24); }
+inline bool RowsServed(long long rows, int C) { return rows < (1ll << 31) && C <= kMaxColumns; }
+
+// A launch holds fewer than 2^32 work-items in x: calls with more rows are several launches.
+constexpr long long kRowsPerLaunch = 1ll << 20;
 
 }  // namespace
 }  // namespace k2amd

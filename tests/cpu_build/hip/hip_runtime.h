@@ -396,6 +396,25 @@ inline void hip_threads_fence(int, const char *scope, const char *) {
   (void)scope;
 #endif
 }
+inline unsigned long long __ballot(int predicate) {
+  unsigned r[2] = {0, 0};
+  r[hip_threads::flat_thread % hip_threads::kWaveSize / 32] = predicate != 0 ? 1u << (hip_threads::flat_thread % 32) : 0;
+  for (int off = 32; off > 0; off >>= 1) {
+    r[0] |= __shfl_xor(r[0], off);
+    r[1] |= __shfl_xor(r[1], off);
+  }
+  return ((unsigned long long)r[1] << 32) | r[0];
+}
+inline int __popcll(unsigned long long v) { return __builtin_popcountll(v); }
+// v_mbcnt: how many bits of the mask's half are below this lane, plus a
+inline unsigned __builtin_amdgcn_mbcnt_lo(unsigned mask, unsigned a) {
+  const int lane = hip_threads::flat_thread % hip_threads::kWaveSize;
+  return a + (unsigned)__builtin_popcount(lane < 32 ? mask & ((1u << lane) - 1) : mask);
+}
+inline unsigned __builtin_amdgcn_mbcnt_hi(unsigned mask, unsigned a) {
+  const int lane = hip_threads::flat_thread % hip_threads::kWaveSize;
+  return a + (unsigned)__builtin_popcount(lane < 32 ? 0u : mask & ((1u << (lane - 32)) - 1));
+}
 inline int __any(int predicate) {
   int r = predicate != 0;
   for (int off = 32; off > 0; off >>= 1) r |= __shfl_xor(r, off);

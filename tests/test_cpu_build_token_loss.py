@@ -124,10 +124,14 @@ def lib():
 
 @pytest.mark.parametrize("at,dtype,code,C", [
     ("end", np.float32, 0, 1), ("end", np.uint16, 3, 3), ("start", np.uint16, 2, 7), ("end", np.uint16, 3, 8),
-    ("end", np.float32, 0, 61), ("start", np.float32, 0, 61), ("end", np.uint16, 2, 515), ("start", np.uint16, 3, 515)])
+    ("end", np.float32, 0, 61), ("start", np.float32, 0, 61), ("end", np.uint16, 2, 515), ("start", np.uint16, 3, 515),
+    # several wavefronts a row; sixteen of them; rows in two parts
+    ("end", np.float32, 0, 1031), ("end", np.uint16, 3, 8203), ("end", np.float32, 0, 16389), ("end", np.float32, 0, 65539)])
 def test_nothing_outside_the_tensors_is_touched(lib, at, dtype, code, C):
     """The C-ABI on buffers next to pages that may not be touched, in either direction, rows at odd addresses."""
     rows, n, k, K = 3, 2, min(5, C + 1), 4
+    nbytes = lib.k2amd_token_logprobs_scratch_bytes(rows, C, k, code)
+    scratch = Fenced((nbytes,), np.uint8, at=at)
     rng = np.random.default_rng(C)
     if dtype == np.float32:
         x = rng.standard_normal((rows, C)).astype(np.float32)
@@ -141,7 +145,8 @@ def test_nothing_outside_the_tensors_is_touched(lib, at, dtype, code, C):
     lp, h, tl, stats = f32(rows, n), f32(rows), f32(rows, k), f32(rows, 2)
     tt = Fenced((rows, k), np.int64, fill=-7, at=at)
     assert lib.k2amd_token_logprobs_forward(p(fx), C, p(tokens), p(mask), p(lp), p(h), p(tl), p(tt), p(stats), rows, C, n, k,
-                                            1.0, code, None) == 0
+                                            1.0, code, p(scratch), nbytes, None) == 0
+    assert scratch.intact()
     for f in (lp, h, stats):
         assert np.isfinite(f.a).all() and f.intact()
     assert (tt.a[0][:min(k, C)] >= 0).all() and (tt.a[1] == -1).all() and tt.intact() and tl.intact()
@@ -177,19 +182,24 @@ def test_entry_points_refuse_before_launching():
     lib = capi.lib()
     one = ctypes.c_void_p(1)
 
-    def forward(rows=1, C=8, n=0, k=0, tau=1.0, dtype=0, x=one, stride=8, tokens=one, out=one):
-        return lib.k2amd_token_logprobs_forward(x, stride, tokens, None, out, None, out, out, None, rows, C, n, k, tau, dtype, None)
+    def forward(rows=1, C=8, n=0, k=0, tau=1.0, dtype=0, x=one, stride=8, tokens=one, out=one, scratch=None, size=0):
+        return lib.k2amd_token_logprobs_forward(x, stride, tokens, None, out, None, out, out, None, rows, C, n, k, tau, dtype,
+                                                scratch, size, None)
 
     assert forward(rows=0) == 0
     assert [forward(rows=-1), forward(C=0), forward(n=-1), forward(k=-1), forward(dtype=1), forward(dtype=9), forward(x=None),
             forward(stride=-8), forward(n=1, tokens=None), forward(n=1, out=None), forward(k=1, out=None)] == [1] * 11
     assert [forward(tau=t) for t in (0.0, -1.0, float("inf"), float("nan"))] == [1] * 4
-    assert [forward(n=65), forward(k=65), forward(rows=1 << 40)] == [2] * 3
+    assert [forward(n=65), forward(k=65), forward(rows=1 << 31), forward(C=(1 << 22) + 1)] == [2] * 4
+    # rows longer than a workgroup holds need scratch
+    need = lib.k2amd_token_logprobs_scratch_bytes(3, 200000, 5, 3)
+    assert need == 3 * 2 * (16 + 5 * 8) and lib.k2amd_token_logprobs_scratch_bytes(3, 131072, 5, 3) == 0
+    assert forward(rows=3, C=200000, k=5, dtype=3) == 3 and forward(rows=3, C=200000, k=5, dtype=3, scratch=one, size=need - 1) == 3
 
     def distill(rows=1, C=8, K=1, tau=1.0, dtype=3, x=one, a=one, out=one):
         return lib.k2amd_distillation_forward(x, 8, a, a, None, out, None, rows, C, K, 0, tau, dtype, None)
 
-    assert distill(rows=0) == 0 and distill(K=257) == 2 and distill(rows=1 << 40) == 2
+    assert distill(rows=0) == 0 and distill(K=257) == 2 and distill(rows=1 << 31) == 2
     assert [distill(rows=-1), distill(C=0), distill(K=-1), distill(tau=0.0), distill(dtype=1), distill(x=None), distill(a=None),
             distill(out=None)] == [1] * 8
     back = lambda per, g=one: lib.k2amd_distillation_backward(one, 8, one, one, one, g, per, None, 1.0, one, 1, 8, 1, 0, 1.0, 0, None)  # noqa: E731
