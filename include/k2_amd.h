@@ -444,7 +444,7 @@ K2AMD_API int k2amd_lattice_fill(const int32_t *ranges, const int32_t *frames,
  * Rows that do not count get 0, 0, -inf and -1.  A row of nothing but -inf has p = 0, entropy 0 and log-probs -inf.
  * stats [rows][2] (or NULL) and entropy are what the backward call reads.  Rows that a workgroup cannot hold are cut into
  * parts; scratch: device memory of at least k2amd_token_logprobs_scratch_bytes(...) (0 for most calls, then NULL will do;
- * nothing in it has to survive the call).
+ * nothing in it has to survive the call), at a multiple of 16 bytes like every scratch here.
  *
  * Backward: logits_grad [rows][C] (dense, of the logits' type) from what reaches the three results (each may be NULL).
  * A token listed twice takes both gradients. */
@@ -463,14 +463,17 @@ K2AMD_API int k2amd_token_logprobs_backward(const void *logits, long long row_st
  * vocabulary: the row's loss is NaN), top_logprobs [rows][K].  rest == 0: the list is renormalised (q = softmax of its
  * log-probs); rest != 0: q = exp(log-probs) and what they leave of 1 is one more outcome, the student's counterpart of
  * which is everything that is not listed (a row without any student mass there has no such outcome).
- * row_losses [rows] = KL(q || p); 0 for rows that do not count or have no list.  records [rows][4] (or NULL): for the
- * backward call, which writes logits_grad [rows][C] for loss_grad[r / rows_per_loss] * factor * inverse_count[0] (or 1
+ * scratch: as above, k2amd_distillation_scratch_bytes(...) bytes.
+ * row_losses [rows] = KL(q || p); 0 for rows that do not count or have no list.  records [rows][4] (or NULL; at a multiple of 16
+ * bytes): for the backward call, which writes logits_grad [rows][C] for loss_grad[r / rows_per_loss] * factor * inverse_count[0] (or 1
  * where NULL) reaching row r's loss.
  * _sum: sums[i] = factor * (sum of rows_per_sum row losses), divided by the number of rows that count where mean != 0;
  * inverse_count [num_sums] (or NULL) = 1 / max(that number, 1); scratch as the query says. */
+K2AMD_API size_t k2amd_distillation_scratch_bytes(long long rows, int C, int dtype);
 K2AMD_API int k2amd_distillation_forward(const void *logits, long long row_stride, const float *top_logprobs,
                                          const int64_t *top_tokens, const uint8_t *mask, float *row_losses, float *records,
-                                         long long rows, int C, int K, int rest, float temperature, int dtype, void *stream);
+                                         long long rows, int C, int K, int rest, float temperature, int dtype, void *scratch,
+                                         size_t scratch_bytes, void *stream);
 K2AMD_API int k2amd_distillation_backward(const void *logits, long long row_stride, const float *top_logprobs,
                                           const int64_t *top_tokens, const float *records, const float *loss_grad,
                                           long long rows_per_loss, const float *inverse_count, float factor,

@@ -76,7 +76,8 @@ _SIGNATURES = {
     "k2amd_token_logprobs_scratch_bytes": ([_ll] + [_ci] * 3, _sz),
     "k2amd_token_logprobs_forward": ([_vp, _ll] + [_vp] * 7 + [_ll] + [_ci] * 3 + [_cf, _ci, _vp, _sz, _vp], _ci),
     "k2amd_token_logprobs_backward": ([_vp, _ll] + [_vp] * 9 + [_ll] + [_ci] * 3 + [_cf, _ci, _vp], _ci),
-    "k2amd_distillation_forward": ([_vp, _ll] + [_vp] * 5 + [_ll] + [_ci] * 3 + [_cf, _ci, _vp], _ci),
+    "k2amd_distillation_scratch_bytes": ([_ll] + [_ci] * 2, _sz),
+    "k2amd_distillation_forward": ([_vp, _ll] + [_vp] * 5 + [_ll] + [_ci] * 3 + [_cf, _ci, _vp, _sz, _vp], _ci),
     "k2amd_distillation_backward": ([_vp, _ll] + [_vp] * 4 + [_ll, _vp, _cf, _vp, _ll] + [_ci] * 3 + [_cf, _ci, _vp], _ci),
     "k2amd_distillation_sum_scratch_bytes": ([_ll] * 2, _sz),
     "k2amd_distillation_sum": ([_vp] * 4 + [_ll] * 2 + [_ci, _cf, _vp, _sz, _vp], _ci),
@@ -898,10 +899,12 @@ def distillation_forward(logits, top_logprobs, top_tokens, mask, temperature, bu
     expect_optional(mask, "mask", torch.bool, dev, lead)
     losses = torch.empty(lead, dtype=torch.float32, device=dev)
     records = torch.empty(lead + (4,), dtype=torch.float32, device=dev) if keep else None
+    nbytes = lib().k2amd_distillation_scratch_bytes(rows, C, dt)
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     with torch.cuda.device(dev):
         check(lib().k2amd_distillation_forward(x.data_ptr(), stride, ptr(top_logprobs), ptr(top_tokens), ptr(mask),
                                                ptr(losses), ptr(records), rows, C, K, int(bucket), temperature, dt,
-                                               stream_ptr(dev)))
+                                               ptr(scratch), nbytes, stream_ptr(dev)))
     return losses, records
 
 

@@ -18,186 +18,440 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / kWave;
+constexpr int kShort = 16;                  // lanes that hold a short row
+constexpr int kShortRows = kThreads / kShort;  // short rows of a workgroup
 constexpr float kSkipped = -1.0f;  // in a record's last place, which is never negative: the row has no gradient
-constexpr int kSegment = 65536;  // columns whose membership of the list is kept as bits in LDS at a time
 
-__device__ __forceinline__ float BlockMax(float v, float *lds) {
-  v = WaveMaxF(v);
-  __syncthreads();
-  if ((threadIdx.x & (kWave - 1)) == 0) lds[threadIdx.x / kWave] = v;
-  __syncthreads();
-  for (int w = 0; w < kWaves; ++w) v = fmaxf(v, lds[w]);
-  return v;
+// ---- a row's list -----------------------------------------------------------------------------------
+//
+// The entries lie in LDS, entry j in the care of lane j mod L of the group that has the row: its token (-1: none), the
+// teacher's log-prob a and the student's logit x.
+struct List {
+  int *token;
+  float *a, *x;
+  int K;  // 0 for a row without a usable list
+  __device__ __forceinline__ List(float *lds, int entries)
+      : token(reinterpret_cast<int *>(lds)), a(lds + entries), x(lds + 2 * entries), K(entries) {}
+};
+enum ListState { kNone, kUsable, kWrong };
+
+template <typename T, int L>
+__device__ __forceinline__ ListState ReadList(const T *x, int C, const float *top_logprobs, const int64_t *top_tokens,
+                                              const List &list, int lane, bool live) {
+  bool present = false, wrong = false;
+  if (live)
+    for (int j = lane; j < list.K; j += L) {
+      const int64_t given = top_tokens[j];
+      const float a = top_logprobs[j];
+      const int token = given >= 0 && given < C ? (int)given : -1;
+      wrong |= given >= C;
+      present |= token >= 0;
+      list.token[j] = token;
+      list.a[j] = token >= 0 ? a : Real<float>::NegInf();
+      list.x[j] = token >= 0 ? ToFloat(x[token]) : Real<float>::NegInf();
+    }
+  const bool any_wrong = GroupBallot<L>(wrong) != 0, any = GroupBallot<L>(present) != 0;
+  return any_wrong ? kWrong : any ? kUsable : kNone;
 }
-__device__ __forceinline__ float BlockSum(float v, float *lds) {
-  v = WaveSumF(v);
-  __syncthreads();
-  if ((threadIdx.x & (kWave - 1)) == 0) lds[threadIdx.x / kWave] = v;
-  __syncthreads();
-  v = 0;
-  for (int w = 0; w < kWaves; ++w) v += lds[w];
-  return v;
+
+// Bit r: the token of this lane's entry lane + r L stands earlier in the list.  All lanes of the wavefront come here.
+template <int L>
+__device__ __forceinline__ unsigned RepeatedEntries(const List &list, int lane) {
+  unsigned repeated = 0;
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  for (int j = lane, r = 0; j < list.K; j += L, ++r) {
+    bool again = false;
+    for (int i = 0; i < j; ++i) again |= list.token[i] == list.token[j];
+    if (again) repeated |= 1u << r;
+  }
+  return repeated;
 }
 
-// One workgroup a row.
-template <typename T, bool kRest>
-__global__ __launch_bounds__(kThreads) void DistillForwardKernel(
-    const T *__restrict__ logits, long long row_stride, const float *__restrict__ top_logprobs,
-    const int64_t *__restrict__ top_tokens, const uint8_t *__restrict__ mask, float *__restrict__ row_losses,
-    float *__restrict__ records, int C, int K, float c, float inv_tau) {
-  __shared__ float lds[kWaves];
-  __shared__ int entry[kMaxTeacher];
-  __shared__ unsigned listed[kRest ? kSegment / 32 : 1];
-  const size_t row = blockIdx.x;
-  const int tid = threadIdx.x;
-  const bool live = mask == nullptr || mask[row] != 0;
-  // the list: entry j in work-item j
-  int token = -1;
-  float a = Real<float>::NegInf();
-  bool wrong = false;
-  if (live && tid < K) {
-    const int64_t given = top_tokens[row * K + tid];
-    wrong = given >= C;
-    if (given >= 0 && !wrong) {
-      token = (int)given;
-      a = top_logprobs[row * K + tid];
-    }
-    entry[tid] = token;
+// Marks the list's tokens in `bits`, columns from `begin` on, and returns whether a lane of the wavefront found its token
+// marked already.
+template <int L>
+__device__ __forceinline__ bool MarkListed(const List &list, int lane, unsigned *bits, int begin, int end) {
+  bool again = false;
+  for (int j = lane; j < list.K; j += L) {
+    const int token = list.token[j];
+    if (token < begin || token >= end) continue;
+    const unsigned bit = 1u << ((token - begin) & 31);
+    again |= (atomicOr(&bits[(token - begin) >> 5], bit) & bit) != 0;
   }
-  const float present = BlockSum(token >= 0 || wrong ? 1.0f : 0.0f, lds);
-  const float bad = BlockSum(wrong ? 1.0f : 0.0f, lds);
-  const float a_max = BlockMax(a, lds);
-  // no list (without a rest, one of impossible tokens alone is none): nothing to learn; an index past the vocabulary is a
-  // mistake of the caller's and shows as NaN
-  if (!live || present == 0.0f || bad != 0.0f || (!kRest && a_max == Real<float>::NegInf())) {
-    const float v = live && bad != 0.0f ? __uint_as_float(0x7fc00000u) : 0.0f;
-    if (tid == 0) row_losses[row] = v;
-    if (records != nullptr && tid < 4) records[4 * row + tid] = v == 0.0f && tid == 3 ? kSkipped : v;
-    return;
-  }
-  const T *x = logits + row * row_stride;
-  const float xj = token >= 0 ? ToFloat(x[token]) : Real<float>::NegInf();
-  bool first = token >= 0;  // a token listed twice is one token of the set
-  if (kRest)
-    for (int j = 0; j < tid && j < K; ++j)
-      if (entry[j] == token) first = false;
+  return __ballot(again) != 0;
+}
 
-  // the sum over the row, or over what is not listed
-  float m_rest = Real<float>::NegInf(), s_rest = 0.0f;
-  for (int pass = 0; pass < 2; ++pass) {
-    for (int lo = 0; lo < C; lo += kSegment) {
-      const int hi = min(C, lo + kSegment);
-      if (kRest) {
-        __syncthreads();
-        for (int i = tid; i < (hi - lo + 31) / 32; i += kThreads) listed[i] = 0;
-        __syncthreads();
-        if (token >= lo && token < hi) atomicOr(&listed[(token - lo) >> 5], 1u << ((token - lo) & 31));
-        __syncthreads();
-      }
-      for (int i = lo + tid; i < hi; i += kThreads) {
-        if (kRest && (listed[(i - lo) >> 5] >> ((i - lo) & 31) & 1u)) continue;
-        const float v = ToFloat(x[i]);
-        if (pass == 0) m_rest = fmaxf(m_rest, v);
-        else s_rest += Exp2((v - m_rest) * c);
-      }
+// -inf in the place of the elements that are marked
+template <typename T, int U, int W, int L>
+__device__ __forceinline__ void DropListed(RowPart<T, U, W, L> &part, int C, int first, int wave, int lane,
+                                           const unsigned *bits) {
+  constexpr int kN = Lanes<T>::kN;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int q = part.Vector(u, first, wave, lane);
+    unsigned marked = 0;
+    if (q < VecsOf<T>(C)) {
+      const int at = VecBase<T>(q, C) - first * kN;  // below `first` only in a row's last vector, read to end with the row
+      const int from = max(at, 0), shift = from & 31;
+      marked = bits[from >> 5] >> shift;
+      if (shift + kN > 32) marked |= bits[(from >> 5) + 1] << (32 - shift);  // (only in a row's last vector)
+      marked <<= from - at;
     }
-    if (pass == 0) {
-      m_rest = BlockMax(m_rest, lds);
-      if (m_rest == Real<float>::NegInf()) m_rest = 0.0f;
-    } else {
-      s_rest = BlockSum(s_rest, lds);
+    marked &= (1u << kN) - 1;
+    if (__ballot(marked != 0) == 0) continue;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      unsigned &w = part.v[u].w[i];
+      if (sizeof(T) == 4) {
+        if (marked >> i & 1u) w = Lanes<T>::kNegInf;
+      } else {
+        if (marked >> (2 * i) & 1u) w = (w & 0xffff0000u) | (Lanes<T>::kNegInf & 0xffffu);
+        if (marked >> (2 * i + 1) & 1u) w = (w & 0xffffu) | (Lanes<T>::kNegInf & 0xffff0000u);
+      }
     }
   }
-  float m = m_rest, s = s_rest;
+}
+
+// m and s of what a group of lanes holds
+template <typename T, int U, int W, int L>
+__device__ __forceinline__ Sums SumsOf(RowPart<T, U, W, L> &part, float c) {
+  constexpr int kN = Lanes<T>::kN;
+  float high[2] = {Real<float>::NegInf(), Real<float>::NegInf()};
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const Vec &v = part.Packed(u);
+#pragma unroll
+    for (int e = 0; e < kN; ++e) high[e & 1] = fmaxf(high[e & 1], ElementOf<T>(v, e));
+  }
+  Sums r{GroupMax<L>(fmaxf(high[0], high[1])), 0.0f, 0.0f};
+  if (r.m == Real<float>::NegInf()) r.m = 0.0f;
+  float s[4] = {0, 0, 0, 0};
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const Vec &v = part.Packed(u);
+#pragma unroll
+    for (int e = 0; e < kN; ++e) s[e & 3] += Exp2((ElementOf<T>(v, e) - r.m) * c);
+  }
+  r.s = GroupSum<L>((s[0] + s[1]) + (s[2] + s[3]));
+  return r;
+}
+
+// The loss of a row and its record {logit that the elements' exponent is taken from, coefficient of 2^..., m or the
+// teacher's log-sum, sum of the target / s}, from its list and the sums over all its elements (kRest: over those that are
+// not listed).  All lanes of the wavefront come here; lane 0 of the group writes.
+template <int L, bool kRest>
+__device__ __forceinline__ void FinishRow(List list, ListState state, unsigned repeated, Sums rest, int lane, float c,
+                                          float inv_tau, bool live, float *loss_out, float *record) {
+  if (state != kUsable) list.K = 0;
+  float a_max = Real<float>::NegInf(), m_set = Real<float>::NegInf();
+  for (int j = lane, r = 0; j < list.K; j += L, ++r) {
+    a_max = fmaxf(a_max, list.a[j]);
+    m_set = fmaxf(m_set, list.x[j]);
+  }
+  a_max = GroupMax<L>(a_max);
+  float m = rest.m, s = rest.s;
   if (kRest) {
-    const float m_set = BlockMax(first ? xj : Real<float>::NegInf(), lds);
-    m = s_rest == 0.0f ? m_set : fmaxf(m_rest, m_set);
+    m_set = GroupMax<L>(m_set);
+    m = rest.s == 0.0f ? m_set : fmaxf(rest.m, m_set);
     if (m == Real<float>::NegInf()) m = 0.0f;
-    const float s_set = BlockSum(first ? Exp2((xj - m) * c) : 0.0f, lds);
-    s = s_set + (s_rest == 0.0f ? 0.0f : s_rest * Exp2((m_rest - m) * c));
+    float s_set = 0.0f;
+    for (int j = lane, r = 0; j < list.K; j += L, ++r)
+      if (!(repeated >> r & 1u)) s_set += Exp2((list.x[j] - m) * c);  // (absent entries: -inf)
+    s = GroupSum<L>(s_set) + (rest.s == 0.0f ? 0.0f : rest.s * Exp2((rest.m - m) * c));
   }
   const float ls = Log2(s);
-
-  // the teacher
-  float lse = 0.0f, q0 = 0.0f;
-  if (!kRest) lse = a_max + logf(BlockSum(token >= 0 ? expf(a - a_max) : 0.0f, lds));
-  const float q = token >= 0 && a > Real<float>::NegInf() ? expf(a - lse) : 0.0f;
-  float mass = BlockSum(q, lds);
+  // the teacher: its log-sum, or which entry is (the first of) the largest
+  float lse = 0.0f, at = Real<float>::NegInf();
   if (kRest) {
+    for (int j = lane; j < list.K; j += L)
+      if (list.a[j] == a_max) at = fmaxf(at, -(float)j);
+    at = GroupMax<L>(at);
+  } else {
+    float sum = 0.0f;
+    for (int j = lane; j < list.K; j += L) sum += expf(list.a[j] - a_max);
+    lse = a_max + logf(GroupSum<L>(sum));
+  }
+  float others = 0.0f, loss = 0.0f;
+  for (int j = lane; j < list.K; j += L) {
+    const float a = list.a[j];
+    const float q = a > Real<float>::NegInf() ? expf(a - lse) : 0.0f;
+    if (-(float)j != at) others += q;
+    if (q > 0.0f) loss += q * ((a - lse) - LogProb(list.x[j], m, ls, inv_tau));
+  }
+  loss = GroupSum<L>(loss);
+  float mass = 1.0f, p0 = 0.0f, q0 = 0.0f;
+  if (kRest) {
+    others = GroupSum<L>(others);
     // 1 - sum q, the largest by expm1: exact where the list holds nearly everything
-    const float at = BlockMax(token >= 0 && a == a_max ? -(float)tid : -(float)kThreads, lds);
-    const float others = BlockSum(at == -(float)tid ? 0.0f : q, lds);
-    q0 = s_rest == 0.0f ? 0.0f : fmaxf(0.0f, -expm1f(a_max) - others);
-    mass += q0;
-  }
-  float loss = 0.0f;
-  if (q > 0.0f) {
-    loss = q * ((a - lse) - LogProb(xj, m, ls, inv_tau));
-  }
-  loss = BlockSum(loss, lds);
-  float p0 = 0.0f;
-  if (kRest && s_rest != 0.0f) {
-    const float log_p0 = kLn2 * ((m_rest - m) * c + Log2(s_rest) - ls);
-    p0 = expf(log_p0);
-    if (q0 > 0.0f) loss += q0 * (logf(q0) - log_p0);
-  }
-  if (tid == 0) {
-    row_losses[row] = loss;
-    if (records != nullptr) {
-      float *r = records + 4 * row;
-      r[0] = m_rest;
-      r[1] = s_rest == 0.0f ? 0.0f : (kRest ? (mass * p0 - q0) / s_rest : 1.0f / s_rest);
-      r[2] = kRest ? m : lse;
-      r[3] = s == 0.0f ? 0.0f : mass / s;
+    if (rest.s != 0.0f) q0 = fmaxf(0.0f, -expm1f(a_max) - others);
+    mass = others + expf(a_max) + q0;
+    if (rest.s != 0.0f) {
+      const float log_p0 = (rest.m - m) * inv_tau + kLn2 * (Log2(rest.s) - ls);
+      p0 = expf(log_p0);
+      if (q0 > 0.0f) loss += q0 * (logf(q0) - log_p0);
     }
   }
+  if (lane != 0) return;
+  // no list (without a rest, one of impossible tokens alone is none): nothing to learn; an index past the vocabulary is a
+  // mistake of the caller's and shows as NaN
+  const bool skipped = !live || state == kNone || (state == kUsable && !kRest && a_max == Real<float>::NegInf());
+  const float nan = __uint_as_float(0x7fc00000u);
+  *loss_out = skipped ? 0.0f : state == kWrong ? nan : loss;
+  if (record == nullptr) return;
+  float4 r = make_float4(rest.m, rest.s == 0.0f ? 0.0f : (kRest ? (mass * p0 - q0) / rest.s : 1.0f / rest.s), kRest ? m : lse,
+                         s == 0.0f ? 0.0f : mass / s);
+  if (state == kWrong) r = make_float4(nan, nan, nan, nan);
+  if (skipped) r = make_float4(0.0f, 0.0f, 0.0f, kSkipped);
+  *reinterpret_cast<float4 *>(record) = r;
 }
+
+// ---- forward ----------------------------------------------------------------------------------------
+
+struct ForwardArgs {
+  long long row_stride;
+  const float *top_logprobs;
+  const int64_t *top_tokens;
+  const uint8_t *mask;
+  float *row_losses, *records;
+  int C, K;
+  float c, inv_tau;
+  // rows in several parts: [rows][parts] m and s
+  int parts;
+  float2 *part_sums;
+};
+
+// Short rows: 16 lanes each.
+template <typename T, int U, bool kRest>
+__global__ __launch_bounds__(kThreads) void DistillShortKernel(const T *__restrict__ logits, long long row0, long long rows,
+                                                               ForwardArgs a) {
+  constexpr int kWords = U * kShort * Lanes<T>::kN / 32 + 1;
+  __shared__ unsigned listed[kRest ? kShortRows : 1][kRest ? kWords : 1];
+  HIP_DYNAMIC_SHARED(float, lists)
+  const int lane = threadIdx.x % kShort, group = threadIdx.x / kShort;
+  const long long in_launch = (long long)blockIdx.x * kShortRows + group;
+  if ((in_launch & ~3ll) >= rows) return;  // (the wavefront's first row)
+  const bool there = in_launch < rows;
+  const size_t row = row0 + in_launch;
+  const bool live = there && (a.mask == nullptr || a.mask[row] != 0);
+  const T *x = logits + row * a.row_stride;
+  RowPart<T, U, 1, kShort> part;
+  part.Load(x, live ? a.C : 0, 0, 0, lane);
+  if (kRest)
+    for (int i = lane; i < kWords; i += kShort) listed[group][i] = 0;
+  List list(lists + (size_t)group * 3 * a.K, a.K);
+  const ListState state = ReadList<T, kShort>(x, a.C, a.top_logprobs + row * a.K, a.top_tokens + row * a.K, list, lane, live);
+  unsigned repeated = 0;
+  if (kRest) {
+    if (state != kUsable) list.K = 0;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    if (MarkListed<kShort>(list, lane, listed[group], 0, a.C)) repeated = RepeatedEntries<kShort>(list, lane);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    DropListed(part, a.C, 0, 0, lane, listed[group]);
+  }
+  const Sums sums = SumsOf(part, a.c);
+  if (!there) list.K = 0;
+  float *loss = a.row_losses + (there ? row : 0), *record = a.records == nullptr ? nullptr : a.records + 4 * (there ? row : 0);
+  // (a group without a row computes along and writes nothing: its lane 0 is given as another)
+  FinishRow<kShort, kRest>(list, state, repeated, sums, there ? lane : lane + kShort, a.c, a.inv_tau, live, loss, record);
+}
+
+// Longer rows: W wavefronts a row or a part of it; the first has the list.
+template <typename T, int U, int W, bool kRest>
+__global__ __launch_bounds__(W *kWave) void DistillLongKernel(const T *__restrict__ logits, long long row0, ForwardArgs a) {
+  constexpr int kN = Lanes<T>::kN, kWords = U * W * kWave * kN / 32 + 1;
+  __shared__ unsigned listed[kRest ? kWords : 1];
+  __shared__ float lists[3 * kMaxTeacher];
+  __shared__ float2 wave_sums[W];
+  const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x / kWave));
+  const size_t row = row0 + blockIdx.x;
+  const int first = (int)blockIdx.y * (U * W * kWave);
+  const bool live = a.mask == nullptr || a.mask[row] != 0, whole = a.parts == 1;
+  const T *x = logits + row * a.row_stride;
+  List list(lists, a.K);
+  if (!live) {
+    if (wave == 0 && whole)
+      FinishRow<kWave, kRest>(list, kNone, 0, Sums{0, 0, 0}, lane, a.c, a.inv_tau, false, a.row_losses + row,
+                              a.records == nullptr ? nullptr : a.records + 4 * row);
+    return;
+  }
+  RowPart<T, U, W> part;
+  part.Load(x, a.C, first, wave, lane);
+  ListState state = kNone;
+  unsigned repeated = 0;
+  if (wave == 0 && (kRest || whole))
+    state = ReadList<T, kWave>(x, a.C, a.top_logprobs + row * a.K, a.top_tokens + row * a.K, list, lane, true);
+  if (kRest) {
+    for (int i = threadIdx.x; i < kWords; i += W * kWave) listed[i] = 0;
+    __syncthreads();
+    if (wave == 0) {
+      const int begin = first * kN;
+      const bool again = MarkListed<kWave>(list, lane, listed, begin, begin + U * W * kWave * kN);
+      if (again && whole) repeated = RepeatedEntries<kWave>(list, lane);
+    }
+    __syncthreads();
+    DropListed(part, a.C, first, wave, lane, listed);
+  }
+  Sums sums = SumsOf(part, a.c);
+  if (lane == 0) wave_sums[wave] = make_float2(sums.m, sums.s);
+  __syncthreads();
+  if (wave != 0) return;
+  for (int w = 1; w < W; ++w) sums = Join(sums, Sums{wave_sums[w].x, wave_sums[w].y, 0.0f}, a.c);
+  if (whole)
+    FinishRow<kWave, kRest>(list, state, repeated, sums, lane, a.c, a.inv_tau, true, a.row_losses + row,
+                            a.records == nullptr ? nullptr : a.records + 4 * row);
+  else if (lane == 0)
+    a.part_sums[row * a.parts + blockIdx.y] = make_float2(sums.m, sums.s);
+}
+
+// Joins the parts of a row: a wavefront a row.
+template <typename T, bool kRest>
+__global__ __launch_bounds__(kWave) void DistillJoinKernel(const T *__restrict__ logits, long long row0, ForwardArgs a) {
+  __shared__ float lists[3 * kMaxTeacher];
+  const int lane = threadIdx.x;
+  const size_t row = row0 + blockIdx.x;
+  const bool live = a.mask == nullptr || a.mask[row] != 0;
+  List list(lists, a.K);
+  const ListState state = ReadList<T, kWave>(logits + row * a.row_stride, a.C, a.top_logprobs + row * a.K,
+                                             a.top_tokens + row * a.K, list, lane, live);
+  if (state != kUsable) list.K = 0;
+  const unsigned repeated = kRest ? RepeatedEntries<kWave>(list, lane) : 0;
+  Sums sums{0, 0, 0};
+  for (int p = 0; p < a.parts && live; ++p) {
+    const float2 v = a.part_sums[row * a.parts + p];
+    sums = p == 0 ? Sums{v.x, v.y, 0.0f} : Join(sums, Sums{v.x, v.y, 0.0f}, a.c);
+  }
+  FinishRow<kWave, kRest>(list, state, repeated, sums, lane, a.c, a.inv_tau, live, a.row_losses + row,
+                          a.records == nullptr ? nullptr : a.records + 4 * row);
+}
+
+// ---- backward ---------------------------------------------------------------------------------------
 
 // What one row's gradient is scaled by: what reaches its loss, and the reduction's factor.
 struct LossScale {
   const float *loss_grad;       // one value for every rows_per_loss rows
-  long long rows_per_loss;
+  unsigned rows_per_loss;
   const float *inverse_count;   // of the rows that count, where the loss is their mean, or null
   float factor;
   __device__ __forceinline__ float At(size_t row) const {
-    float g = loss_grad[row / rows_per_loss] * factor;
+    const float g = loss_grad[(unsigned)row / rows_per_loss] * factor;
     return inverse_count != nullptr ? g * inverse_count[0] : g;
   }
 };
 
-template <typename T, bool kRest>
-__global__ __launch_bounds__(kThreads) void DistillBackwardKernel(
-    const T *__restrict__ logits, long long row_stride, const float *__restrict__ top_logprobs,
-    const int64_t *__restrict__ top_tokens, const float *__restrict__ records, LossScale scale,
-    T *__restrict__ logits_grad, int C, int K, float c) {
-  __shared__ int entry[kMaxTeacher];
-  __shared__ float entry_q[kMaxTeacher];
-  const size_t row = blockIdx.x;
-  const int tid = threadIdx.x;
-  T *dx = logits_grad + row * C;
-  const float base = records[4 * row + 1], third = records[4 * row + 2], share = records[4 * row + 3];
-  if (share == kSkipped) {
-    for (int i = tid; i < C; i += kThreads) FromFloat(0.0f, &dx[i]);
-    return;
-  }
-  const T *x = logits + row * row_stride;
-  const float g = scale.At(row), m_rest = records[4 * row];
-  if (tid < K) {
-    const int64_t token = top_tokens[row * K + tid];
-    const float a = top_logprobs[row * K + tid];
-    entry[tid] = token >= 0 && token < C ? (int)token : -1;
-    entry_q[tid] = a > Real<float>::NegInf() ? expf(a - (kRest ? 0.0f : third)) : 0.0f;
-  }
-  for (int i = tid; i < C; i += kThreads) FromFloat(g * base * Exp2((ToFloat(x[i]) - m_rest) * c), &dx[i]);
-  __syncthreads();
-  if (tid < K && entry[tid] >= 0) {
-    float q = 0.0f;
-    for (int j = 0; j < K; ++j)
-      if (entry[j] == entry[tid]) q += entry_q[j];
-    const float p = share * Exp2((ToFloat(x[entry[tid]]) - (kRest ? third : m_rest)) * c);
-    FromFloat(g * (p - q), &dx[entry[tid]]);
+struct BackwardArgs {
+  long long row_stride;
+  const float *top_logprobs;
+  const int64_t *top_tokens;
+  const float *records;
+  LossScale scale;
+  int C, K;
+  float c;
+};
+
+// One row's gradient: coefficient * 2^((x - from) c) for an element that is not listed, p - (sum of its entries' q) else.
+template <bool kRest>
+struct RowGrad {
+  float from, coefficient, m, share, lse, g;
+  bool skipped;
+  __device__ __forceinline__ RowGrad(const float4 &r, float scale, float /*c*/)
+      : from(r.x), coefficient(r.y * scale), m(kRest ? r.z : r.x), share(r.w), lse(kRest ? 0.0f : r.z), g(scale),
+        skipped(r.w == kSkipped) {}
+  __device__ __forceinline__ float Unlisted(float x, float c) const { return coefficient * Exp2((x - from) * c); }
+  __device__ __forceinline__ float Listed(float x, float q, float c) const { return g * (share * Exp2((x - m) * c) - q); }
+};
+
+// The elements of the vectors that a group of lanes holds.
+template <typename T, int U, int W, int L, bool kRest>
+__device__ __forceinline__ void WriteUnlisted(RowPart<T, U, W, L> &part, T *dx, int C, int first, int wave, int lane,
+                                              const RowGrad<kRest> &f, float c, bool there) {
+  constexpr int kN = Lanes<T>::kN;
+  const int whole = C / kN, all = there ? VecsOf<T>(C) : 0;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int q = part.Vector(u, first, wave, lane);
+    if (q >= all) continue;
+    float g[kN];
+#pragma unroll
+    for (int e = 0; e < kN; ++e) g[e] = f.skipped ? 0.0f : f.Unlisted(ElementOf<T>(part.v[u], e), c);
+    if (q < whole) {
+      StoreVec(dx + (size_t)q * kN, PackOf<T>(g));
+    } else {  // the incomplete last vector, element by element
+      const int base = VecBase<T>(q, C);
+#pragma unroll
+      for (int e = 0; e < kN; ++e)
+        if (base + e >= q * kN && base + e < C) FromFloat(g[e], &dx[base + e]);
+    }
   }
 }
+
+// The listed elements of columns [begin, end), over what is there: entry j by work-item j mod n.
+template <typename T, bool kRest>
+__device__ __forceinline__ void WriteListed(const T *x, T *dx, const int *token, const float *q, int K, int begin, int end, int i,
+                                            int n, const RowGrad<kRest> &f, float c) {
+  for (int j = i; j < K; j += n) {
+    const int at = token[j];
+    if (at < begin || at >= end) continue;
+    float sum = 0.0f;  // a token that is listed twice takes both
+    for (int l = 0; l < K; ++l)
+      if (token[l] == at) sum += q[l];
+    FromFloat(f.Listed(ToFloat(x[at]), sum, c), &dx[at]);
+  }
+}
+
+template <typename T, int U, bool kRest>
+__global__ __launch_bounds__(kThreads) void DistillShortGradKernel(const T *__restrict__ logits, T *__restrict__ logits_grad,
+                                                                   long long row0, long long rows, BackwardArgs a) {
+  HIP_DYNAMIC_SHARED(float, lists)
+  const int lane = threadIdx.x % kShort, group = threadIdx.x / kShort;
+  // the last row first: of a batch larger than the 256 MB memory-side cache it is the tail that the forward pass left there
+  const long long from_last = (long long)blockIdx.x * kShortRows + group;
+  if ((from_last & ~3ll) >= rows) return;  // (the wavefront's first row)
+  const bool there = from_last < rows;
+  const size_t row = row0 + (there ? rows - 1 - from_last : 0);
+  const T *x = logits + row * a.row_stride;
+  T *dx = logits_grad + row * (size_t)a.C;
+  const RowGrad<kRest> f(*reinterpret_cast<const float4 *>(a.records + 4 * row), a.scale.At(row), a.c);
+  RowPart<T, U, 1, kShort> part;
+  part.Load(x, f.skipped ? 0 : a.C, 0, 0, lane);
+  int *token = reinterpret_cast<int *>(lists) + (size_t)group * 2 * a.K;
+  float *q = lists + (size_t)group * 2 * a.K + a.K;
+  for (int j = lane; j < a.K; j += kShort) {
+    const int64_t given = a.top_tokens[row * a.K + j];
+    token[j] = given >= 0 && given < a.C && there && !f.skipped ? (int)given : -1;
+    q[j] = expf(a.top_logprobs[row * a.K + j] - f.lse);
+  }
+  WriteUnlisted(part, dx, a.C, 0, 0, lane, f, a.c, there);
+  // (the stores above, and the list, are before what follows for every lane of the wavefront)
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  WriteListed(x, dx, token, q, a.K, 0, a.C, lane, kShort, f, a.c);
+}
+
+template <typename T, int U, int W, bool kRest>
+__global__ __launch_bounds__(W *kWave) void DistillLongGradKernel(const T *__restrict__ logits, T *__restrict__ logits_grad,
+                                                                  long long row0, long long rows, BackwardArgs a) {
+  constexpr int kN = Lanes<T>::kN;
+  __shared__ int token[kMaxTeacher];
+  __shared__ float q[kMaxTeacher];
+  const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x / kWave));
+  const size_t row = row0 + rows - 1 - blockIdx.x;  // (the last row first, as above)
+  const int first = (int)blockIdx.y * (U * W * kWave);
+  const T *x = logits + row * a.row_stride;
+  T *dx = logits_grad + row * (size_t)a.C;
+  const RowGrad<kRest> f(*reinterpret_cast<const float4 *>(a.records + 4 * row), a.scale.At(row), a.c);
+  RowPart<T, U, W> part;
+  part.Load(x, f.skipped ? 0 : a.C, first, wave, lane);
+  for (int j = threadIdx.x; j < a.K; j += W * kWave) {
+    const int64_t given = a.top_tokens[row * a.K + j];
+    token[j] = given >= 0 && given < a.C && !f.skipped ? (int)given : -1;
+    q[j] = expf(a.top_logprobs[row * a.K + j] - f.lse);
+  }
+  WriteUnlisted(part, dx, a.C, first, wave, lane, f, a.c, true);
+  __syncthreads();
+  const long long end = (long long)(first + U * W * kWave) * kN;
+  WriteListed(x, dx, token, q, a.K, first * kN, (int)min((long long)a.C, end), (int)threadIdx.x, W * kWave, f, a.c);
+}
+
+// ---- sums, masks and launches -----------------------------------------------------------------------
 
 // Sums of rows_per_sum values each, and how many rows count, in a fixed order: chunks of kChunk values a workgroup, in
 // double, then one workgroup a sum over its chunks.
@@ -263,34 +517,60 @@ __global__ void PrunedMaskKernel(const int64_t *__restrict__ ranges, const int64
   mask[row] = t >= boundary[4 * b + 1] && t < boundary[4 * b + 3] && s >= boundary[4 * b] && s <= boundary[4 * b + 2];
 }
 
-template <typename T>
-int Forward(const void *logits, long long row_stride, const float *top_logprobs, const int64_t *top_tokens,
-            const uint8_t *mask, float *row_losses, float *records, long long rows, int C, int K, int rest,
-            float temperature, hipStream_t stream) {
-  const float c = (float)(kLog2E / (double)temperature);
-  const dim3 grid((unsigned)rows), block(kThreads);
-  if (rest)
-    hipLaunchKernelGGL((DistillForwardKernel<T, true>), grid, block, 0, stream, (const T *)logits, row_stride, top_logprobs,
-                       top_tokens, mask, row_losses, records, C, K, c, (float)(1.0 / (double)temperature));
-  else
-    hipLaunchKernelGGL((DistillForwardKernel<T, false>), grid, block, 0, stream, (const T *)logits, row_stride, top_logprobs,
-                       top_tokens, mask, row_losses, records, C, K, c, (float)(1.0 / (double)temperature));
+// One workgroup of 16 wavefronts with 16 vectors a lane holds 16384 vectors.
+constexpr int kPartVecs = 16 * 16 * kWave;
+int PartsOf(int C, int dtype) {
+  const int vecs = dtype == K2AMD_F32 ? VecsOf<float>(C) : VecsOf<Half>(C);
+  return (vecs + kPartVecs - 1) / kPartVecs;
+}
+
+template <typename T, bool kRest>
+int ForwardOf(const T *logits, long long rows, const ForwardArgs &a, hipStream_t stream) {
+  const int vecs = VecsOf<T>(a.C);
+  for (long long row0 = 0; row0 < rows; row0 += kRowsPerLaunch) {
+    const long long n = rows - row0 < kRowsPerLaunch ? rows - row0 : kRowsPerLaunch;
+    const dim3 short_grid((unsigned)((n + kShortRows - 1) / kShortRows)), block(kThreads), grid((unsigned)n, (unsigned)a.parts);
+    const size_t lds = (size_t)kShortRows * 3 * a.K * sizeof(float);
+    if (vecs <= 2 * kShort) hipLaunchKernelGGL((DistillShortKernel<T, 2, kRest>), short_grid, block, lds, stream, logits, row0, n, a);
+    else if (vecs <= 4 * kShort) hipLaunchKernelGGL((DistillShortKernel<T, 4, kRest>), short_grid, block, lds, stream, logits, row0, n, a);
+    else if (vecs <= 8 * kShort) hipLaunchKernelGGL((DistillShortKernel<T, 8, kRest>), short_grid, block, lds, stream, logits, row0, n, a);
+    else if (vecs <= 16 * kShort) hipLaunchKernelGGL((DistillShortKernel<T, 16, kRest>), short_grid, block, lds, stream, logits, row0, n, a);
+    else if (vecs <= 16 * kWave) hipLaunchKernelGGL((DistillLongKernel<T, 4, 4, kRest>), grid, block, 0, stream, logits, row0, a);
+    else if (vecs <= 64 * kWave) hipLaunchKernelGGL((DistillLongKernel<T, 16, 4, kRest>), grid, block, 0, stream, logits, row0, a);
+    else hipLaunchKernelGGL((DistillLongKernel<T, 16, 16, kRest>), grid, dim3(16 * kWave), 0, stream, logits, row0, a);
+    if (a.parts > 1) hipLaunchKernelGGL((DistillJoinKernel<T, kRest>), dim3((unsigned)n), dim3(kWave), 0, stream, logits, row0, a);
+  }
+  return LaunchStatus();
+}
+
+template <typename T, bool kRest>
+int BackwardOf(const T *logits, T *grad, long long rows, const BackwardArgs &a, hipStream_t stream) {
+  const int vecs = VecsOf<T>(a.C);
+  for (long long done = 0; done < rows; done += kRowsPerLaunch) {
+    const long long n = rows - done < kRowsPerLaunch ? rows - done : kRowsPerLaunch, row0 = rows - done - n;
+    const dim3 short_grid((unsigned)((n + kShortRows - 1) / kShortRows)), block(kThreads);
+    const dim3 grid((unsigned)n, (unsigned)((vecs + 16 * kWave - 1) / (16 * kWave)));
+    const size_t lds = (size_t)kShortRows * 2 * a.K * sizeof(float);
+    if (vecs <= 2 * kShort) hipLaunchKernelGGL((DistillShortGradKernel<T, 2, kRest>), short_grid, block, lds, stream, logits, grad, row0, n, a);
+    else if (vecs <= 4 * kShort) hipLaunchKernelGGL((DistillShortGradKernel<T, 4, kRest>), short_grid, block, lds, stream, logits, grad, row0, n, a);
+    else if (vecs <= 8 * kShort) hipLaunchKernelGGL((DistillShortGradKernel<T, 8, kRest>), short_grid, block, lds, stream, logits, grad, row0, n, a);
+    else if (vecs <= 16 * kShort) hipLaunchKernelGGL((DistillShortGradKernel<T, 16, kRest>), short_grid, block, lds, stream, logits, grad, row0, n, a);
+    else hipLaunchKernelGGL((DistillLongGradKernel<T, 4, 4, kRest>), grid, block, 0, stream, logits, grad, row0, n, a);
+  }
   return LaunchStatus();
 }
 
 template <typename T>
-int Backward(const void *logits, long long row_stride, const float *top_logprobs, const int64_t *top_tokens,
-             const float *records, LossScale scale, void *logits_grad, long long rows, int C, int K,
-             int rest, float temperature, hipStream_t stream) {
-  const float c = (float)(kLog2E / (double)temperature);
-  const dim3 grid((unsigned)rows), block(kThreads);
-  if (rest)
-    hipLaunchKernelGGL((DistillBackwardKernel<T, true>), grid, block, 0, stream, (const T *)logits, row_stride, top_logprobs,
-                       top_tokens, records, scale, (T *)logits_grad, C, K, c);
-  else
-    hipLaunchKernelGGL((DistillBackwardKernel<T, false>), grid, block, 0, stream, (const T *)logits, row_stride, top_logprobs,
-                       top_tokens, records, scale, (T *)logits_grad, C, K, c);
-  return LaunchStatus();
+int Forward(const void *logits, long long rows, int rest, const ForwardArgs &a, hipStream_t stream) {
+  const T *x = static_cast<const T *>(logits);
+  return rest ? ForwardOf<T, true>(x, rows, a, stream) : ForwardOf<T, false>(x, rows, a, stream);
+}
+
+template <typename T>
+int Backward(const void *logits, void *grad, long long rows, int rest, const BackwardArgs &a, hipStream_t stream) {
+  const T *x = static_cast<const T *>(logits);
+  T *dx = static_cast<T *>(grad);
+  return rest ? BackwardOf<T, true>(x, dx, rows, a, stream) : BackwardOf<T, false>(x, dx, rows, a, stream);
 }
 
 long long SumChunks(long long rows_per_sum) { return (rows_per_sum + kChunk - 1) / kChunk; }
@@ -302,39 +582,50 @@ using namespace k2amd;
 
 extern "C" {
 
+size_t k2amd_distillation_scratch_bytes(long long rows, int C, int dtype) {
+  if (rows < 0 || C < 1 || C > kMaxColumns) return 0;
+  const size_t parts = PartsOf(C, dtype);
+  return parts <= 1 ? 0 : (size_t)rows * parts * sizeof(float2);
+}
+
 int k2amd_distillation_forward(const void *logits, long long row_stride, const float *top_logprobs,
                                const int64_t *top_tokens, const uint8_t *mask, float *row_losses, float *records,
-                               long long rows, int C, int K, int rest, float temperature, int dtype, void *stream) {
+                               long long rows, int C, int K, int rest, float temperature, int dtype, void *scratch,
+                               size_t scratch_bytes, void *stream) {
   if (!RowsOk(rows, row_stride, C, temperature, dtype) || K < 0) return K2AMD_ERR_INVALID_ARGUMENT;
   if (!RowsServed(rows, C) || K > kMaxTeacher) return K2AMD_ERR_UNSUPPORTED;
   if (rows == 0) return K2AMD_OK;
-  if (logits == nullptr || row_losses == nullptr || (K > 0 && (top_logprobs == nullptr || top_tokens == nullptr)))
+  if (logits == nullptr || row_losses == nullptr || Misaligned(records) || (K > 0 && (top_logprobs == nullptr || top_tokens == nullptr)))
     return K2AMD_ERR_INVALID_ARGUMENT;
+  const int parts = PartsOf(C, dtype);
+  if (parts > 1 && (scratch == nullptr || Misaligned(scratch) || scratch_bytes < k2amd_distillation_scratch_bytes(rows, C, dtype)))
+    return K2AMD_ERR_WORKSPACE;
+  const ForwardArgs a{row_stride, top_logprobs, top_tokens, mask, row_losses, records, C, K,
+                      (float)(kLog2E / (double)temperature), (float)(1.0 / (double)temperature), parts,
+                      static_cast<float2 *>(scratch)};
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (dtype == K2AMD_F32)
-    return Forward<float>(logits, row_stride, top_logprobs, top_tokens, mask, row_losses, records, rows, C, K, rest, temperature, st);
-  if (dtype == K2AMD_F16)
-    return Forward<Half>(logits, row_stride, top_logprobs, top_tokens, mask, row_losses, records, rows, C, K, rest, temperature, st);
-  return Forward<Bfloat>(logits, row_stride, top_logprobs, top_tokens, mask, row_losses, records, rows, C, K, rest, temperature, st);
+  if (dtype == K2AMD_F32) return Forward<float>(logits, rows, rest, a, st);
+  if (dtype == K2AMD_F16) return Forward<Half>(logits, rows, rest, a, st);
+  return Forward<Bfloat>(logits, rows, rest, a, st);
 }
 
 int k2amd_distillation_backward(const void *logits, long long row_stride, const float *top_logprobs,
-                                const int64_t *top_tokens, const float *records, const float *loss_grad, long long rows_per_loss, const float *inverse_count, float factor,
-                                void *logits_grad, long long rows, int C, int K, int rest, float temperature, int dtype,
-                                void *stream) {
+                                const int64_t *top_tokens, const float *records, const float *loss_grad,
+                                long long rows_per_loss, const float *inverse_count, float factor, void *logits_grad,
+                                long long rows, int C, int K, int rest, float temperature, int dtype, void *stream) {
   if (!RowsOk(rows, row_stride, C, temperature, dtype) || K < 0 || rows_per_loss < 1) return K2AMD_ERR_INVALID_ARGUMENT;
   if (!RowsServed(rows, C) || K > kMaxTeacher) return K2AMD_ERR_UNSUPPORTED;
   if (rows == 0) return K2AMD_OK;
-  if (logits == nullptr || records == nullptr || loss_grad == nullptr || logits_grad == nullptr ||
+  if (logits == nullptr || records == nullptr || loss_grad == nullptr || logits_grad == nullptr || Misaligned(records) ||
       (K > 0 && (top_logprobs == nullptr || top_tokens == nullptr)))
     return K2AMD_ERR_INVALID_ARGUMENT;
+  const BackwardArgs a{row_stride, top_logprobs, top_tokens, records,
+                       LossScale{loss_grad, (unsigned)(rows_per_loss < rows ? rows_per_loss : rows), inverse_count, (float)((double)factor / (double)temperature)}, C, K,
+                       (float)(kLog2E / (double)temperature)};
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const LossScale scale{loss_grad, rows_per_loss, inverse_count, (float)((double)factor / (double)temperature)};
-  if (dtype == K2AMD_F32)
-    return Backward<float>(logits, row_stride, top_logprobs, top_tokens, records, scale, logits_grad, rows, C, K, rest, temperature, st);
-  if (dtype == K2AMD_F16)
-    return Backward<Half>(logits, row_stride, top_logprobs, top_tokens, records, scale, logits_grad, rows, C, K, rest, temperature, st);
-  return Backward<Bfloat>(logits, row_stride, top_logprobs, top_tokens, records, scale, logits_grad, rows, C, K, rest, temperature, st);
+  if (dtype == K2AMD_F32) return Backward<float>(logits, logits_grad, rows, rest, a, st);
+  if (dtype == K2AMD_F16) return Backward<Half>(logits, logits_grad, rows, rest, a, st);
+  return Backward<Bfloat>(logits, logits_grad, rows, rest, a, st);
 }
 
 size_t k2amd_distillation_sum_scratch_bytes(long long sums, long long rows_per_sum) {
@@ -349,7 +640,7 @@ int k2amd_distillation_sum(const float *row_losses, const uint8_t *mask, float *
   if (num_sums > 65535 || SumChunks(rows_per_sum) > (1 << 20)) return K2AMD_ERR_UNSUPPORTED;
   if (num_sums == 0) return K2AMD_OK;
   if (sums == nullptr || (rows_per_sum > 0 && row_losses == nullptr)) return K2AMD_ERR_INVALID_ARGUMENT;
-  if (scratch_bytes < k2amd_distillation_sum_scratch_bytes(num_sums, rows_per_sum) || (rows_per_sum > 0 && scratch == nullptr))
+  if (scratch_bytes < k2amd_distillation_sum_scratch_bytes(num_sums, rows_per_sum) || (rows_per_sum > 0 && (scratch == nullptr || Misaligned(scratch))))
     return K2AMD_ERR_WORKSPACE;
   hipStream_t st = static_cast<hipStream_t>(stream);
   const int chunks = (int)SumChunks(rows_per_sum);

@@ -1016,12 +1016,16 @@ std::tuple<torch::Tensor, OptionalTensor> DistillationForward(torch::Tensor logi
   torch::Tensor losses = torch::empty(r.lead, r.Floats());
   OptionalTensor records;
   if (keep) records = torch::empty(r.Shape(4), r.Floats());
+  const size_t bytes = k2amd_distillation_scratch_bytes(r.rows, Int(r.C), r.dtype);
+  torch::Tensor scratch;
+  if (bytes > 0) scratch = torch::empty({static_cast<int64_t>(bytes)}, r.x.options().dtype(torch::kUInt8));
   void *stream = StreamOf(logits);
   {
     pybind11::gil_scoped_release release;
     Check(k2amd_distillation_forward(r.x.data_ptr(), r.stride, top_logprobs.data_ptr<float>(), I64(top_tokens), MaskPtr(mask),
                                      losses.data_ptr<float>(), FloatPtr(records), r.rows, Int(r.C), Int(K), bucket ? 1 : 0,
-                                     static_cast<float>(temperature), r.dtype, stream));
+                                     static_cast<float>(temperature), r.dtype, bytes > 0 ? scratch.data_ptr() : nullptr, bytes,
+                                     stream));
   }
   return std::make_tuple(losses, records);
 }

@@ -581,7 +581,7 @@ int k2amd_token_logprobs_forward(const void *logits, long long row_stride, const
       (k > 0 && (top_logprobs == nullptr || top_tokens == nullptr)))
     return K2AMD_ERR_INVALID_ARGUMENT;
   const int parts = PartsOf(C, dtype);
-  if (parts > 1 && (scratch == nullptr || scratch_bytes < k2amd_token_logprobs_scratch_bytes(rows, C, k, dtype)))
+  if (parts > 1 && (scratch == nullptr || Misaligned(scratch) || scratch_bytes < k2amd_token_logprobs_scratch_bytes(rows, C, k, dtype)))
     return K2AMD_ERR_WORKSPACE;
   float4 *sums = static_cast<float4 *>(scratch);
   const ForwardArgs a{row_stride, tokens, mask, logprobs, entropy, top_logprobs, top_tokens, stats, C, n, k,

@@ -7,8 +7,11 @@
 // has filled with the type's lowest value stay rows of equal logits (c x alone would overflow).  m is the row's largest
 // logit, or 0 where that is -inf (a row that a mask left nothing of): then s = 0 and every p_i is 0.
 //
-// A row is read once, 16 bytes a lane at a time, and stays in registers: wavefront w of the W that share a row takes, in
-// round u of U, vector (u W + w) 64 + lane.  Rows start at any element: the loads are unaligned ones (a row of odd length
+// A row is read once, 16 bytes a lane at a time, and stays in registers.  Short rows (up to 256 vectors of 16 bytes) are
+// held by 16 lanes each, four rows a wavefront: a reduction is four moves within the 16 lanes that the hardware moves data
+// in, for four rows at once, and what is done once a row (its list, its results) is done for four rows at once.  Longer
+// rows are held by W wavefronts.  Lane l of wavefront w takes, in round u of U, vector (u W + w) L + l, with L = 16 or 64
+// lanes.  Rows start at any element: the loads are unaligned ones (a row of odd length
 // in 16 bits moves the start of every other row off the dword), which cost nothing measurable beside aligned ones here.
 // The last vector of a row whose length is no multiple of the vector's is read so that it ends with the row, and what the
 // vector in front of it holds already is set to -inf in it: no byte outside the row is read, without a loop over elements.
@@ -139,14 +142,13 @@ __device__ __forceinline__ Vec LoadRowVec(const T *x, int q, int C, bool ragged)
   return v;
 }
 
-// A wavefront's U vectors of a row (or of the row's part that starts at vector `first`); -inf past the row's end.
-template <typename T, int U, int W>
+// The U vectors of a row (or of the row's part that starts at vector `first`) that one of W groups of L lanes holds; -inf
+// past the row's end.  lane: within the group.
+template <typename T, int U, int W, int L = kWave>
 struct RowPart {
   Vec v[U];
 
-  __device__ __forceinline__ static int Vector(int u, int first, int wave, int lane) {
-    return first + (u * W + wave) * kWave + lane;
-  }
+  __device__ __forceinline__ static int Vector(int u, int first, int wave, int lane) { return first + (u * W + wave) * L + lane; }
   // Vector u as a pass over the vectors reads it.  The empty statement is a change of it to the compiler, which would
   // otherwise hold all vectors' elements unpacked from one pass to the next (twice the registers for 16-bit types).
   __device__ __forceinline__ const Vec &Packed(int u) {
@@ -164,7 +166,7 @@ struct RowPart {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int q = Vector(u, first, wave, lane);
-      const int q_last = first + (u * W + wave) * kWave + kWave - 1;  // the same in every lane
+      const int q_last = first + (u * W + wave) * L + L - 1;  // the same in every lane
 #pragma unroll
       for (int i = 0; i < 4; ++i) v[u].w[i] = Lanes<T>::kNegInf;
       if (q_last < whole) v[u] = LoadRowVec<T>(x, q, C, false);
@@ -198,6 +200,31 @@ __device__ __forceinline__ float WaveSumF(float v) {
   v += DppMove<0x141>(v);
   v += DppMove<0x140>(v);
   return (ReadLane(v, 0) + ReadLane(v, 16)) + (ReadLane(v, 32) + ReadLane(v, 48));
+}
+// The same over the L lanes of a group: 16 lanes of one row of lanes, or the wavefront.
+template <int L>
+__device__ __forceinline__ float GroupMax(float v) {
+  if (L == kWave) return WaveMaxF(v);
+  v = fmaxf(v, DppMove<0xb1>(v));
+  v = fmaxf(v, DppMove<0x4e>(v));
+  v = fmaxf(v, DppMove<0x141>(v));
+  return fmaxf(v, DppMove<0x140>(v));
+}
+template <int L>
+__device__ __forceinline__ float GroupSum(float v) {
+  if (L == kWave) return WaveSumF(v);
+  v += DppMove<0xb1>(v);
+  v += DppMove<0x4e>(v);
+  v += DppMove<0x141>(v);
+  return v + DppMove<0x140>(v);
+}
+// the lanes of this lane's group among those where `predicate` holds, the group's first lane in bit 0
+template <int L>
+__device__ __forceinline__ unsigned long long GroupBallot(bool predicate) {
+  const unsigned long long all = __ballot(predicate);
+  if (L == kWave) return all;
+  const int shift = (int)(threadIdx.x & (kWave - 1) & ~(unsigned)(L - 1));
+  return (all >> shift) & ((1ull << (L & 63)) - 1);
 }
 __device__ __forceinline__ unsigned BelowLane(unsigned long long lanes) {  // how many of `lanes` are below this one
   return __builtin_amdgcn_mbcnt_hi((unsigned)(lanes >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)lanes, 0u));
@@ -246,6 +273,8 @@ inline bool RowsOk(long long rows, long long row_stride, int C, float temperatur
   return dtype == K2AMD_F32 || dtype == K2AMD_F16 || dtype == K2AMD_BF16;
 }
 inline bool RowsServed(long long rows, int C) { return rows < (1ll << 31) && C <= kMaxColumns; }
+
+inline bool Misaligned(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; }  // of what is accessed by 16 bytes
 
 // A launch holds fewer than 2^32 work-items in x: calls with more rows are several launches.
 constexpr long long kRowsPerLaunch = 1ll << 20;

@@ -160,13 +160,15 @@ def test_nothing_outside_the_tensors_is_touched(lib, at, dtype, code, C):
     ft, fa = fenced(entries, at), fenced(np.log(np.full((rows, K), 0.2, np.float32)), at)
     for rest in (0, 1):
         losses, records = f32(rows), f32(rows, 4)
+        dbytes = lib.k2amd_distillation_scratch_bytes(rows, C, code)
+        dscratch = Fenced((dbytes,), np.uint8, at=at)
         dx = Fenced((rows, C), dtype, fill=77, at=at)
         up = fenced(np.ones(rows, np.float32), at)
         assert lib.k2amd_distillation_forward(p(fx), C, p(fa), p(ft), p(mask), p(losses), p(records), rows, C, K, rest, 1.0, code,
-                                              None) == 0
+                                              p(dscratch), dbytes, None) == 0
         assert lib.k2amd_distillation_backward(p(fx), C, p(fa), p(ft), p(records), p(up), 1, None, 1.0, p(dx), rows, C, K, rest,
                                                1.0, code, None) == 0
-        assert np.isfinite(losses.a).all() and losses.intact() and records.intact() and dx.intact()
+        assert np.isfinite(losses.a).all() and losses.intact() and dscratch.intact() and records.intact() and dx.intact()
         assert (dx.a[1] == 0).all() and not (dx.a[0] == 77).any()
         nbytes = lib.k2amd_distillation_sum_scratch_bytes(1, rows)
         scratch, out, inv = Fenced((nbytes,), np.uint8, at=at), f32(1), f32(1)
@@ -197,9 +199,10 @@ def test_entry_points_refuse_before_launching():
     assert forward(rows=3, C=200000, k=5, dtype=3) == 3 and forward(rows=3, C=200000, k=5, dtype=3, scratch=one, size=need - 1) == 3
 
     def distill(rows=1, C=8, K=1, tau=1.0, dtype=3, x=one, a=one, out=one):
-        return lib.k2amd_distillation_forward(x, 8, a, a, None, out, None, rows, C, K, 0, tau, dtype, None)
+        return lib.k2amd_distillation_forward(x, 8, a, a, None, out, None, rows, C, K, 0, tau, dtype, None, 0, None)
 
     assert distill(rows=0) == 0 and distill(K=257) == 2 and distill(rows=1 << 31) == 2
+    assert distill(C=200000) == 3 and lib.k2amd_distillation_scratch_bytes(3, 200000, 2) == 3 * 2 * 8
     assert [distill(rows=-1), distill(C=0), distill(K=-1), distill(tau=0.0), distill(dtype=1), distill(x=None), distill(a=None),
             distill(out=None)] == [1] * 8
     back = lambda per, g=one: lib.k2amd_distillation_backward(one, 8, one, one, one, g, per, None, 1.0, one, 1, 8, 1, 0, 1.0, 0, None)  # noqa: E731
