@@ -88,7 +88,7 @@ __device__ __forceinline__ void DropListed(RowPart<T, U, W, L> &part, int C, int
   constexpr int kN = Lanes<T>::kN;
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const int q = part.Vector(u, first, wave, lane);
+    const int q = part.VectorAnew(u, first, wave, lane);
     unsigned marked = 0;
     if (q < VecsOf<T>(C)) {
       const int at = VecBase<T>(q, C) - first * kN;  // below `first` only in a row's last vector, read to end with the row
@@ -112,28 +112,18 @@ __device__ __forceinline__ void DropListed(RowPart<T, U, W, L> &part, int C, int
   }
 }
 
-// m and s of what a group of lanes holds
+// the largest logit of what a group of lanes holds
 template <typename T, int U, int W, int L>
-__device__ __forceinline__ Sums SumsOf(RowPart<T, U, W, L> &part, float c) {
-  constexpr int kN = Lanes<T>::kN;
+__device__ __forceinline__ float HighOf(RowPart<T, U, W, L> &part) {
   float high[2] = {Real<float>::NegInf(), Real<float>::NegInf()};
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const Vec &v = part.Packed(u);
 #pragma unroll
-    for (int e = 0; e < kN; ++e) high[e & 1] = fmaxf(high[e & 1], ElementOf<T>(v, e));
+    for (int e = 0; e < Lanes<T>::kN; e += 2)
+      high[e / 2 & 1] = fmaxf(fmaxf(high[e / 2 & 1], ElementOf<T>(v, e)), ElementOf<T>(v, e + 1));
   }
-  Sums r{GroupMax<L>(fmaxf(high[0], high[1])), 0.0f, 0.0f};
-  if (r.m == Real<float>::NegInf()) r.m = 0.0f;
-  float s[4] = {0, 0, 0, 0};
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const Vec &v = part.Packed(u);
-#pragma unroll
-    for (int e = 0; e < kN; ++e) s[e & 3] += Exp2((ElementOf<T>(v, e) - r.m) * c);
-  }
-  r.s = GroupSum<L>((s[0] + s[1]) + (s[2] + s[3]));
-  return r;
+  return GroupMax<L>(fmaxf(high[0], high[1]));
 }
 
 // The loss of a row and its record {logit that the elements' exponent is taken from, coefficient of 2^..., m or the
@@ -248,7 +238,7 @@ __global__ __launch_bounds__(kThreads) void DistillShortKernel(const T *__restri
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     DropListed(part, a.C, 0, 0, lane, listed[group]);
   }
-  const Sums sums = SumsOf(part, a.c);
+  const Sums sums = SumsOf<false>(part, HighOf(part), a.c);
   if (!there) list.K = 0;
   float *loss = a.row_losses + (there ? row : 0), *record = a.records == nullptr ? nullptr : a.records + 4 * (there ? row : 0);
   // (a group without a row computes along and writes nothing: its lane 0 is given as another)
@@ -291,7 +281,7 @@ __global__ __launch_bounds__(W *kWave) void DistillLongKernel(const T *__restric
     __syncthreads();
     DropListed(part, a.C, first, wave, lane, listed);
   }
-  Sums sums = SumsOf(part, a.c);
+  Sums sums = SumsOf<false>(part, HighOf(part), a.c);
   if (lane == 0) wave_sums[wave] = make_float2(sums.m, sums.s);
   __syncthreads();
   if (wave != 0) return;
@@ -316,10 +306,11 @@ __global__ __launch_bounds__(kWave) void DistillJoinKernel(const T *__restrict__
   if (state != kUsable) list.K = 0;
   const unsigned repeated = kRest ? RepeatedEntries<kWave>(list, lane) : 0;
   Sums sums{0, 0, 0};
-  for (int p = 0; p < a.parts && live; ++p) {
-    const float2 v = a.part_sums[row * a.parts + p];
-    sums = p == 0 ? Sums{v.x, v.y, 0.0f} : Join(sums, Sums{v.x, v.y, 0.0f}, a.c);
+  if (live && lane < a.parts) {
+    const float2 v = a.part_sums[row * a.parts + lane];
+    sums = Sums{v.x, v.y, 0.0f};
   }
+  sums = JoinLanes(sums, a.c);
   FinishRow<kWave, kRest>(list, state, repeated, sums, lane, a.c, a.inv_tau, live, a.row_losses + row,
                           a.records == nullptr ? nullptr : a.records + 4 * row);
 }
@@ -517,16 +508,10 @@ __global__ void PrunedMaskKernel(const int64_t *__restrict__ ranges, const int64
   mask[row] = t >= boundary[4 * b + 1] && t < boundary[4 * b + 3] && s >= boundary[4 * b] && s <= boundary[4 * b + 2];
 }
 
-// One workgroup of 16 wavefronts with 16 vectors a lane holds 16384 vectors.
-constexpr int kPartVecs = 16 * 16 * kWave;
-int PartsOf(int C, int dtype) {
-  const int vecs = dtype == K2AMD_F32 ? VecsOf<float>(C) : VecsOf<Half>(C);
-  return (vecs + kPartVecs - 1) / kPartVecs;
-}
-
 template <typename T, bool kRest>
 int ForwardOf(const T *logits, long long rows, const ForwardArgs &a, hipStream_t stream) {
   const int vecs = VecsOf<T>(a.C);
+  const LongShape shape = LongShapeOf(rows, vecs);
   for (long long row0 = 0; row0 < rows; row0 += kRowsPerLaunch) {
     const long long n = rows - row0 < kRowsPerLaunch ? rows - row0 : kRowsPerLaunch;
     const dim3 short_grid((unsigned)((n + kShortRows - 1) / kShortRows)), block(kThreads), grid((unsigned)n, (unsigned)a.parts);
@@ -535,9 +520,8 @@ int ForwardOf(const T *logits, long long rows, const ForwardArgs &a, hipStream_t
     else if (vecs <= 4 * kShort) hipLaunchKernelGGL((DistillShortKernel<T, 4, kRest>), short_grid, block, lds, stream, logits, row0, n, a);
     else if (vecs <= 8 * kShort) hipLaunchKernelGGL((DistillShortKernel<T, 8, kRest>), short_grid, block, lds, stream, logits, row0, n, a);
     else if (vecs <= 16 * kShort) hipLaunchKernelGGL((DistillShortKernel<T, 16, kRest>), short_grid, block, lds, stream, logits, row0, n, a);
-    else if (vecs <= 16 * kWave) hipLaunchKernelGGL((DistillLongKernel<T, 4, 4, kRest>), grid, block, 0, stream, logits, row0, a);
-    else if (vecs <= 64 * kWave) hipLaunchKernelGGL((DistillLongKernel<T, 16, 4, kRest>), grid, block, 0, stream, logits, row0, a);
-    else hipLaunchKernelGGL((DistillLongKernel<T, 16, 16, kRest>), grid, dim3(16 * kWave), 0, stream, logits, row0, a);
+    else if (shape.rounds == 4) hipLaunchKernelGGL((DistillLongKernel<T, 4, 4, kRest>), grid, block, 0, stream, logits, row0, a);
+    else hipLaunchKernelGGL((DistillLongKernel<T, 16, 4, kRest>), grid, block, 0, stream, logits, row0, a);
     if (a.parts > 1) hipLaunchKernelGGL((DistillJoinKernel<T, kRest>), dim3((unsigned)n), dim3(kWave), 0, stream, logits, row0, a);
   }
   return LaunchStatus();
@@ -584,8 +568,8 @@ extern "C" {
 
 size_t k2amd_distillation_scratch_bytes(long long rows, int C, int dtype) {
   if (rows < 0 || C < 1 || C > kMaxColumns) return 0;
-  const size_t parts = PartsOf(C, dtype);
-  return parts <= 1 ? 0 : (size_t)rows * parts * sizeof(float2);
+  const size_t parts = PartsOf(rows, C, dtype);
+  return parts <= 1 ? 0 : ((size_t)rows * parts * sizeof(float2) + 15) / 16 * 16;
 }
 
 int k2amd_distillation_forward(const void *logits, long long row_stride, const float *top_logprobs,
@@ -597,7 +581,7 @@ int k2amd_distillation_forward(const void *logits, long long row_stride, const f
   if (rows == 0) return K2AMD_OK;
   if (logits == nullptr || row_losses == nullptr || Misaligned(records) || (K > 0 && (top_logprobs == nullptr || top_tokens == nullptr)))
     return K2AMD_ERR_INVALID_ARGUMENT;
-  const int parts = PartsOf(C, dtype);
+  const int parts = PartsOf(rows, C, dtype);
   if (parts > 1 && (scratch == nullptr || Misaligned(scratch) || scratch_bytes < k2amd_distillation_scratch_bytes(rows, C, dtype)))
     return K2AMD_ERR_WORKSPACE;
   const ForwardArgs a{row_stride, top_logprobs, top_tokens, mask, row_losses, records, C, K,

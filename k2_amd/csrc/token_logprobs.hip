@@ -231,27 +231,14 @@ __global__ __launch_bounds__(W == 1 ? 4 * kWave : W *kWave) void TokenForwardKer
   for (int u = 0; u < U; ++u) {
     const Vec &v = part.Packed(u);
 #pragma unroll
-    for (int e = 0; e < kN; ++e) group[u % kGroups] = fmaxf(group[u % kGroups], ElementOf<T>(v, e));
+    for (int e = 0; e < kN; e += 2)
+      group[u % kGroups] = fmaxf(fmaxf(group[u % kGroups], ElementOf<T>(v, e)), ElementOf<T>(v, e + 1));
   }
   float high = group[0];
 #pragma unroll
   for (int g = 1; g < kGroups; ++g) high = fmaxf(high, group[g]);
   high = WaveMaxF(high);
-  Sums sums;
-  sums.m = high == Real<float>::NegInf() ? 0.0f : high;
-  float s[4] = {0, 0, 0, 0}, t[4] = {0, 0, 0, 0};
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const Vec &v = part.Packed(u);
-#pragma unroll
-    for (int e = 0; e < kN; ++e) {
-      const float d = (ElementOf<T>(v, e) - sums.m) * a.c, p = Exp2(d);
-      s[e & 3] += p;
-      if (kEntropy) t[e & 3] += fmaxf(d, kNothing) * p;
-    }
-  }
-  sums.s = WaveSumF((s[0] + s[1]) + (s[2] + s[3]));
-  sums.t = kEntropy ? WaveSumF((t[0] + t[1]) + (t[2] + t[3])) : 0.0f;
+  Sums sums = SumsOf<kEntropy>(part, high, a.c);
 
   const bool odd = sums.s != sums.s;  // a NaN or +inf among them
   float threshold = Real<float>::NegInf();
@@ -321,6 +308,15 @@ __global__ __launch_bounds__(W == 1 ? 4 * kWave : W *kWave) void TokenForwardKer
   }
 }
 
+// How many of the n keys at `keys`, the largest first, are larger than `key` (n <= 64).
+__device__ __forceinline__ int LargerKeys(const unsigned long long *keys, int n, unsigned long long key) {
+  int larger = 0;
+#pragma unroll
+  for (int step = 64; step > 0; step >>= 1)
+    if (larger + step <= n && keys[larger + step - 1] > key) larger += step;
+  return larger;
+}
+
 // Joins the parts of a row: a workgroup a row.  The keys of a part are in order, so a key's place among all is its place in
 // its own part and, in every other part, the number of larger ones, by bisection.
 constexpr int kJoinThreads = 256;
@@ -329,60 +325,48 @@ __global__ __launch_bounds__(kJoinThreads) void TokenJoinKernel(const T *__restr
   HIP_DYNAMIC_SHARED(unsigned long long, keys)
   const size_t row = row0 + blockIdx.x;
   if (a.mask != nullptr && a.mask[row] == 0) return;
+  const int i = threadIdx.x, lane = i & (kWave - 1), all = a.parts * a.k;
+  int64_t token = -1;
+  float x_token = 0.0f;
+  if (i < a.n) {
+    token = a.tokens[row * a.n + i];
+    if (token >= 0 && token < a.C) x_token = ToFloat(logits[row * a.row_stride + token]);
+  }
   Sums sums{0, 0, 0};
-  for (int p = 0; p < a.parts; ++p) {
-    const float4 v = a.part_sums[row * a.parts + p];
-    sums = p == 0 ? Sums{v.x, v.y, v.z} : Join(sums, Sums{v.x, v.y, v.z}, a.c);
+  if (lane < a.parts) {
+    const float4 v = a.part_sums[row * a.parts + lane];
+    sums = Sums{v.x, v.y, v.z};
   }
-  const int i = threadIdx.x;
-  if (i < kWave) {
-    int64_t token = -1;
-    float x_token = 0.0f;
-    if (i < a.n) {
-      token = a.tokens[row * a.n + i];
-      if (token >= 0 && token < a.C) x_token = ToFloat(logits[row * a.row_stride + token]);
-    }
-    WriteRow(a, row, i, sums, token, x_token);
-  }
-  if (a.k == 0) return;
-  const int all = a.parts * a.k;
   for (int j = i; j < all; j += kJoinThreads) keys[j] = a.part_keys[row * all + j];
+  sums = JoinLanes(sums, a.c);
+  if (i < kWave) WriteRow(a, row, i, sums, token, x_token);
+  if (a.k == 0) return;
   __syncthreads();
   const float ls = Log2(sums.s);
   for (int j = i; j < all; j += kJoinThreads) {
     const unsigned long long key = keys[j];
     const int part = j / a.k;
     int place = j - part * a.k;
-    if (key == 0) {  // past the last of its part: behind every key, in the order of the parts' ends
+    if (key != 0) {
+#pragma unroll 4
       for (int p = 0; p < a.parts; ++p) {
-        if (p == part) continue;
-        int lo = 0, hi = a.k;  // keys of p that are not 0
-        while (lo < hi) {
-          const int mid = (lo + hi) / 2;
-          if (keys[p * a.k + mid] != 0) lo = mid + 1;
-          else hi = mid;
-        }
-        place += p < part ? a.k : lo;
+        const int larger = LargerKeys(keys + p * a.k, a.k, key);
+        place += p != part ? larger : 0;
       }
       if (place < a.k) {
-        a.top_tokens[row * a.k + place] = -1;
-        a.top_logprobs[row * a.k + place] = Real<float>::NegInf();
+        a.top_tokens[row * a.k + place] = IndexOf(key);
+        a.top_logprobs[row * a.k + place] = LogProb(LogitOf(key), sums.m, ls, a.inv_tau);
       }
       continue;
     }
+    // past the last of its part: behind every key, in the order of the parts' ends
     for (int p = 0; p < a.parts; ++p) {
       if (p == part) continue;
-      int lo = 0, hi = a.k;
-      while (lo < hi) {
-        const int mid = (lo + hi) / 2;
-        if (keys[p * a.k + mid] > key) lo = mid + 1;
-        else hi = mid;
-      }
-      place += lo;
+      place += p < part ? a.k : LargerKeys(keys + p * a.k, a.k, 0ull);
     }
     if (place < a.k) {
-      a.top_tokens[row * a.k + place] = IndexOf(key);
-      a.top_logprobs[row * a.k + place] = LogProb(LogitOf(key), sums.m, ls, a.inv_tau);
+      a.top_tokens[row * a.k + place] = -1;
+      a.top_logprobs[row * a.k + place] = Real<float>::NegInf();
     }
   }
 }
@@ -514,13 +498,6 @@ void LaunchForward(const T *logits, long long rows, bool entropy, const ForwardA
   }
 }
 
-// How many parts a row of C elements is held in: one workgroup of 16 wavefronts with 16 vectors a lane holds 16384 vectors.
-constexpr int kPartVecs = 16 * 16 * kWave;
-int PartsOf(int C, int dtype) {
-  const int vecs = dtype == K2AMD_F32 ? VecsOf<float>(C) : VecsOf<Half>(C);
-  return (vecs + kPartVecs - 1) / kPartVecs;
-}
-
 template <typename T>
 int Forward(const void *logits_v, long long rows, ForwardArgs a, hipStream_t stream) {
   const T *logits = static_cast<const T *>(logits_v);
@@ -529,9 +506,8 @@ int Forward(const void *logits_v, long long rows, ForwardArgs a, hipStream_t str
   if (vecs <= kWave) LaunchForward<T, 1, 1>(logits, rows, entropy, a, stream);
   else if (vecs <= 2 * kWave) LaunchForward<T, 2, 1>(logits, rows, entropy, a, stream);
   else if (vecs <= 4 * kWave) LaunchForward<T, 4, 1>(logits, rows, entropy, a, stream);
-  else if (vecs <= 16 * kWave) LaunchForward<T, 4, 4>(logits, rows, entropy, a, stream);
-  else if (vecs <= 64 * kWave) LaunchForward<T, 16, 4>(logits, rows, entropy, a, stream);
-  else LaunchForward<T, 16, 16>(logits, rows, entropy, a, stream);
+  else if (LongShapeOf(rows, vecs).rounds == 4) LaunchForward<T, 4, 4>(logits, rows, entropy, a, stream);
+  else LaunchForward<T, 16, 4>(logits, rows, entropy, a, stream);
   return LaunchStatus();
 }
 
@@ -566,8 +542,8 @@ extern "C" {
 
 size_t k2amd_token_logprobs_scratch_bytes(long long rows, int C, int k, int dtype) {
   if (rows < 0 || C < 1 || k < 0 || C > kMaxColumns || k > kMaxTop) return 0;
-  const size_t parts = PartsOf(C, dtype);
-  return parts <= 1 ? 0 : (size_t)rows * parts * (sizeof(float4) + (size_t)k * sizeof(unsigned long long));
+  const size_t parts = PartsOf(rows, C, dtype);
+  return parts <= 1 ? 0 : ((size_t)rows * parts * (sizeof(float4) + (size_t)k * sizeof(unsigned long long)) + 15) / 16 * 16;
 }
 
 int k2amd_token_logprobs_forward(const void *logits, long long row_stride, const int64_t *tokens, const uint8_t *mask,
@@ -580,7 +556,7 @@ int k2amd_token_logprobs_forward(const void *logits, long long row_stride, const
   if (logits == nullptr || (n > 0 && (tokens == nullptr || logprobs == nullptr)) ||
       (k > 0 && (top_logprobs == nullptr || top_tokens == nullptr)))
     return K2AMD_ERR_INVALID_ARGUMENT;
-  const int parts = PartsOf(C, dtype);
+  const int parts = PartsOf(rows, C, dtype);
   if (parts > 1 && (scratch == nullptr || Misaligned(scratch) || scratch_bytes < k2amd_token_logprobs_scratch_bytes(rows, C, k, dtype)))
     return K2AMD_ERR_WORKSPACE;
   float4 *sums = static_cast<float4 *>(scratch);

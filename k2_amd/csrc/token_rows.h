@@ -30,7 +30,7 @@ constexpr float kNothing = -1024.0f;
 constexpr int kMaxTokens = 64;        // given tokens of a row
 constexpr int kMaxTop = 64;           // listed alternatives of a row
 constexpr int kMaxTeacher = 256;      // entries of a teacher's list
-constexpr int kMaxColumns = 1 << 22;  // columns of a row: 64 parts of the longest stretch that a workgroup holds
+constexpr int kMaxColumns = 1 << 20;  // columns of a row: 64 parts of what a workgroup holds in 32 bits
 
 // the bits of one 16-bit element and back (to nearest even)
 struct Half {
@@ -57,6 +57,12 @@ __device__ __forceinline__ unsigned Narrow(float f, const Bfloat *) { return Flo
 __device__ __forceinline__ void FromFloat(float f, float *x) { *x = f; }
 __device__ __forceinline__ void FromFloat(float f, Half *x) { x->bits = FloatToHalf(f); }
 __device__ __forceinline__ void FromFloat(float f, Bfloat *x) { x->bits = FloatToBfloat(f); }
+
+// `v`, as a value that the compiler knows nothing of: what is computed from it is computed here and not kept from before
+__device__ __forceinline__ unsigned Anew(unsigned v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
 
 // 16 bytes of a row: four or eight elements
 struct Vec {
@@ -149,17 +155,16 @@ struct RowPart {
   Vec v[U];
 
   __device__ __forceinline__ static int Vector(int u, int first, int wave, int lane) { return first + (u * W + wave) * L + lane; }
-  // Vector u as a pass over the vectors reads it.  The empty statement is a change of it to the compiler, which would
-  // otherwise hold all vectors' elements unpacked from one pass to the next (twice the registers for 16-bit types).
+  // Vector u as a pass over the vectors reads it: the compiler would otherwise hold all vectors' elements unpacked from one
+  // pass to the next (twice the registers for 16-bit types).
   __device__ __forceinline__ const Vec &Packed(int u) {
-    asm volatile("" : "+v"(v[u].w[0]), "+v"(v[u].w[1]), "+v"(v[u].w[2]), "+v"(v[u].w[3]));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[u].w[i] = Anew(v[u].w[i]);
     return v[u];
   }
   // the same as Vector, and likewise not kept from one pass to the next (nor what is compared with it)
   __device__ __forceinline__ static int VectorAnew(int u, int first, int wave, int lane) {
-    int q = Vector(u, first, wave, lane);
-    asm volatile("" : "+v"(q));
-    return q;
+    return (int)Anew((unsigned)Vector(u, first, wave, lane));
   }
   __device__ __forceinline__ void Load(const T *x, int C, int first, int wave, int lane) {
     const int whole = C / Lanes<T>::kN, all = VecsOf<T>(C);
@@ -251,6 +256,60 @@ __device__ __forceinline__ Sums Join(const Sums &a, const Sums &b, float c) {
   return r;
 }
 
+// the sums of the up to 64 stretches that a wavefront's lanes have (s = 0: none) as one, in every lane
+__device__ __forceinline__ Sums JoinLanes(const Sums &a, float c) {
+  Sums r{WaveMaxF(a.s == 0.0f ? Real<float>::NegInf() : a.m), 0.0f, 0.0f};
+  if (r.m == Real<float>::NegInf()) r.m = 0.0f;
+  const float d = a.s == 0.0f ? 0.0f : (a.m - r.m) * c, e = Exp2(d);
+  r.s = WaveSumF(a.s * e);
+  r.t = WaveSumF((a.t + fmaxf(d, kNothing) * a.s) * e);
+  return r;
+}
+
+// m, s and t (kEntropy) of what a group of lanes holds, from its largest logit.  The inner loop is one fused multiply-add,
+// one exponential and one addition an element: d = x c - M with M = m c rounded, which leaves every exponent off by the same
+// M - m c, exactly known, and that is taken out of the sums at the end.  Logits beyond 1e30 (the lowest of a type) would
+// overflow there: rows with a largest logit of that size take the difference first.
+template <bool kEntropy, typename T, int U, int W, int L>
+__device__ __forceinline__ Sums SumsOf(RowPart<T, U, W, L> &part, float high, float c) {
+  constexpr int kN = Lanes<T>::kN;
+  Sums r{high == Real<float>::NegInf() ? 0.0f : high, 0.0f, 0.0f};
+  float s[4] = {0, 0, 0, 0}, t[4] = {0, 0, 0, 0};
+#pragma unroll
+  for (int u = 0; u < U; ++u) part.Packed(u);  // (here, and not in the two branches: each would get registers of its own)
+  const bool can_overflow = sizeof(T) == 4 || Lanes<T>::kNegInf != 0xfc00fc00u;  // (halves end at 65504)
+  const bool far = can_overflow && __ballot(fabsf(r.m) > 1e30f) != 0;
+  const float shift = far ? 0.0f : -(r.m * c);
+  if (far) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      Vec v;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v.w[i] = Anew(part.v[u].w[i]);
+#pragma unroll
+      for (int e = 0; e < kN; ++e) {
+        const float d = (ElementOf<T>(v, e) - r.m) * c, p = Exp2(d);
+        s[e & 3] += p;
+        if (kEntropy) t[e & 3] += fmaxf(d, kNothing) * p;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int e = 0; e < kN; ++e) {
+        const float d = __builtin_fmaf(ElementOf<T>(part.v[u], e), c, shift), p = Exp2(d);
+        s[e & 3] += p;
+        if (kEntropy) t[e & 3] += fmaxf(d, kNothing) * p;
+      }
+  }
+  const float off = far ? 0.0f : __builtin_fmaf(r.m, c, shift), scale = Exp2(-off);
+  r.s = GroupSum<L>((s[0] + s[1]) + (s[2] + s[3]));
+  if (kEntropy) r.t = (GroupSum<L>((t[0] + t[1]) + (t[2] + t[3])) - off * r.s) * scale;
+  r.s *= scale;
+  return r;
+}
+
 // The order of alternatives as one whole number: the larger logit first (a NaN before everything, -0 and 0 alike), the
 // lower index first where logits are equal.  Never 0 for an element of a row.
 __device__ __forceinline__ unsigned OrderOf(float x) {
@@ -274,6 +333,22 @@ inline bool RowsOk(long long rows, long long row_stride, int C, float temperatur
 }
 inline bool RowsServed(long long rows, int C) { return rows < (1ll << 31) && C <= kMaxColumns; }
 
+// How a row of more than 256 vectors is held by workgroups of four wavefronts: in `rounds` vectors a lane, in parts where
+// that does not hold it.
+struct LongShape {
+  int rounds, parts;
+};
+inline LongShape LongShapeOf(long long rows, int vecs) {
+  // 16 vectors a lane hold 4096 vectors; parts of 1024 where that alone would leave compute units without work
+  const int whole = (vecs + 16 * 4 * kWave - 1) / (16 * 4 * kWave), fine = (vecs + 4 * 4 * kWave - 1) / (4 * 4 * kWave);
+  if (fine == 1) return LongShape{4, 1};
+  if (rows * whole < 256 && fine <= 64) return LongShape{4, fine};
+  return LongShape{16, whole};
+}
+inline int PartsOf(long long rows, int C, int dtype) {
+  const int vecs = dtype == K2AMD_F32 ? VecsOf<float>(C) : VecsOf<Half>(C);
+  return vecs <= 4 * kWave ? 1 : LongShapeOf(rows, vecs).parts;
+}
 inline bool Misaligned(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; }  // of what is accessed by 16 bytes
 
 // A launch holds fewer than 2^32 work-items in x: calls with more rows are several launches.
