@@ -468,7 +468,7 @@ K2AMD_API int k2amd_token_logprobs_backward(const void *logits, long long row_st
  * bytes): for the backward call, which writes logits_grad [rows][C] for loss_grad[r / rows_per_loss] * factor * inverse_count[0] (or 1
  * where NULL) reaching row r's loss.
  * _sum: sums[i] = factor * (sum of rows_per_sum row losses), divided by the number of rows that count where mean != 0;
- * inverse_count [num_sums] (or NULL) = 1 / max(that number, 1); scratch as the query says. */
+ * inverse_count [num_sums] (or NULL) = 1 / max(that number, 1); scratch as its query says (0 up to 16384 rows a sum). */
 K2AMD_API size_t k2amd_distillation_scratch_bytes(long long rows, int C, int dtype);
 K2AMD_API int k2amd_distillation_forward(const void *logits, long long row_stride, const float *top_logprobs,
                                          const int64_t *top_tokens, const uint8_t *mask, float *row_losses, float *records,

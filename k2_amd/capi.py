@@ -919,10 +919,10 @@ def distillation_sum(losses, mask, sums, mean, factor):
     out = torch.empty(sums, dtype=torch.float32, device=dev)
     inverse_count = torch.empty(sums, dtype=torch.float32, device=dev) if mean else None
     nbytes = lib().k2amd_distillation_sum_scratch_bytes(sums, per_sum)
-    scratch = torch.empty(max(nbytes, 8), dtype=torch.uint8, device=dev)
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     with torch.cuda.device(dev):
         check(lib().k2amd_distillation_sum(ptr(losses), ptr(mask), ptr(out), ptr(inverse_count), sums, per_sum, int(mean),
-                                           factor, ptr(scratch), scratch.numel(), stream_ptr(dev)))
+                                           factor, ptr(scratch), nbytes, stream_ptr(dev)))
     return out, inverse_count
 
 

@@ -35,9 +35,10 @@ struct List {
 };
 enum ListState { kNone, kUsable, kWrong };
 
-template <typename T, int L>
-__device__ __forceinline__ ListState ReadList(const T *x, int C, const float *top_logprobs, const int64_t *top_tokens,
-                                              const List &list, int lane, bool live) {
+// The tokens and the teacher's log-probs.
+template <int L>
+__device__ __forceinline__ ListState ReadList(int C, const float *top_logprobs, const int64_t *top_tokens, const List &list,
+                                              int lane, bool live) {
   bool present = false, wrong = false;
   if (live)
     for (int j = lane; j < list.K; j += L) {
@@ -48,10 +49,22 @@ __device__ __forceinline__ ListState ReadList(const T *x, int C, const float *to
       present |= token >= 0;
       list.token[j] = token;
       list.a[j] = token >= 0 ? a : Real<float>::NegInf();
-      list.x[j] = token >= 0 ? ToFloat(x[token]) : Real<float>::NegInf();
     }
   const bool any_wrong = GroupBallot<L>(wrong) != 0, any = GroupBallot<L>(present) != 0;
   return any_wrong ? kWrong : any ? kUsable : kNone;
+}
+
+// The logit of entry j's token.
+template <typename T>
+__device__ __forceinline__ float ListedLogit(const T *x, const List &list, int j) {
+  const int token = j < list.K ? list.token[j] : -1;
+  return token >= 0 ? ToFloat(x[token]) : Real<float>::NegInf();
+}
+// The logits of the whole list; that of the lane's first entry is at hand.
+template <typename T, int L>
+__device__ __forceinline__ void ReadLogits(const T *x, const List &list, int lane, float x_first) {
+  if (lane < list.K) list.x[lane] = x_first;
+  for (int j = lane + L; j < list.K; j += L) list.x[j] = ListedLogit(x, list, j);
 }
 
 // Bit r: the token of this lane's entry lane + r L stands earlier in the list.  All lanes of the wavefront come here.
@@ -81,34 +94,13 @@ __device__ __forceinline__ bool MarkListed(const List &list, int lane, unsigned 
   return __ballot(again) != 0;
 }
 
-// -inf in the place of the elements that are marked
 template <typename T, int U, int W, int L>
-__device__ __forceinline__ void DropListed(RowPart<T, U, W, L> &part, int C, int first, int wave, int lane,
-                                           const unsigned *bits) {
-  constexpr int kN = Lanes<T>::kN;
+__device__ __forceinline__ void DropListed(RowPart<T, U, W, L> &part, int C, int lane, const unsigned *bits) {
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const int q = part.VectorAnew(u, first, wave, lane);
-    unsigned marked = 0;
-    if (q < VecsOf<T>(C)) {
-      const int at = VecBase<T>(q, C) - first * kN;  // below `first` only in a row's last vector, read to end with the row
-      const int from = max(at, 0), shift = from & 31;
-      marked = bits[from >> 5] >> shift;
-      if (shift + kN > 32) marked |= bits[(from >> 5) + 1] << (32 - shift);  // (only in a row's last vector)
-      marked <<= from - at;
-    }
-    marked &= (1u << kN) - 1;
-    if (__ballot(marked != 0) == 0) continue;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      unsigned &w = part.v[u].w[i];
-      if (sizeof(T) == 4) {
-        if (marked >> i & 1u) w = Lanes<T>::kNegInf;
-      } else {
-        if (marked >> (2 * i) & 1u) w = (w & 0xffff0000u) | (Lanes<T>::kNegInf & 0xffffu);
-        if (marked >> (2 * i + 1) & 1u) w = (w & 0xffffu) | (Lanes<T>::kNegInf & 0xffff0000u);
-      }
-    }
+    const int q = part.VectorAnew(u, 0, 0, lane);
+    const unsigned marked = q < VecsOf<T>(C) ? MarksOf<T>(bits, VecBase<T>(q, C), 0) : 0u;
+    if (__ballot(marked != 0) != 0) DropMarked<T>(&part.v[u], marked);
   }
 }
 
@@ -210,7 +202,8 @@ struct ForwardArgs {
   float2 *part_sums;
 };
 
-// Short rows: 16 lanes each.
+// Short rows: 16 lanes each.  What the row depends on (mask, list) is asked for first and together, then the row and the
+// listed logits: two round trips to memory before the arithmetic, not four.
 template <typename T, int U, bool kRest>
 __global__ __launch_bounds__(kThreads) void DistillShortKernel(const T *__restrict__ logits, long long row0, long long rows,
                                                                ForwardArgs a) {
@@ -221,40 +214,43 @@ __global__ __launch_bounds__(kThreads) void DistillShortKernel(const T *__restri
   const long long in_launch = (long long)blockIdx.x * kShortRows + group;
   if ((in_launch & ~3ll) >= rows) return;  // (the wavefront's first row)
   const bool there = in_launch < rows;
-  const size_t row = row0 + in_launch;
-  const bool live = there && (a.mask == nullptr || a.mask[row] != 0);
+  const size_t row = row0 + (there ? in_launch : rows - 1);  // (a group without a row follows along and writes nothing)
+  const uint8_t masked = a.mask == nullptr ? 1 : a.mask[row];
+  List list(lists + (size_t)group * 3 * a.K, a.K);
+  ListState state = ReadList<kShort>(a.C, a.top_logprobs + row * a.K, a.top_tokens + row * a.K, list, lane, there);
+  const bool live = there && masked != 0;
+  if (!live) state = kNone;
+  if (state != kUsable) list.K = 0;
   const T *x = logits + row * a.row_stride;
   RowPart<T, U, 1, kShort> part;
-  part.Load(x, live ? a.C : 0, 0, 0, lane);
-  if (kRest)
-    for (int i = lane; i < kWords; i += kShort) listed[group][i] = 0;
-  List list(lists + (size_t)group * 3 * a.K, a.K);
-  const ListState state = ReadList<T, kShort>(x, a.C, a.top_logprobs + row * a.K, a.top_tokens + row * a.K, list, lane, live);
+  part.Load(x, state == kUsable ? a.C : 0, 0, 0, lane);
+  const float x_first = ListedLogit(x, list, lane);
   unsigned repeated = 0;
   if (kRest) {
-    if (state != kUsable) list.K = 0;
+    for (int i = lane; i < kWords; i += kShort) listed[group][i] = 0;
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     if (MarkListed<kShort>(list, lane, listed[group], 0, a.C)) repeated = RepeatedEntries<kShort>(list, lane);
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    DropListed(part, a.C, 0, 0, lane, listed[group]);
+    DropListed(part, a.C, lane, listed[group]);
   }
   const Sums sums = SumsOf<false>(part, HighOf(part), a.c);
-  if (!there) list.K = 0;
-  float *loss = a.row_losses + (there ? row : 0), *record = a.records == nullptr ? nullptr : a.records + 4 * (there ? row : 0);
-  // (a group without a row computes along and writes nothing: its lane 0 is given as another)
-  FinishRow<kShort, kRest>(list, state, repeated, sums, there ? lane : lane + kShort, a.c, a.inv_tau, live, loss, record);
+  ReadLogits<T, kShort>(x, list, lane, x_first);
+  // (lane 0 of a group writes: one without a row is given another)
+  FinishRow<kShort, kRest>(list, state, repeated, sums, there ? lane : lane + kShort, a.c, a.inv_tau, live, a.row_losses + row,
+                           a.records == nullptr ? nullptr : a.records + 4 * row);
 }
 
-// Longer rows: W wavefronts a row or a part of it; the first has the list.
-template <typename T, int U, int W, bool kRest>
-__global__ __launch_bounds__(W *kWave) void DistillLongKernel(const T *__restrict__ logits, long long row0, ForwardArgs a) {
-  constexpr int kN = Lanes<T>::kN, kWords = U * W * kWave * kN / 32 + 1;
-  __shared__ unsigned listed[kRest ? kWords : 1];
+// Longer rows: four wavefronts read along a row or a part of it; the first has the list.
+template <typename T, bool kRest>
+__global__ __launch_bounds__(kThreads) void DistillLongKernel(const T *__restrict__ logits, long long row0, int part_vecs,
+                                                              ForwardArgs a) {
+  constexpr int kN = Lanes<T>::kN;
   __shared__ float lists[3 * kMaxTeacher];
-  __shared__ float2 wave_sums[W];
+  __shared__ float2 wave_sums[kWaves];
+  HIP_DYNAMIC_SHARED(unsigned, listed)
   const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x / kWave));
   const size_t row = row0 + blockIdx.x;
-  const int first = (int)blockIdx.y * (U * W * kWave);
+  const int first = (int)blockIdx.y * part_vecs, end = min(VecsOf<T>(a.C), first + part_vecs);
   const bool live = a.mask == nullptr || a.mask[row] != 0, whole = a.parts == 1;
   const T *x = logits + row * a.row_stride;
   List list(lists, a.K);
@@ -264,33 +260,34 @@ __global__ __launch_bounds__(W *kWave) void DistillLongKernel(const T *__restric
                               a.records == nullptr ? nullptr : a.records + 4 * row);
     return;
   }
-  RowPart<T, U, W> part;
-  part.Load(x, a.C, first, wave, lane);
   ListState state = kNone;
   unsigned repeated = 0;
-  if (wave == 0 && (kRest || whole))
-    state = ReadList<T, kWave>(x, a.C, a.top_logprobs + row * a.K, a.top_tokens + row * a.K, list, lane, true);
+  if (wave == 0 && (kRest || whole)) {
+    state = ReadList<kWave>(a.C, a.top_logprobs + row * a.K, a.top_tokens + row * a.K, list, lane, true);
+    if (state != kUsable) list.K = 0;
+  }
   if (kRest) {
-    for (int i = threadIdx.x; i < kWords; i += W * kWave) listed[i] = 0;
+    for (int i = threadIdx.x; i < part_vecs * kN / 32 + 1; i += kThreads) listed[i] = 0;
     __syncthreads();
     if (wave == 0) {
       const int begin = first * kN;
-      const bool again = MarkListed<kWave>(list, lane, listed, begin, begin + U * W * kWave * kN);
+      const bool again = MarkListed<kWave>(list, lane, listed, begin, min(a.C, begin + part_vecs * kN));
       if (again && whole) repeated = RepeatedEntries<kWave>(list, lane);
     }
     __syncthreads();
-    DropListed(part, a.C, first, wave, lane, listed);
   }
-  Sums sums = SumsOf<false>(part, HighOf(part), a.c);
+  Sums sums = StreamSums<T, kWaves, false, kRest>(x, a.C, first, end, wave, lane, a.c, listed);
   if (lane == 0) wave_sums[wave] = make_float2(sums.m, sums.s);
   __syncthreads();
   if (wave != 0) return;
-  for (int w = 1; w < W; ++w) sums = Join(sums, Sums{wave_sums[w].x, wave_sums[w].y, 0.0f}, a.c);
-  if (whole)
+  for (int w = 1; w < kWaves; ++w) sums = Join(sums, Sums{wave_sums[w].x, wave_sums[w].y, 0.0f}, a.c);
+  if (whole) {
+    ReadLogits<T, kWave>(x, list, lane, ListedLogit(x, list, lane));
     FinishRow<kWave, kRest>(list, state, repeated, sums, lane, a.c, a.inv_tau, true, a.row_losses + row,
                             a.records == nullptr ? nullptr : a.records + 4 * row);
-  else if (lane == 0)
+  } else if (lane == 0) {
     a.part_sums[row * a.parts + blockIdx.y] = make_float2(sums.m, sums.s);
+  }
 }
 
 // Joins the parts of a row: a wavefront a row.
@@ -301,15 +298,16 @@ __global__ __launch_bounds__(kWave) void DistillJoinKernel(const T *__restrict__
   const size_t row = row0 + blockIdx.x;
   const bool live = a.mask == nullptr || a.mask[row] != 0;
   List list(lists, a.K);
-  const ListState state = ReadList<T, kWave>(logits + row * a.row_stride, a.C, a.top_logprobs + row * a.K,
-                                             a.top_tokens + row * a.K, list, lane, live);
-  if (state != kUsable) list.K = 0;
-  const unsigned repeated = kRest ? RepeatedEntries<kWave>(list, lane) : 0;
   Sums sums{0, 0, 0};
   if (live && lane < a.parts) {
     const float2 v = a.part_sums[row * a.parts + lane];
     sums = Sums{v.x, v.y, 0.0f};
   }
+  const ListState state = ReadList<kWave>(a.C, a.top_logprobs + row * a.K, a.top_tokens + row * a.K, list, lane, live);
+  if (state != kUsable) list.K = 0;
+  const T *x = logits + row * a.row_stride;
+  ReadLogits<T, kWave>(x, list, lane, ListedLogit(x, list, lane));
+  const unsigned repeated = kRest ? RepeatedEntries<kWave>(list, lane) : 0;
   sums = JoinLanes(sums, a.c);
   FinishRow<kWave, kRest>(list, state, repeated, sums, lane, a.c, a.inv_tau, live, a.row_losses + row,
                           a.records == nullptr ? nullptr : a.records + 4 * row);
@@ -444,44 +442,69 @@ __global__ __launch_bounds__(W *kWave) void DistillLongGradKernel(const T *__res
 
 // ---- sums, masks and launches -----------------------------------------------------------------------
 
-// Sums of rows_per_sum values each, and how many rows count, in a fixed order: chunks of kChunk values a workgroup, in
-// double, then one workgroup a sum over its chunks.
-constexpr int kChunk = 8192;
+// Sums of rows_per_sum values each, and how many rows count, in a fixed order and in double: a workgroup of 1024 a chunk of
+// kChunk values, eight of them on their way at a time in each work-item; where a sum has several chunks, a wavefront joins
+// them.  (A sum of one chunk, as of most batches of sequences, is one launch.)
+constexpr int kChunk = 16384, kSumThreads = 1024;
 
-__global__ __launch_bounds__(kThreads) void RowChunkSumKernel(const float *__restrict__ values,
-                                                              const uint8_t *__restrict__ mask, long long rows_per_sum,
-                                                              double *__restrict__ partial) {
-  __shared__ double lds[2 * kWaves];
-  const long long first = (long long)blockIdx.x * kChunk, last = min(rows_per_sum, first + (long long)kChunk);
+struct SumOutput {
+  float *sums, *inverse_count;
+  int mean;
+  float factor;
+  __device__ __forceinline__ void Write(size_t i, double sum, double count) const {
+    count = count > 1 ? count : 1;
+    sums[i] = (float)(sum * factor / (mean ? count : 1.0));
+    if (inverse_count != nullptr) inverse_count[i] = (float)(1.0 / count);
+  }
+};
+
+__global__ __launch_bounds__(kSumThreads) void RowChunkSumKernel(const float *__restrict__ values,
+                                                                 const uint8_t *__restrict__ mask, int rows_per_sum,
+                                                                 double *__restrict__ partial, SumOutput out) {
+  __shared__ double lds[2 * kSumThreads / kWave];
+  const int first = (int)blockIdx.x * kChunk, last = min(rows_per_sum, first + kChunk);
   const size_t base = (size_t)blockIdx.y * rows_per_sum;
   double sum = 0, count = 0;
-  for (long long i = first + threadIdx.x; i < last; i += kThreads) {
-    sum += values[base + i];
-    if (mask == nullptr || mask[base + i] != 0) count += 1;
+  for (int i = first + (int)threadIdx.x; i < last; i += 8 * kSumThreads) {
+    float v[8];
+    uint8_t m[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int at = i + j * kSumThreads;
+      v[j] = at < last ? values[base + at] : 0.0f;
+      m[j] = at < last ? (mask != nullptr ? mask[base + at] : 1) : 0;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      sum += v[j];
+      count += m[j] != 0 ? 1.0 : 0.0;
+    }
   }
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) {
     sum += __shfl_xor(sum, off, kWave);
     count += __shfl_xor(count, off, kWave);
   }
-  if ((threadIdx.x & (kWave - 1)) == 0) {
-    lds[threadIdx.x / kWave] = sum;
-    lds[kWaves + threadIdx.x / kWave] = count;
+  const int wave = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1);
+  if (lane == 0) {
+    lds[2 * wave] = sum;
+    lds[2 * wave + 1] = count;
   }
   __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int w = 1; w < kWaves; ++w) {
-      sum += lds[w];
-      count += lds[kWaves + w];
-    }
-    double *out = partial + 2 * ((size_t)blockIdx.y * gridDim.x + blockIdx.x);
-    out[0] = sum;
-    out[1] = count;
+  if (threadIdx.x != 0) return;
+  for (int w = 1; w < kSumThreads / kWave; ++w) {
+    sum += lds[2 * w];
+    count += lds[2 * w + 1];
+  }
+  if (gridDim.x == 1) {
+    out.Write(blockIdx.y, sum, count);
+  } else {
+    partial[2 * ((size_t)blockIdx.y * gridDim.x + blockIdx.x)] = sum;
+    partial[2 * ((size_t)blockIdx.y * gridDim.x + blockIdx.x) + 1] = count;
   }
 }
 
-__global__ __launch_bounds__(kWave) void RowSumKernel(const double *__restrict__ partial, int chunks, int mean, float factor,
-                                                      float *__restrict__ sums, float *__restrict__ inverse_count) {
+__global__ __launch_bounds__(kWave) void RowSumKernel(const double *__restrict__ partial, int chunks, SumOutput out) {
   double sum = 0, count = 0;
   for (int i = threadIdx.x; i < chunks; i += kWave) {
     sum += partial[2 * ((size_t)blockIdx.x * chunks + i)];
@@ -492,11 +515,7 @@ __global__ __launch_bounds__(kWave) void RowSumKernel(const double *__restrict__
     sum += __shfl_xor(sum, off, kWave);
     count += __shfl_xor(count, off, kWave);
   }
-  if (threadIdx.x == 0) {
-    count = count > 1 ? count : 1;
-    sums[blockIdx.x] = (float)(sum * factor / (mean ? count : 1.0));
-    if (inverse_count != nullptr) inverse_count[blockIdx.x] = (float)(1.0 / count);
-  }
+  if (threadIdx.x == 0) out.Write(blockIdx.x, sum, count);
 }
 
 __global__ void PrunedMaskKernel(const int64_t *__restrict__ ranges, const int64_t *__restrict__ boundary,
@@ -508,10 +527,16 @@ __global__ void PrunedMaskKernel(const int64_t *__restrict__ ranges, const int64
   mask[row] = t >= boundary[4 * b + 1] && t < boundary[4 * b + 3] && s >= boundary[4 * b] && s <= boundary[4 * b + 2];
 }
 
+int PartsOf(long long rows, int C, int dtype) {
+  const int each = dtype == K2AMD_F32 ? Lanes<float>::kN : Lanes<Half>::kN, vecs = (C + each - 1) / each;
+  return vecs <= 16 * kShort || rows == 0 ? 1 : StreamShapeOf(rows, vecs, each).parts;
+}
+
 template <typename T, bool kRest>
 int ForwardOf(const T *logits, long long rows, const ForwardArgs &a, hipStream_t stream) {
   const int vecs = VecsOf<T>(a.C);
-  const LongShape shape = LongShapeOf(rows, vecs);
+  const LongShape shape = StreamShapeOf(rows, vecs, Lanes<T>::kN);
+  const size_t marks = kRest ? (size_t)(shape.vecs * Lanes<T>::kN / 32 + 1) * sizeof(unsigned) : 0;
   for (long long row0 = 0; row0 < rows; row0 += kRowsPerLaunch) {
     const long long n = rows - row0 < kRowsPerLaunch ? rows - row0 : kRowsPerLaunch;
     const dim3 short_grid((unsigned)((n + kShortRows - 1) / kShortRows)), block(kThreads), grid((unsigned)n, (unsigned)a.parts);
@@ -520,8 +545,7 @@ int ForwardOf(const T *logits, long long rows, const ForwardArgs &a, hipStream_t
     else if (vecs <= 4 * kShort) hipLaunchKernelGGL((DistillShortKernel<T, 4, kRest>), short_grid, block, lds, stream, logits, row0, n, a);
     else if (vecs <= 8 * kShort) hipLaunchKernelGGL((DistillShortKernel<T, 8, kRest>), short_grid, block, lds, stream, logits, row0, n, a);
     else if (vecs <= 16 * kShort) hipLaunchKernelGGL((DistillShortKernel<T, 16, kRest>), short_grid, block, lds, stream, logits, row0, n, a);
-    else if (shape.rounds == 4) hipLaunchKernelGGL((DistillLongKernel<T, 4, 4, kRest>), grid, block, 0, stream, logits, row0, a);
-    else hipLaunchKernelGGL((DistillLongKernel<T, 16, 4, kRest>), grid, block, 0, stream, logits, row0, a);
+    else hipLaunchKernelGGL((DistillLongKernel<T, kRest>), grid, block, marks, stream, logits, row0, shape.vecs, a);
     if (a.parts > 1) hipLaunchKernelGGL((DistillJoinKernel<T, kRest>), dim3((unsigned)n), dim3(kWave), 0, stream, logits, row0, a);
   }
   return LaunchStatus();
@@ -612,27 +636,30 @@ int k2amd_distillation_backward(const void *logits, long long row_stride, const 
   return Backward<Bfloat>(logits, logits_grad, rows, rest, a, st);
 }
 
-size_t k2amd_distillation_sum_scratch_bytes(long long sums, long long rows_per_sum) {
-  if (sums < 0 || rows_per_sum < 0) return 0;
-  return (size_t)sums * (size_t)SumChunks(rows_per_sum) * 2 * sizeof(double);
+size_t k2amd_distillation_sum_scratch_bytes(long long num_sums, long long rows_per_sum) {
+  if (num_sums < 0 || rows_per_sum < 0) return 0;
+  const size_t chunks = (size_t)SumChunks(rows_per_sum);
+  return chunks <= 1 ? 0 : (size_t)num_sums * chunks * 2 * sizeof(double);
 }
 
 int k2amd_distillation_sum(const float *row_losses, const uint8_t *mask, float *sums, float *inverse_count,
                            long long num_sums, long long rows_per_sum, int mean, float factor, void *scratch,
                            size_t scratch_bytes, void *stream) {
   if (num_sums < 0 || rows_per_sum < 0) return K2AMD_ERR_INVALID_ARGUMENT;
-  if (num_sums > 65535 || SumChunks(rows_per_sum) > (1 << 20)) return K2AMD_ERR_UNSUPPORTED;
+  if (num_sums > 65535 || rows_per_sum >= (1ll << 31)) return K2AMD_ERR_UNSUPPORTED;
   if (num_sums == 0) return K2AMD_OK;
   if (sums == nullptr || (rows_per_sum > 0 && row_losses == nullptr)) return K2AMD_ERR_INVALID_ARGUMENT;
-  if (scratch_bytes < k2amd_distillation_sum_scratch_bytes(num_sums, rows_per_sum) || (rows_per_sum > 0 && (scratch == nullptr || Misaligned(scratch))))
+  const int chunks = rows_per_sum > 0 ? (int)SumChunks(rows_per_sum) : 1;
+  if (chunks > 1 && (scratch == nullptr || Misaligned(scratch) ||
+                     scratch_bytes < k2amd_distillation_sum_scratch_bytes(num_sums, rows_per_sum)))
     return K2AMD_ERR_WORKSPACE;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const int chunks = (int)SumChunks(rows_per_sum);
-  if (chunks > 0)
-    hipLaunchKernelGGL(RowChunkSumKernel, dim3((unsigned)chunks, (unsigned)num_sums), dim3(kThreads), 0, st, row_losses, mask,
-                       rows_per_sum, (double *)scratch);
-  hipLaunchKernelGGL(RowSumKernel, dim3((unsigned)num_sums), dim3(kWave), 0, st, (const double *)scratch, chunks, mean, factor,
-                     sums, inverse_count);
+  const SumOutput out{sums, inverse_count, mean, factor};
+  hipLaunchKernelGGL(RowChunkSumKernel, dim3((unsigned)chunks, (unsigned)num_sums), dim3(kSumThreads), 0, st, row_losses, mask,
+                     (int)rows_per_sum, static_cast<double *>(scratch), out);
+  if (chunks > 1)
+    hipLaunchKernelGGL(RowSumKernel, dim3((unsigned)num_sums), dim3(kWave), 0, st, static_cast<const double *>(scratch), chunks,
+                       out);
   return LaunchStatus();
 }
 

@@ -1043,14 +1043,14 @@ std::tuple<torch::Tensor, OptionalTensor> DistillationSum(torch::Tensor losses, 
   OptionalTensor inverse_count;
   if (mean) inverse_count = torch::empty({sums}, losses.options());
   const size_t bytes = k2amd_distillation_sum_scratch_bytes(sums, per_sum);
-  torch::Tensor scratch =
-      torch::empty({static_cast<int64_t>(std::max<size_t>(bytes, 8))}, losses.options().dtype(torch::kUInt8));
+  torch::Tensor scratch;
+  if (bytes > 0) scratch = torch::empty({static_cast<int64_t>(bytes)}, losses.options().dtype(torch::kUInt8));
   void *stream = StreamOf(losses);
   {
     pybind11::gil_scoped_release release;
     Check(k2amd_distillation_sum(losses.data_ptr<float>(), MaskPtr(mask), out.data_ptr<float>(), FloatPtr(inverse_count), sums,
-                                 per_sum, mean ? 1 : 0, static_cast<float>(factor), scratch.data_ptr(),
-                                 static_cast<size_t>(scratch.numel()), stream));
+                                 per_sum, mean ? 1 : 0, static_cast<float>(factor), bytes > 0 ? scratch.data_ptr() : nullptr,
+                                 bytes, stream));
   }
   return std::make_tuple(out, inverse_count);
 }

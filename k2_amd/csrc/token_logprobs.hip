@@ -498,6 +498,11 @@ void LaunchForward(const T *logits, long long rows, bool entropy, const ForwardA
   }
 }
 
+int PartsOf(long long rows, int C, int dtype) {
+  const int vecs = dtype == K2AMD_F32 ? VecsOf<float>(C) : VecsOf<Half>(C);
+  return vecs <= 4 * kWave ? 1 : HeldShapeOf(rows, vecs).parts;
+}
+
 template <typename T>
 int Forward(const void *logits_v, long long rows, ForwardArgs a, hipStream_t stream) {
   const T *logits = static_cast<const T *>(logits_v);
@@ -506,7 +511,7 @@ int Forward(const void *logits_v, long long rows, ForwardArgs a, hipStream_t str
   if (vecs <= kWave) LaunchForward<T, 1, 1>(logits, rows, entropy, a, stream);
   else if (vecs <= 2 * kWave) LaunchForward<T, 2, 1>(logits, rows, entropy, a, stream);
   else if (vecs <= 4 * kWave) LaunchForward<T, 4, 1>(logits, rows, entropy, a, stream);
-  else if (LongShapeOf(rows, vecs).rounds == 4) LaunchForward<T, 4, 4>(logits, rows, entropy, a, stream);
+  else if (HeldShapeOf(rows, vecs).vecs == 1024) LaunchForward<T, 4, 4>(logits, rows, entropy, a, stream);
   else LaunchForward<T, 16, 4>(logits, rows, entropy, a, stream);
   return LaunchStatus();
 }

@@ -310,6 +310,121 @@ __device__ __forceinline__ Sums SumsOf(RowPart<T, U, W, L> &part, float high, fl
   return r;
 }
 
+// -inf in the place of a vector's elements that are marked
+template <typename T>
+__device__ __forceinline__ void DropMarked(Vec *v, unsigned marked) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    unsigned &w = v->w[i];
+    if (sizeof(T) == 4) {
+      if (marked >> i & 1u) w = Lanes<T>::kNegInf;
+    } else {
+      if (marked >> (2 * i) & 1u) w = (w & 0xffff0000u) | (Lanes<T>::kNegInf & 0xffffu);
+      if (marked >> (2 * i + 1) & 1u) w = (w & 0xffffu) | (Lanes<T>::kNegInf & 0xffff0000u);
+    }
+  }
+}
+// the marks of the elements of a vector that is read from column `base` on; bit 0 of `bits` is column `begin` (`base` is
+// below it only in a row's last vector, which is read to end with the row); one word behind the last is readable
+template <typename T>
+__device__ __forceinline__ unsigned MarksOf(const unsigned *bits, int base, int begin) {
+  constexpr int kN = Lanes<T>::kN;
+  const int at = base - begin, from = max(at, 0), shift = from & 31;
+  unsigned marked = bits[from >> 5] >> shift;
+  if (shift + kN > 32) marked |= bits[(from >> 5) + 1] << (32 - shift);  // (only in a row's last vector)
+  return (marked << (from - at)) & ((1u << kN) - 1);
+}
+
+// m, s and t (kEntropy) of vectors [first, end) of a row that W wavefronts read, each on its own and without keeping them:
+// a lane runs along its vectors with a largest logit of its own, four vectors at a time, while the next four are on their
+// way.  kMarked: without the elements marked in `bits` (of columns from first on).
+template <typename T, int W, bool kEntropy, bool kMarked>
+__device__ __forceinline__ Sums StreamSums(const T *x, int C, int first, int end, int wave, int lane, float c,
+                                           const unsigned *bits) {
+  constexpr int kN = Lanes<T>::kN, kStep = 4;
+  const int whole = C / kN;
+  const int rounds = (end - first + W * kWave - 1) / (W * kWave);
+  Sums r{Real<float>::NegInf(), 0.0f, 0.0f};
+  bool far = false;
+  float reference = 0.0f;  // M: what the exponents are taken from, m c rounded
+  float s[4] = {0, 0, 0, 0}, t[4] = {0, 0, 0, 0};
+  Vec next[kStep];
+  auto fetch = [&](int round) {
+#pragma unroll
+    for (int i = 0; i < kStep; ++i) {
+      const int q = first + ((round + i) * W + wave) * kWave + lane;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) next[i].w[j] = Lanes<T>::kNegInf;
+      if (q < end) next[i] = LoadRowVec<T>(x, q, C, q >= whole);
+    }
+  };
+  fetch(0);
+  for (int round = 0; round < rounds; round += kStep) {
+    Vec v[kStep];
+#pragma unroll
+    for (int i = 0; i < kStep; ++i) v[i] = next[i];
+    if (round + kStep < rounds) fetch(round + kStep);
+    if (kMarked) {
+#pragma unroll
+      for (int i = 0; i < kStep; ++i) {
+        const int q = first + ((round + i) * W + wave) * kWave + lane;
+        const unsigned marked = q < end ? MarksOf<T>(bits, VecBase<T>(q, C), first * kN) : 0u;
+        if (__ballot(marked != 0) != 0) DropMarked<T>(&v[i], marked);
+      }
+    }
+    float high[2] = {r.m, Real<float>::NegInf()};
+#pragma unroll
+    for (int i = 0; i < kStep; ++i)
+#pragma unroll
+      for (int e = 0; e < kN; e += 2)
+        high[e / 2 & 1] = fmaxf(fmaxf(high[e / 2 & 1], ElementOf<T>(v[i], e)), ElementOf<T>(v[i], e + 1));
+    r.m = fmaxf(high[0], high[1]);
+    const float before = reference;
+    reference = r.m == Real<float>::NegInf() ? 0.0f : r.m * c;
+    far |= fabsf(r.m) > 1e30f && r.m != Real<float>::NegInf();
+    const float down = fminf(before - reference, 0.0f), scale = Exp2(down);  // (the first reference may be below 0: s is 0 then)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (kEntropy) t[i] = (t[i] + fmaxf(down, kNothing) * s[i]) * scale;
+      s[i] *= scale;
+    }
+#pragma unroll
+    for (int i = 0; i < kStep; ++i)
+#pragma unroll
+      for (int e = 0; e < kN; ++e) {
+        const float d = __builtin_fmaf(ElementOf<T>(v[i], e), c, -reference), p = Exp2(d);
+        s[e & 3] += p;
+        if (kEntropy) t[e & 3] += fmaxf(d, kNothing) * p;
+      }
+  }
+  if (__ballot(far) != 0) {  // logits at the end of the type's range: differences first, no reference (as in SumsOf)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[i] = t[i] = 0.0f;
+    r.m = WaveMaxF(r.m);
+    for (int round = 0; round < rounds; ++round) {
+      const int q = first + (round * W + wave) * kWave + lane;
+      if (q >= end) continue;
+      Vec v = LoadRowVec<T>(x, q, C, q >= whole);
+      if (kMarked) DropMarked<T>(&v, MarksOf<T>(bits, VecBase<T>(q, C), first * kN));
+#pragma unroll
+      for (int e = 0; e < kN; ++e) {
+        const float d = (ElementOf<T>(v, e) - r.m) * c, p = Exp2(d);
+        s[e & 3] += p;
+        if (kEntropy) t[e & 3] += fmaxf(d, kNothing) * p;
+      }
+    }
+    r.s = (s[0] + s[1]) + (s[2] + s[3]);
+    r.t = (t[0] + t[1]) + (t[2] + t[3]);
+  } else {
+    if (r.m == Real<float>::NegInf()) r.m = 0.0f;
+    const float off = __builtin_fmaf(r.m, c, -reference), scale = Exp2(-off);
+    r.s = (s[0] + s[1]) + (s[2] + s[3]);
+    r.t = (((t[0] + t[1]) + (t[2] + t[3])) - off * r.s) * scale;
+    r.s *= scale;
+  }
+  return JoinLanes(r, c);
+}
+
 // The order of alternatives as one whole number: the larger logit first (a NaN before everything, -0 and 0 alike), the
 // lower index first where logits are equal.  Never 0 for an element of a row.
 __device__ __forceinline__ unsigned OrderOf(float x) {
@@ -333,21 +448,27 @@ inline bool RowsOk(long long rows, long long row_stride, int C, float temperatur
 }
 inline bool RowsServed(long long rows, int C) { return rows < (1ll << 31) && C <= kMaxColumns; }
 
-// How a row of more than 256 vectors is held by workgroups of four wavefronts: in `rounds` vectors a lane, in parts where
-// that does not hold it.
+// How rows of more than 256 vectors are cut into parts, each for a workgroup of four wavefronts.
 struct LongShape {
-  int rounds, parts;
+  int vecs;   // of a part
+  int parts;
 };
-inline LongShape LongShapeOf(long long rows, int vecs) {
-  // 16 vectors a lane hold 4096 vectors; parts of 1024 where that alone would leave compute units without work
-  const int whole = (vecs + 16 * 4 * kWave - 1) / (16 * 4 * kWave), fine = (vecs + 4 * 4 * kWave - 1) / (4 * 4 * kWave);
-  if (fine == 1) return LongShape{4, 1};
-  if (rows * whole < 256 && fine <= 64) return LongShape{4, fine};
-  return LongShape{16, whole};
+// Rows that are read along (no alternatives): whole up to kPartColumns (a lane then adds up 256 terms, in four sums; the
+// marks of a part take 8 KB of LDS), unless that leaves compute units without work.
+constexpr int kPartColumns = 1 << 16;
+inline LongShape StreamShapeOf(long long rows, int vecs, int vec) {
+  const int max_vecs = kPartColumns / vec;
+  long long parts = (vecs + max_vecs - 1) / max_vecs;
+  const long long wanted = (1024 + rows - 1) / rows, finest = (vecs + 1023) / 1024;
+  if (parts < wanted) parts = wanted < finest ? wanted : finest;
+  if (parts > 64) parts = 64;
+  const int each = (int)(((vecs + parts - 1) / parts + 255) / 256 * 256);
+  return LongShape{each, (vecs + each - 1) / each};
 }
-inline int PartsOf(long long rows, int C, int dtype) {
-  const int vecs = dtype == K2AMD_F32 ? VecsOf<float>(C) : VecsOf<Half>(C);
-  return vecs <= 4 * kWave ? 1 : LongShapeOf(rows, vecs).parts;
+// Rows that are held: 16 vectors a lane hold 4096 vectors; parts of 1024 where that would leave compute units without work.
+inline LongShape HeldShapeOf(long long rows, int vecs) {
+  const int whole = (vecs + 4095) / 4096, fine = (vecs + 1023) / 1024;
+  return fine == 1 || (rows * whole < 256 && fine <= 64) ? LongShape{1024, fine} : LongShape{4096, whole};
 }
 inline bool Misaligned(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; }  // of what is accessed by 16 bytes
 

@@ -204,17 +204,18 @@ def test_entry_points_refuse_before_launching():
         return lib.k2amd_distillation_forward(x, 8, a, a, None, out, None, rows, C, K, 0, tau, dtype, None, 0, None)
 
     assert distill(rows=0) == 0 and distill(K=257) == 2 and distill(rows=1 << 31) == 2
-    assert distill(C=200000) == 3 and lib.k2amd_distillation_scratch_bytes(3000, 40000, 2) == 3000 * 2 * 8
+    assert distill(C=200000) == 3 and lib.k2amd_distillation_scratch_bytes(3000, 100000, 2) == 3000 * 2 * 8
     assert [distill(rows=-1), distill(C=0), distill(K=-1), distill(tau=0.0), distill(dtype=1), distill(x=None), distill(a=None),
             distill(out=None)] == [1] * 8
     back = lambda per, g=one: lib.k2amd_distillation_backward(one, 8, one, one, one, g, per, None, 1.0, one, 1, 8, 1, 0, 1.0, 0, None)  # noqa: E731
     assert back(0) == 1 and back(1, None) == 1
     assert lib.k2amd_token_logprobs_backward(one, 8, None, None, one, None, None, one, None, None, one, 1, 8, 1, 0, 1.0, 0, None) == 1
     assert lib.k2amd_token_logprobs_backward(one, 8, one, None, one, None, None, None, one, None, one, 1, 8, 1, 0, 1.0, 0, None) == 1
-    assert lib.k2amd_distillation_sum(one, None, one, None, 1, 10, 0, 1.0, one, 8, None) == 3
+    assert lib.k2amd_distillation_sum(one, None, one, None, 1, 20000, 0, 1.0, ok, 31, None) == 3
+    assert lib.k2amd_distillation_sum(one, None, one, None, 1, 20000, 0, 1.0, one, 32, None) == 3
     assert lib.k2amd_distillation_sum(one, None, one, None, 1, -1, 0, 1.0, one, 8, None) == 1
     assert lib.k2amd_distillation_sum(None, None, None, None, 0, 0, 0, 1.0, None, 0, None) == 0
-    assert lib.k2amd_distillation_sum_scratch_bytes(2, 10) == 32
+    assert lib.k2amd_distillation_sum_scratch_bytes(2, 10) == 0 and lib.k2amd_distillation_sum_scratch_bytes(2, 20000) == 64
     assert lib.k2amd_rnnt_pruned_mask(None, None, None, 0, 3, 3, None) == 0
     assert lib.k2amd_rnnt_pruned_mask(None, None, None, 1, 3, 3, None) == 1
     assert lib.k2amd_rnnt_pruned_mask(one, one, one, 1 << 20, 1 << 11, 1, None) == 2
