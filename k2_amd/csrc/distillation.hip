@@ -350,7 +350,7 @@ struct RowGrad {
 };
 
 // The elements of the vectors that a group of lanes holds.
-template <typename T, int U, int W, int L, bool kRest>
+template <bool kPast, typename T, int U, int W, int L, bool kRest>
 __device__ __forceinline__ void WriteUnlisted(RowPart<T, U, W, L> &part, T *dx, int C, int first, int wave, int lane,
                                               const RowGrad<kRest> &f, float c, bool there) {
   constexpr int kN = Lanes<T>::kN;
@@ -363,7 +363,7 @@ __device__ __forceinline__ void WriteUnlisted(RowPart<T, U, W, L> &part, T *dx, 
 #pragma unroll
     for (int e = 0; e < kN; ++e) g[e] = f.skipped ? 0.0f : f.Unlisted(ElementOf<T>(part.v[u], e), c);
     if (q < whole) {
-      StoreVec(dx + (size_t)q * kN, PackOf<T>(g));
+      StoreVec<kPast>(dx + (size_t)q * kN, PackOf<T>(g));
     } else {  // the incomplete last vector, element by element
       const int base = VecBase<T>(q, C);
 #pragma unroll
@@ -409,13 +409,13 @@ __global__ __launch_bounds__(kThreads) void DistillShortGradKernel(const T *__re
     token[j] = given >= 0 && given < a.C && there && !f.skipped ? (int)given : -1;
     q[j] = expf(a.top_logprobs[row * a.K + j] - f.lse);
   }
-  WriteUnlisted(part, dx, a.C, 0, 0, lane, f, a.c, there);
+  WriteUnlisted<false>(part, dx, a.C, 0, 0, lane, f, a.c, there);
   // (the stores above, and the list, are before what follows for every lane of the wavefront)
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   WriteListed(x, dx, token, q, a.K, 0, a.C, lane, kShort, f, a.c);
 }
 
-template <typename T, int U, int W, bool kRest>
+template <typename T, int U, int W, bool kRest, bool kPast>
 __global__ __launch_bounds__(W *kWave) void DistillLongGradKernel(const T *__restrict__ logits, T *__restrict__ logits_grad,
                                                                   long long row0, long long rows, BackwardArgs a) {
   constexpr int kN = Lanes<T>::kN;
@@ -428,13 +428,13 @@ __global__ __launch_bounds__(W *kWave) void DistillLongGradKernel(const T *__res
   T *dx = logits_grad + row * (size_t)a.C;
   const RowGrad<kRest> f(*reinterpret_cast<const float4 *>(a.records + 4 * row), a.scale.At(row), a.c);
   RowPart<T, U, W> part;
-  part.Load(x, f.skipped ? 0 : a.C, first, wave, lane);
+  part.template Load<kPast>(x, f.skipped ? 0 : a.C, first, wave, lane);
   for (int j = threadIdx.x; j < a.K; j += W * kWave) {
     const int64_t given = a.top_tokens[row * a.K + j];
     token[j] = given >= 0 && given < a.C && !f.skipped ? (int)given : -1;
     q[j] = expf(a.top_logprobs[row * a.K + j] - f.lse);
   }
-  WriteUnlisted(part, dx, a.C, first, wave, lane, f, a.c, true);
+  WriteUnlisted<kPast>(part, dx, a.C, first, wave, lane, f, a.c, true);
   __syncthreads();
   const long long end = (long long)(first + U * W * kWave) * kN;
   WriteListed(x, dx, token, q, a.K, first * kN, (int)min((long long)a.C, end), (int)threadIdx.x, W * kWave, f, a.c);
@@ -554,6 +554,7 @@ int ForwardOf(const T *logits, long long rows, const ForwardArgs &a, hipStream_t
 template <typename T, bool kRest>
 int BackwardOf(const T *logits, T *grad, long long rows, const BackwardArgs &a, hipStream_t stream) {
   const int vecs = VecsOf<T>(a.C);
+  const bool past = PastCache(rows, a.C, sizeof(T));
   for (long long done = 0; done < rows; done += kRowsPerLaunch) {
     const long long n = rows - done < kRowsPerLaunch ? rows - done : kRowsPerLaunch, row0 = rows - done - n;
     const dim3 short_grid((unsigned)((n + kShortRows - 1) / kShortRows)), block(kThreads);
@@ -563,7 +564,8 @@ int BackwardOf(const T *logits, T *grad, long long rows, const BackwardArgs &a, 
     else if (vecs <= 4 * kShort) hipLaunchKernelGGL((DistillShortGradKernel<T, 4, kRest>), short_grid, block, lds, stream, logits, grad, row0, n, a);
     else if (vecs <= 8 * kShort) hipLaunchKernelGGL((DistillShortGradKernel<T, 8, kRest>), short_grid, block, lds, stream, logits, grad, row0, n, a);
     else if (vecs <= 16 * kShort) hipLaunchKernelGGL((DistillShortGradKernel<T, 16, kRest>), short_grid, block, lds, stream, logits, grad, row0, n, a);
-    else hipLaunchKernelGGL((DistillLongGradKernel<T, 4, 4, kRest>), grid, block, 0, stream, logits, grad, row0, n, a);
+    else if (past) hipLaunchKernelGGL((DistillLongGradKernel<T, 4, 4, kRest, true>), grid, block, 0, stream, logits, grad, row0, n, a);
+    else hipLaunchKernelGGL((DistillLongGradKernel<T, 4, 4, kRest, false>), grid, block, 0, stream, logits, grad, row0, n, a);
   }
   return LaunchStatus();
 }

@@ -192,35 +192,175 @@ __device__ __forceinline__ void WriteRow(const ForwardArgs &a, size_t row, int i
   }
 }
 
-// W wavefronts a row (or a part of it), W == 1: four rows a workgroup.  kEntropy: whether t is summed up.
+// Short rows: 16 lanes each, four rows a wavefront.  What a row depends on (mask, tokens) is asked for first and together, then
+// the row.  Every vector of a row is a group of the threshold's; each row has a threshold of its own, so that the counting is
+// done in the 16 lanes of the row.  A lane collects which of its elements reach it in bits and then lists them one after the
+// other, reading each again (it is in the nearest cache): the list's code is run as often as the busiest lane has elements in
+// it, not once for each place of an element in a lane.
+constexpr int kShort = 16, kShortRows = 16;
+constexpr int kThreads = kShort * kShortRows;
+
+template <int U>
+__device__ __forceinline__ int RowGroupsReaching(const float (&group)[U], float v) {
+  float n = 0.0f;
+#pragma unroll
+  for (int u = 0; u < U; ++u) n += group[u] >= v ? 1.0f : 0.0f;
+  return (int)GroupSum<kShort>(n);
+}
+
+// as Threshold above, for each of the wavefront's rows
+template <int U>
+__device__ __forceinline__ float RowThreshold(const float (&group)[U], float high, int k) {
+  float lo = high, hi = high;
+  bool found = RowGroupsReaching(group, high) >= k, done = found;
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+    if (__ballot(!found) == 0) continue;
+    const float v = high - (i == 0 ? 8.0f : i == 1 ? 64.0f : 4096.0f);
+    const bool reached = RowGroupsReaching(group, v) >= k;
+    if (!found) (reached ? lo : hi) = v;
+    found |= reached;
+  }
+  if (!found) lo = Real<float>::NegInf();
+  done |= !found;
+  for (int step = 0; step < 24 && __ballot(!done) != 0; ++step) {
+    const float mid = 0.5f * (lo + hi);
+    const int n = RowGroupsReaching(group, mid);
+    if (!done) (n >= k ? lo : hi) = mid;
+    done |= n >= k && n <= k + (k >> 1) + 2;
+  }
+  return lo;
+}
+
+template <typename T, int U, bool kEntropy>
+__global__ __launch_bounds__(kThreads) void TokenShortKernel(const T *__restrict__ logits, long long row0, long long rows,
+                                                             ForwardArgs a) {
+  constexpr int kN = Lanes<T>::kN;
+  __shared__ unsigned long long lists[kShortRows][kListed];
+  __shared__ int listed[kShortRows];
+  const int lane = threadIdx.x % kShort, in_block = threadIdx.x / kShort;
+  const long long in_launch = (long long)blockIdx.x * kShortRows + in_block;
+  if ((in_launch & ~3ll) >= rows) return;  // (the wavefront's first row)
+  const bool there = in_launch < rows;
+  const size_t row = row0 + (there ? in_launch : rows - 1);  // (lanes without a row follow along and write nothing)
+  const uint8_t masked = a.mask == nullptr ? 1 : a.mask[row];
+  int64_t token = lane < a.n ? a.tokens[row * a.n + lane] : -1;
+  const bool live = there && masked != 0;
+  const T *x = logits + row * a.row_stride;
+  RowPart<T, U, 1, kShort> part;
+  part.Load(x, live ? a.C : 0, 0, 0, lane);
+  float x_token = live && token >= 0 && token < a.C ? ToFloat(x[token]) : 0.0f;
+  float group[U], high = Real<float>::NegInf();
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const Vec &v = part.Packed(u);
+    group[u] = Real<float>::NegInf();
+#pragma unroll
+    for (int e = 0; e < kN; e += 2) group[u] = fmaxf(fmaxf(group[u], ElementOf<T>(v, e)), ElementOf<T>(v, e + 1));
+    high = fmaxf(high, group[u]);
+  }
+  high = GroupMax<kShort>(high);
+  const Sums sums = SumsOf<kEntropy>(part, high, a.c);
+  if (there && !live) {
+    for (int i = lane; i < max(max(a.n, a.k), 1); i += kShort) WriteSkippedRow(a, row, i);
+  } else if (there) {
+    WriteRow(a, row, lane, sums, token, x_token);
+    for (int i = lane + kShort; i < a.n; i += kShort) {
+      token = a.tokens[row * a.n + i];
+      x_token = token >= 0 && token < a.C ? ToFloat(x[token]) : 0.0f;
+      WriteRow(a, row, i, sums, token, x_token);
+    }
+  }
+  if (a.k == 0) return;
+
+  unsigned long long *list = lists[in_block];
+  if (lane == 0) listed[in_block] = 0;
+  const bool odd = sums.s != sums.s;  // a NaN or +inf among them
+  const float threshold = RowThreshold<U>(group, live && !odd ? high : Real<float>::NegInf(), live && !odd ? a.k : 0);
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  constexpr int kPerWord = 32 / kN;  // vectors whose elements share a word of bits
+#pragma unroll
+  for (int word = 0; word < (U + kPerWord - 1) / kPerWord; ++word) {
+    unsigned bits = 0;
+#pragma unroll
+    for (int i = 0; i < kPerWord && word * kPerWord + i < U; ++i) {
+      const int u = word * kPerWord + i;
+      if (__ballot(group[u] >= threshold) == 0) continue;
+      const Vec &v = part.Packed(u);
+      unsigned of_vector = 0;
+#pragma unroll
+      for (int e = 0; e < kN; ++e) of_vector |= ElementOf<T>(v, e) >= threshold ? 1u << e : 0u;
+      // (the -inf that pads a row is no element of it)
+      const int q = part.VectorAnew(u, 0, 0, lane), base = VecBase<T>(q, a.C);
+      of_vector &= q < VecsOf<T>(a.C) ? ((1u << kN) - 1) << min(kN, q * kN - base) : 0u;
+      if (base + kN > a.C) of_vector &= (1u << (a.C - base)) - 1;
+      bits |= of_vector << (i * kN);
+    }
+    if (!live || odd) bits = 0;
+    int at = bits != 0 ? atomicAdd(&listed[in_block], __popc(bits)) : 0;
+    while (__ballot(bits != 0) != 0) {
+      if (bits != 0) {
+        const int bit = __ffs((int)bits) - 1, q = part.Vector(word * kPerWord + bit / kN, 0, 0, lane);
+        const int index = VecBase<T>(q, a.C) + bit % kN;
+        if (at < kListed) list[at] = KeyOf(ToFloat(x[index]), (unsigned)index);
+        ++at;
+        bits &= bits - 1;
+      }
+    }
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  // rows that list too much, or NaNs: by the whole wavefront, one after the other
+  const unsigned long long again = __ballot(live && (odd || listed[in_block] > kListed));
+  if (again != 0) {
+    for (int g = 0; g < kWave / kShort; ++g) {
+      if ((again >> (g * kShort) & 1) == 0) continue;
+      const int other = in_block / 4 * 4 + g, wave_lane = threadIdx.x & (kWave - 1);
+      RowPart<T, (U + 3) / 4, 1> wide;
+      wide.Load(logits + (row0 + (long long)blockIdx.x * kShortRows + other) * a.row_stride, a.C, 0, 0, wave_lane);
+      const int count = ListByClasses<T, (U + 3) / 4, 1>(wide, a.C, 0, 0, wave_lane, a.k, lists[other]);
+      if (wave_lane == 0) listed[other] = count;
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  }
+  if (!live) return;
+  const int count = listed[in_block];
+  const float ls = Log2(sums.s);
+  for (int i = lane; i < count; i += kShort) {
+    const unsigned long long key = list[i];
+    int place = 0;
+    for (int j = 0; j < count; ++j) place += list[j] > key ? 1 : 0;
+    if (place < a.k) {
+      a.top_tokens[row * a.k + place] = IndexOf(key);
+      a.top_logprobs[row * a.k + place] = LogProb(LogitOf(key), sums.m, ls, a.inv_tau);
+    }
+  }
+  for (int i = count + lane; i < a.k; i += kShort) {  // rows shorter than the list
+    a.top_tokens[row * a.k + i] = -1;
+    a.top_logprobs[row * a.k + i] = Real<float>::NegInf();
+  }
+}
+
+// Long rows with alternatives: W wavefronts hold a row or a part of it.  kEntropy: whether t is summed up.
 template <typename T, int U, int W, bool kEntropy>
-__global__ __launch_bounds__(W == 1 ? 4 * kWave : W *kWave) void TokenForwardKernel(const T *__restrict__ logits,
-                                                                                   long long row0, long long rows,
-                                                                                   ForwardArgs a) {
-  constexpr int kN = Lanes<T>::kN, kWaves = W == 1 ? 4 : W;
-  __shared__ unsigned long long lists[kWaves][kListed];
-  __shared__ float4 wave_sums[kWaves];      // of W > 1 wavefronts: m, s, t, the threshold that k of its groups reach
-  __shared__ float wave_low[kWaves];        // and the one that its share of k reach
-  __shared__ int listed[kWaves];
-  const int lane = threadIdx.x & (kWave - 1);
-  const int in_block = __builtin_amdgcn_readfirstlane((int)(threadIdx.x / kWave));
-  const int wave = W == 1 ? 0 : in_block;   // of the row
-  const size_t row = row0 + (W == 1 ? (long long)blockIdx.x * 4 + in_block : (long long)blockIdx.x);
-  if (W == 1 && (long long)row >= row0 + rows) return;
-  const int first = W == 1 ? 0 : (int)blockIdx.y * (U * W * kWave);
+__global__ __launch_bounds__(W *kWave) void TokenHeldKernel(const T *__restrict__ logits, long long row0, ForwardArgs a) {
+  constexpr int kN = Lanes<T>::kN;
+  __shared__ unsigned long long lists[W][kListed];
+  __shared__ float4 wave_sums[W];      // m, s, t, the threshold that k of a wavefront's groups reach
+  __shared__ float wave_low[W];        // and the one that its share of k reach
+  __shared__ int listed[W];
+  const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x / kWave));
+  const size_t row = row0 + blockIdx.x;
+  const int first = (int)blockIdx.y * (U * W * kWave);
   if (a.mask != nullptr && a.mask[row] == 0) {
     if (wave == 0 && blockIdx.y == 0) WriteSkippedRow(a, row, lane);
     return;
   }
   const T *x = logits + row * a.row_stride;
+  // (the tokens in front of the row, the logits that they point to behind it: results of loads come in order)
+  const int64_t token = wave == 0 && a.parts == 1 && lane < a.n ? a.tokens[row * a.n + lane] : -1;
   RowPart<T, U, W> part;
   part.Load(x, a.C, first, wave, lane);
-  int64_t token = -1;
-  float x_token = 0.0f;
-  if (wave == 0 && a.parts == 1 && lane < a.n) {
-    token = a.tokens[row * a.n + lane];
-    if (token >= 0 && token < a.C) x_token = ToFloat(x[token]);
-  }
+  const float x_token = token >= 0 && token < a.C ? ToFloat(x[token]) : 0.0f;
 
   // the wavefront's sums
   constexpr int kGroups = U < 4 ? U : 4;
@@ -241,53 +381,46 @@ __global__ __launch_bounds__(W == 1 ? 4 * kWave : W *kWave) void TokenForwardKer
   Sums sums = SumsOf<kEntropy>(part, high, a.c);
 
   const bool odd = sums.s != sums.s;  // a NaN or +inf among them
-  float threshold = Real<float>::NegInf();
-  if (a.k > 0 && !odd) threshold = Threshold<kGroups>(group, high, a.k, threshold);
-  if (W > 1) {
-    const float low = a.k > 0 && !odd ? Threshold<kGroups>(group, high, (a.k + W - 1) / W, threshold) : threshold;
-    if (lane == 0) {
-      wave_sums[wave] = make_float4(sums.m, sums.s, sums.t, threshold);
-      wave_low[wave] = low;
-    }
-    __syncthreads();
-    // k elements of the part reach every wavefront's own threshold, and the lowest of those that k / W reach in each
-    float lowest = wave_low[0];
-    threshold = Real<float>::NegInf();
-    for (int w = 0; w < W; ++w) {
-      threshold = fmaxf(threshold, wave_sums[w].w);
-      lowest = fminf(lowest, wave_low[w]);
-    }
-    threshold = fmaxf(threshold, lowest);
-    sums = Sums{wave_sums[0].x, wave_sums[0].y, wave_sums[0].z};
-    for (int w = 1; w < W; ++w) sums = Join(sums, Sums{wave_sums[w].x, wave_sums[w].y, wave_sums[w].z}, a.c);
+  float threshold = Real<float>::NegInf(), low = threshold;
+  if (!odd) {
+    threshold = Threshold<kGroups>(group, high, a.k, threshold);
+    low = Threshold<kGroups>(group, high, (a.k + W - 1) / W, threshold);
   }
+  if (lane == 0) {
+    wave_sums[wave] = make_float4(sums.m, sums.s, sums.t, threshold);
+    wave_low[wave] = low;
+  }
+  __syncthreads();
+  // k elements of the part reach every wavefront's own threshold, and the lowest of those that k / W reach in each
+  float lowest = wave_low[0];
+  threshold = Real<float>::NegInf();
+  for (int w = 0; w < W; ++w) {
+    threshold = fmaxf(threshold, wave_sums[w].w);
+    lowest = fminf(lowest, wave_low[w]);
+  }
+  threshold = fmaxf(threshold, lowest);
+  sums = Sums{wave_sums[0].x, wave_sums[0].y, wave_sums[0].z};
+  for (int w = 1; w < W; ++w) sums = Join(sums, Sums{wave_sums[w].x, wave_sums[w].y, wave_sums[w].z}, a.c);
   if (wave == 0) {
     if (a.parts == 1) WriteRow(a, row, lane, sums, token, x_token);
     else if (lane == 0) a.part_sums[row * a.parts + blockIdx.y] = make_float4(sums.m, sums.s, sums.t, 0.0f);
   }
-  if (a.k == 0) return;
-
-  unsigned long long *own = lists[in_block];
+  unsigned long long *own = lists[wave];
   int count = odd ? kListed + 1 : ListReaching<T, U, W>(part, a.C, first, wave, lane, threshold, own);
   if (count > kListed)
     count = ListByClasses<T, U, W>(part, a.C, first, wave, lane, a.k, own);
-  if (W > 1) {
-    if (lane == 0) listed[wave] = count;
-    __syncthreads();
-  } else {
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  }
+  if (lane == 0) listed[wave] = count;
+  __syncthreads();
   // each listed element's place
   const float ls = Log2(sums.s);
   int all = 0;
-  for (int w = 0; w < W; ++w) all += W == 1 ? count : listed[w];
+  for (int w = 0; w < W; ++w) all += listed[w];
   for (int i = lane; i < count; i += kWave) {
     const unsigned long long key = own[i];
     int place = 0;
     for (int w = 0; w < W; ++w) {
-      const unsigned long long *other = W == 1 ? own : lists[w];
-      const int n = W == 1 ? count : listed[w];
-      for (int j = 0; j < n; ++j) place += other[j] > key ? 1 : 0;
+      const int n = listed[w];
+      for (int j = 0; j < n; ++j) place += lists[w][j] > key ? 1 : 0;
     }
     if (place < a.k) {
       if (a.parts == 1) {
@@ -306,6 +439,33 @@ __global__ __launch_bounds__(W == 1 ? 4 * kWave : W *kWave) void TokenForwardKer
       a.part_keys[(row * a.parts + blockIdx.y) * a.k + lane] = 0;
     }
   }
+}
+
+// Long rows without alternatives: four wavefronts read along a row or a part of it.
+constexpr int kStreamWaves = 4;
+template <typename T, bool kEntropy>
+__global__ __launch_bounds__(kStreamWaves *kWave) void TokenStreamKernel(const T *__restrict__ logits, long long row0,
+                                                                        int part_vecs, ForwardArgs a) {
+  __shared__ float4 wave_sums[kStreamWaves];
+  const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x / kWave));
+  const size_t row = row0 + blockIdx.x;
+  const int first = (int)blockIdx.y * part_vecs, end = min(VecsOf<T>(a.C), first + part_vecs);
+  if (a.mask != nullptr && a.mask[row] == 0) {
+    if (wave == 0 && blockIdx.y == 0) WriteSkippedRow(a, row, lane);
+    return;
+  }
+  const T *x = logits + row * a.row_stride;
+  Sums sums = StreamSums<T, kStreamWaves, kEntropy, false>(x, a.C, first, end, wave, lane, a.c, nullptr);
+  if (lane == 0) wave_sums[wave] = make_float4(sums.m, sums.s, sums.t, 0.0f);
+  __syncthreads();
+  if (wave != 0) return;
+  for (int w = 1; w < kStreamWaves; ++w) sums = Join(sums, Sums{wave_sums[w].x, wave_sums[w].y, wave_sums[w].z}, a.c);
+  if (a.parts > 1) {
+    if (lane == 0) a.part_sums[row * a.parts + blockIdx.y] = make_float4(sums.m, sums.s, sums.t, 0.0f);
+    return;
+  }
+  const int64_t token = lane < a.n ? a.tokens[row * a.n + lane] : -1;
+  WriteRow(a, row, lane, sums, token, token >= 0 && token < a.C ? ToFloat(x[token]) : 0.0f);
 }
 
 // How many of the n keys at `keys`, the largest first, are larger than `key` (n <= 64).
@@ -393,65 +553,47 @@ struct SoftmaxGrad {
   }
 };
 
-// W wavefronts take U vectors a lane of a row, or of the stretch of it that blockIdx.y counts; W == 1: four rows a
-// workgroup, each in rounds of U.  The softmax part of every element first; then the entries' own elements over it.
-template <typename T, int U, int W>
-__global__ __launch_bounds__(W == 1 ? 4 * kWave : W *kWave) void TokenBackwardKernel(const T *__restrict__ logits,
-                                                                                    T *__restrict__ logits_grad, long long row0,
-                                                                                    long long rows, BackwardArgs a) {
-  constexpr int kN = Lanes<T>::kN, kWaves = W == 1 ? 4 : W;
-  constexpr int kEntries = kMaxTokens + kMaxTop;
-  __shared__ int entry_lds[kWaves][W == 1 ? kEntries : 1];
-  __shared__ float grad_lds[kWaves][W == 1 ? kEntries : 1];
-  __shared__ int block_entry[W == 1 ? 1 : kEntries];
-  __shared__ float block_grad[W == 1 ? 1 : kEntries];
-  const int lane = threadIdx.x & (kWave - 1);
-  const int in_block = __builtin_amdgcn_readfirstlane((int)(threadIdx.x / kWave));
-  const int wave = W == 1 ? 0 : in_block;
-  // the last row first: of a batch larger than the 256 MB memory-side cache it is the tail that the forward pass left there
-  const long long from_last = W == 1 ? (long long)blockIdx.x * 4 + in_block : (long long)blockIdx.x;
-  if (W == 1 && from_last >= rows) return;
-  const size_t row = row0 + rows - 1 - from_last;
-  const int first = W == 1 ? 0 : (int)blockIdx.y * (U * W * kWave);
-  T *dx = logits_grad + row * (size_t)a.C;
-  const int all = VecsOf<T>(a.C);
-  const bool live = a.mask == nullptr || a.mask[row] != 0;
-  const T *x = logits + row * a.row_stride;
-  RowPart<T, U, W> part;
-  SoftmaxGrad f{0.0f, 0.0f, 0.0f, 0.0f};
-  int *entry = W == 1 ? entry_lds[in_block] : block_entry;
-  float *entry_grad = W == 1 ? grad_lds[in_block] : block_grad;
-  const int used = a.logprobs_grad != nullptr ? a.n : 0, both = live ? used + (a.top_grad != nullptr ? a.k : 0) : 0;
-  if (live) {
-    part.Load(x, a.C, first, wave, lane);
-    float sum = 0.0f;
-    for (int i = lane; i < both; i += kWave) {  // (every wavefront of a row: all need the sum)
-      const bool given = i < used;
-      const int64_t token = given ? a.tokens[row * a.n + i] : a.top_tokens[row * a.k + (i - used)];
-      float g = given ? a.logprobs_grad[row * a.n + i] : a.top_grad[row * a.k + (i - used)];
-      if (token < 0) g = 0.0f;
-      if (token >= a.C) g = __uint_as_float(0x7fc00000u);
-      sum += g;
-      if (wave == 0) {
-        entry[i] = token < 0 || token >= a.C ? -1 : (int)token;
-        entry_grad[i] = g;
-      }
-    }
-    sum = both > 0 ? WaveSumF(sum) : 0.0f;
-    const float s = a.stats[2 * row + 1];
-    const float h = a.entropy_grad != nullptr ? a.entropy[row] : 0.0f;
-    const float gh = a.entropy_grad != nullptr ? a.entropy_grad[row] : 0.0f;
-    f.m = a.stats[2 * row];
-    f.c = a.c;
-    if (s != 0.0f) {  // (a row without any mass: every p is 0)
-      const float inv_s = a.inv_tau / s;
-      f.flat = -inv_s * (sum + gh * (h - kLn2 * Log2(s)));
-      f.slope = -inv_s * gh * kLn2;
-    } else if (sum != sum) {
-      f.flat = sum;
+// A row's entries in LDS, lane by lane of the n that share it; returns this lane's part of the sum of their gradients.
+__device__ __forceinline__ float ReadEntries(const BackwardArgs &a, size_t row, int i, int n, int entries, int *entry,
+                                             float *entry_grad, bool write) {
+  const int used = a.logprobs_grad != nullptr ? a.n : 0;
+  float sum = 0.0f;
+  for (; i < entries; i += n) {
+    const bool given = i < used;
+    const int64_t token = given ? a.tokens[row * a.n + i] : a.top_tokens[row * a.k + (i - used)];
+    float g = given ? a.logprobs_grad[row * a.n + i] : a.top_grad[row * a.k + (i - used)];
+    if (token < 0) g = 0.0f;
+    if (token >= a.C) g = __uint_as_float(0x7fc00000u);
+    sum += g;
+    if (write) {
+      entry[i] = token < 0 || token >= a.C ? -1 : (int)token;
+      entry_grad[i] = g;
     }
   }
-  const int whole = a.C / kN;
+  return sum;
+}
+
+__device__ __forceinline__ SoftmaxGrad RowGradOf(const BackwardArgs &a, size_t row, float sum) {
+  const float s = a.stats[2 * row + 1];
+  const float h = a.entropy_grad != nullptr ? a.entropy[row] : 0.0f;
+  const float gh = a.entropy_grad != nullptr ? a.entropy_grad[row] : 0.0f;
+  SoftmaxGrad f{a.stats[2 * row], a.c, 0.0f, 0.0f};
+  if (s != 0.0f) {  // (a row without any mass: every p is 0)
+    const float inv_s = a.inv_tau / s;
+    f.flat = -inv_s * (sum + gh * (h - kLn2 * Log2(s)));
+    f.slope = -inv_s * gh * kLn2;
+  } else if (sum != sum) {
+    f.flat = sum;
+  }
+  return f;
+}
+
+// The softmax part of the elements that a group of lanes holds; zeros for rows that do not count.
+template <bool kPast, typename T, int U, int W, int L>
+__device__ __forceinline__ void WriteSoftmaxPart(const RowPart<T, U, W, L> &part, T *dx, int C, int first, int wave, int lane,
+                                                 const SoftmaxGrad &f, bool there, bool live) {
+  constexpr int kN = Lanes<T>::kN;
+  const int whole = C / kN, all = there ? VecsOf<T>(C) : 0;
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const int q = part.Vector(u, first, wave, lane);
@@ -460,47 +602,131 @@ __global__ __launch_bounds__(W == 1 ? 4 * kWave : W *kWave) void TokenBackwardKe
 #pragma unroll
     for (int e = 0; e < kN; ++e) g[e] = live ? f.At(ElementOf<T>(part.v[u], e)) : 0.0f;
     if (q < whole) {
-      StoreVec(dx + (size_t)q * kN, PackOf<T>(g));
+      StoreVec<kPast>(dx + (size_t)q * kN, PackOf<T>(g));
     } else {  // the incomplete last vector, element by element
-      const int base = VecBase<T>(q, a.C);
+      const int base = VecBase<T>(q, C);
 #pragma unroll
       for (int e = 0; e < kN; ++e)
-        if (base + e >= q * kN && base + e < a.C) FromFloat(g[e], &dx[base + e]);
+        if (base + e >= q * kN && base + e < C) FromFloat(g[e], &dx[base + e]);
     }
   }
-  if (both == 0) return;
-  // (the stores above are before the ones below for every lane of the wavefront or workgroup)
-  if (W == 1) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  else __syncthreads();
-  const int begin = first * kN, end = min((long long)a.C, (long long)(first + U * W * kWave) * kN);
-  for (int i = W == 1 ? lane : (int)threadIdx.x; i < both; i += W * kWave) {
+}
+
+// The entries' own elements of columns [begin, end), over what is there.
+template <typename T>
+__device__ __forceinline__ void WriteEntries(const T *x, T *dx, const int *entry, const float *entry_grad, int entries, int begin,
+                                             int end, int i, int n, const SoftmaxGrad &f, float inv_tau) {
+  for (; i < entries; i += n) {
     const int token = entry[i];
     if (token < begin || token >= end) continue;
     float own = 0.0f;  // a token that is listed twice takes both gradients
-    for (int j = 0; j < both; ++j)
+    for (int j = 0; j < entries; ++j)
       if (entry[j] == token) own += entry_grad[j];
-    FromFloat(f.At(ToFloat(x[token])) + own * a.inv_tau, &dx[token]);
+    FromFloat(f.At(ToFloat(x[token])) + own * inv_tau, &dx[token]);
   }
+}
+
+__device__ __forceinline__ int EntriesOf(const BackwardArgs &a) {
+  return (a.logprobs_grad != nullptr ? a.n : 0) + (a.top_grad != nullptr ? a.k : 0);
+}
+
+template <typename T, int U>
+__global__ __launch_bounds__(kThreads) void TokenShortGradKernel(const T *__restrict__ logits, T *__restrict__ logits_grad,
+                                                                 long long row0, long long rows, BackwardArgs a) {
+  HIP_DYNAMIC_SHARED(float, entries_lds)
+  const int lane = threadIdx.x % kShort, in_block = threadIdx.x / kShort, entries = EntriesOf(a);
+  // the last row first: of a batch larger than the 256 MB memory-side cache it is the tail that the forward pass left there
+  const long long from_last = (long long)blockIdx.x * kShortRows + in_block;
+  if ((from_last & ~3ll) >= rows) return;  // (the wavefront's first row)
+  const bool there = from_last < rows;
+  const size_t row = row0 + (there ? rows - 1 - from_last : 0);  // (lanes without a row follow along and write nothing)
+  const bool live = there && (a.mask == nullptr || a.mask[row] != 0);
+  const T *x = logits + row * a.row_stride;
+  T *dx = logits_grad + row * (size_t)a.C;
+  float *entry_grad = entries_lds + (size_t)in_block * 2 * entries;
+  int *entry = reinterpret_cast<int *>(entry_grad + entries);
+  const float sum = GroupSum<kShort>(ReadEntries(a, row, lane, kShort, live ? entries : 0, entry, entry_grad, true));
+  RowPart<T, U, 1, kShort> part;
+  part.Load(x, live ? a.C : 0, 0, 0, lane);
+  const SoftmaxGrad f = RowGradOf(a, row, sum);
+  WriteSoftmaxPart<false>(part, dx, a.C, 0, 0, lane, f, there, live);
+  // (the stores above, and the list, are before what follows for every lane of the wavefront)
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  WriteEntries(x, dx, entry, entry_grad, live ? entries : 0, 0, a.C, lane, kShort, f, a.inv_tau);
+}
+
+// Longer rows: W wavefronts take U vectors a lane of the stretch of a row that blockIdx.y counts.
+template <typename T, int U, int W, bool kPast>
+__global__ __launch_bounds__(W *kWave) void TokenLongGradKernel(const T *__restrict__ logits, T *__restrict__ logits_grad,
+                                                                long long row0, long long rows, BackwardArgs a) {
+  constexpr int kN = Lanes<T>::kN;
+  __shared__ int entry[kMaxTokens + kMaxTop];
+  __shared__ float entry_grad[kMaxTokens + kMaxTop];
+  const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x / kWave));
+  const int entries = EntriesOf(a);
+  const size_t row = row0 + rows - 1 - blockIdx.x;  // (the last row first, as above)
+  const int first = (int)blockIdx.y * (U * W * kWave);
+  const bool live = a.mask == nullptr || a.mask[row] != 0;
+  const T *x = logits + row * a.row_stride;
+  T *dx = logits_grad + row * (size_t)a.C;
+  RowPart<T, U, W> part;
+  SoftmaxGrad f{0.0f, 0.0f, 0.0f, 0.0f};
+  if (live) {
+    // (every wavefront needs the sum; the first leaves the list)
+    const float sum = WaveSumF(ReadEntries(a, row, lane, kWave, entries, entry, entry_grad, wave == 0));
+    part.template Load<kPast>(x, a.C, first, wave, lane);
+    f = RowGradOf(a, row, sum);
+  }
+  WriteSoftmaxPart<kPast>(part, dx, a.C, first, wave, lane, f, true, live);
+  if (!live || entries == 0) return;
+  __syncthreads();
+  const long long end = (long long)(first + U * W * kWave) * kN;
+  WriteEntries(x, dx, entry, entry_grad, entries, first * kN, (int)min((long long)a.C, end), (int)threadIdx.x, W * kWave, f,
+               a.inv_tau);
 }
 
 // ---- launches ---------------------------------------------------------------------------------------
 
-template <typename T, int U, int W>
-void LaunchForward(const T *logits, long long rows, bool entropy, const ForwardArgs &a, hipStream_t stream) {
+template <typename T, int U>
+void LaunchShort(const T *logits, long long rows, bool entropy, const ForwardArgs &a, hipStream_t stream) {
   for (long long row0 = 0; row0 < rows; row0 += kRowsPerLaunch) {
     const long long n = rows - row0 < kRowsPerLaunch ? rows - row0 : kRowsPerLaunch;
-    const dim3 grid((unsigned)(W == 1 ? (n + 3) / 4 : n), (unsigned)a.parts), block(W == 1 ? 4 * kWave : W * kWave);
-    if (entropy) hipLaunchKernelGGL((TokenForwardKernel<T, U, W, true>), grid, block, 0, stream, logits, row0, n, a);
-    else hipLaunchKernelGGL((TokenForwardKernel<T, U, W, false>), grid, block, 0, stream, logits, row0, n, a);
+    const dim3 grid((unsigned)((n + kShortRows - 1) / kShortRows)), block(kThreads);
+    if (entropy) hipLaunchKernelGGL((TokenShortKernel<T, U, true>), grid, block, 0, stream, logits, row0, n, a);
+    else hipLaunchKernelGGL((TokenShortKernel<T, U, false>), grid, block, 0, stream, logits, row0, n, a);
+  }
+}
+
+template <typename T, int U, int W>
+void LaunchHeld(const T *logits, long long rows, bool entropy, const ForwardArgs &a, hipStream_t stream) {
+  for (long long row0 = 0; row0 < rows; row0 += kRowsPerLaunch) {
+    const long long n = rows - row0 < kRowsPerLaunch ? rows - row0 : kRowsPerLaunch;
+    const dim3 grid((unsigned)n, (unsigned)a.parts), block(W * kWave);
+    if (entropy) hipLaunchKernelGGL((TokenHeldKernel<T, U, W, true>), grid, block, 0, stream, logits, row0, a);
+    else hipLaunchKernelGGL((TokenHeldKernel<T, U, W, false>), grid, block, 0, stream, logits, row0, a);
     if (a.parts > 1)
       hipLaunchKernelGGL(TokenJoinKernel<T>, dim3((unsigned)n), dim3(kJoinThreads),
                          (size_t)a.parts * a.k * sizeof(unsigned long long), stream, logits, row0, a);
   }
 }
 
-int PartsOf(long long rows, int C, int dtype) {
+template <typename T>
+void LaunchStream(const T *logits, long long rows, bool entropy, const ForwardArgs &a, hipStream_t stream) {
+  const int part_vecs = StreamShapeOf(rows, VecsOf<T>(a.C), Lanes<T>::kN).vecs;
+  for (long long row0 = 0; row0 < rows; row0 += kRowsPerLaunch) {
+    const long long n = rows - row0 < kRowsPerLaunch ? rows - row0 : kRowsPerLaunch;
+    const dim3 grid((unsigned)n, (unsigned)a.parts), block(kStreamWaves * kWave);
+    if (entropy) hipLaunchKernelGGL((TokenStreamKernel<T, true>), grid, block, 0, stream, logits, row0, part_vecs, a);
+    else hipLaunchKernelGGL((TokenStreamKernel<T, false>), grid, block, 0, stream, logits, row0, part_vecs, a);
+    if (a.parts > 1)
+      hipLaunchKernelGGL(TokenJoinKernel<T>, dim3((unsigned)n), dim3(kJoinThreads), 0, stream, logits, row0, a);
+  }
+}
+
+int PartsOf(long long rows, int C, int k, int dtype) {
   const int vecs = dtype == K2AMD_F32 ? VecsOf<float>(C) : VecsOf<Half>(C);
-  return vecs <= 4 * kWave ? 1 : HeldShapeOf(rows, vecs).parts;
+  if (vecs <= 16 * kShort || rows == 0) return 1;
+  return k > 0 ? HeldShapeOf(rows, vecs).parts : StreamShapeOf(rows, vecs, dtype == K2AMD_F32 ? 4 : 8).parts;
 }
 
 template <typename T>
@@ -508,33 +734,33 @@ int Forward(const void *logits_v, long long rows, ForwardArgs a, hipStream_t str
   const T *logits = static_cast<const T *>(logits_v);
   const int vecs = VecsOf<T>(a.C);
   const bool entropy = a.entropy != nullptr;
-  if (vecs <= kWave) LaunchForward<T, 1, 1>(logits, rows, entropy, a, stream);
-  else if (vecs <= 2 * kWave) LaunchForward<T, 2, 1>(logits, rows, entropy, a, stream);
-  else if (vecs <= 4 * kWave) LaunchForward<T, 4, 1>(logits, rows, entropy, a, stream);
-  else if (HeldShapeOf(rows, vecs).vecs == 1024) LaunchForward<T, 4, 4>(logits, rows, entropy, a, stream);
-  else LaunchForward<T, 16, 4>(logits, rows, entropy, a, stream);
+  if (vecs <= 2 * kShort) LaunchShort<T, 2>(logits, rows, entropy, a, stream);
+  else if (vecs <= 4 * kShort) LaunchShort<T, 4>(logits, rows, entropy, a, stream);
+  else if (vecs <= 8 * kShort) LaunchShort<T, 8>(logits, rows, entropy, a, stream);
+  else if (vecs <= 16 * kShort) LaunchShort<T, 16>(logits, rows, entropy, a, stream);
+  else if (a.k == 0) LaunchStream<T>(logits, rows, entropy, a, stream);
+  else if (HeldShapeOf(rows, vecs).vecs == 1024) LaunchHeld<T, 4, 4>(logits, rows, entropy, a, stream);
+  else LaunchHeld<T, 16, 4>(logits, rows, entropy, a, stream);
   return LaunchStatus();
-}
-
-template <typename T, int U, int W>
-void LaunchBackward(const T *logits, T *logits_grad, long long rows, const BackwardArgs &a, hipStream_t stream) {
-  const int stretches = W == 1 ? 1 : (VecsOf<T>(a.C) + U * W * kWave - 1) / (U * W * kWave);
-  for (long long done = 0; done < rows; done += kRowsPerLaunch) {
-    const long long n = rows - done < kRowsPerLaunch ? rows - done : kRowsPerLaunch;
-    const dim3 grid((unsigned)(W == 1 ? (n + 3) / 4 : n), (unsigned)stretches), block(W == 1 ? 4 * kWave : W * kWave);
-    hipLaunchKernelGGL((TokenBackwardKernel<T, U, W>), grid, block, 0, stream, logits, logits_grad, rows - done - n, n, a);
-  }
 }
 
 template <typename T>
 int Backward(const void *logits_v, void *grad_v, long long rows, const BackwardArgs &a, hipStream_t stream) {
   const T *logits = static_cast<const T *>(logits_v);
   T *grad = static_cast<T *>(grad_v);
-  const int vecs = VecsOf<T>(a.C);
-  if (vecs <= kWave) LaunchBackward<T, 1, 1>(logits, grad, rows, a, stream);
-  else if (vecs <= 2 * kWave) LaunchBackward<T, 2, 1>(logits, grad, rows, a, stream);
-  else if (vecs <= 4 * kWave) LaunchBackward<T, 4, 1>(logits, grad, rows, a, stream);
-  else LaunchBackward<T, 4, 4>(logits, grad, rows, a, stream);
+  const int vecs = VecsOf<T>(a.C), entries = (a.logprobs_grad != nullptr ? a.n : 0) + (a.top_grad != nullptr ? a.k : 0);
+  for (long long done = 0; done < rows; done += kRowsPerLaunch) {
+    const long long n = rows - done < kRowsPerLaunch ? rows - done : kRowsPerLaunch, row0 = rows - done - n;
+    const dim3 short_grid((unsigned)((n + kShortRows - 1) / kShortRows)), block(kThreads);
+    const dim3 grid((unsigned)n, (unsigned)((vecs + 16 * kWave - 1) / (16 * kWave)));
+    const size_t lds = (size_t)kShortRows * 2 * entries * sizeof(float);
+    if (vecs <= 2 * kShort) hipLaunchKernelGGL((TokenShortGradKernel<T, 2>), short_grid, block, lds, stream, logits, grad, row0, n, a);
+    else if (vecs <= 4 * kShort) hipLaunchKernelGGL((TokenShortGradKernel<T, 4>), short_grid, block, lds, stream, logits, grad, row0, n, a);
+    else if (vecs <= 8 * kShort) hipLaunchKernelGGL((TokenShortGradKernel<T, 8>), short_grid, block, lds, stream, logits, grad, row0, n, a);
+    else if (vecs <= 16 * kShort) hipLaunchKernelGGL((TokenShortGradKernel<T, 16>), short_grid, block, lds, stream, logits, grad, row0, n, a);
+    else if (PastCache(rows, a.C, sizeof(T))) hipLaunchKernelGGL((TokenLongGradKernel<T, 4, 4, true>), grid, block, 0, stream, logits, grad, row0, n, a);
+    else hipLaunchKernelGGL((TokenLongGradKernel<T, 4, 4, false>), grid, block, 0, stream, logits, grad, row0, n, a);
+  }
   return LaunchStatus();
 }
 
@@ -547,7 +773,7 @@ extern "C" {
 
 size_t k2amd_token_logprobs_scratch_bytes(long long rows, int C, int k, int dtype) {
   if (rows < 0 || C < 1 || k < 0 || C > kMaxColumns || k > kMaxTop) return 0;
-  const size_t parts = PartsOf(rows, C, dtype);
+  const size_t parts = PartsOf(rows, C, k, dtype);
   return parts <= 1 ? 0 : ((size_t)rows * parts * (sizeof(float4) + (size_t)k * sizeof(unsigned long long)) + 15) / 16 * 16;
 }
 
@@ -561,7 +787,7 @@ int k2amd_token_logprobs_forward(const void *logits, long long row_stride, const
   if (logits == nullptr || (n > 0 && (tokens == nullptr || logprobs == nullptr)) ||
       (k > 0 && (top_logprobs == nullptr || top_tokens == nullptr)))
     return K2AMD_ERR_INVALID_ARGUMENT;
-  const int parts = PartsOf(rows, C, dtype);
+  const int parts = PartsOf(rows, C, k, dtype);
   if (parts > 1 && (scratch == nullptr || Misaligned(scratch) || scratch_bytes < k2amd_token_logprobs_scratch_bytes(rows, C, k, dtype)))
     return K2AMD_ERR_WORKSPACE;
   float4 *sums = static_cast<float4 *>(scratch);

@@ -68,6 +68,7 @@ __device__ __forceinline__ unsigned Anew(unsigned v) {
 struct Vec {
   unsigned w[4];
 };
+typedef unsigned VecAnywhere __attribute__((ext_vector_type(4), aligned(2)));
 template <typename T>
 struct Lanes {
   static constexpr int kN = 16 / sizeof(T);
@@ -100,12 +101,32 @@ __device__ __forceinline__ Vec PackOf(const float *f) {
   }
   return v;
 }
+// kPast: past the caches, for what is larger than they are
+template <bool kPast = false>
 __device__ __forceinline__ Vec LoadVec(const void *p) {
   Vec v;
-  __builtin_memcpy(&v, p, 16);
+  if (kPast) {
+    const VecAnywhere w = __builtin_nontemporal_load(static_cast<const VecAnywhere *>(p));
+    __builtin_memcpy(&v, &w, 16);
+  } else {
+    __builtin_memcpy(&v, p, 16);
+  }
   return v;
 }
-__device__ __forceinline__ void StoreVec(void *p, const Vec &v) { __builtin_memcpy(p, &v, 16); }
+template <bool kPast>
+__device__ __forceinline__ void StoreVec(void *p, const Vec &v) {
+  if (kPast) {
+    const VecAnywhere w = {v.w[0], v.w[1], v.w[2], v.w[3]};
+    __builtin_nontemporal_store(w, static_cast<VecAnywhere *>(p));
+  } else {
+    __builtin_memcpy(p, &v, 16);
+  }
+}
+// Whether a backward pass reads its logits and writes their gradient past the 256 MB memory-side cache.  The gradient would
+// push the logits out of it that the pass has still to read (the end of what the forward pass read), and the logits, read
+// for the last time, what else there is: 8191 x 32000 bfloat16 forward and backward take 234 us instead of 294, 8192 x 32000
+// distilled 300 instead of 337.  A gradient that fits is better left there: 64000 x 500 float32 137 us instead of 157.
+inline bool PastCache(long long rows, int C, size_t element) { return (double)rows * C * element > 268435456.0; }
 
 // vectors of a row
 template <typename T>
@@ -166,6 +187,7 @@ struct RowPart {
   __device__ __forceinline__ static int VectorAnew(int u, int first, int wave, int lane) {
     return (int)Anew((unsigned)Vector(u, first, wave, lane));
   }
+  template <bool kPast = false>
   __device__ __forceinline__ void Load(const T *x, int C, int first, int wave, int lane) {
     const int whole = C / Lanes<T>::kN, all = VecsOf<T>(C);
 #pragma unroll
@@ -174,7 +196,7 @@ struct RowPart {
       const int q_last = first + (u * W + wave) * L + L - 1;  // the same in every lane
 #pragma unroll
       for (int i = 0; i < 4; ++i) v[u].w[i] = Lanes<T>::kNegInf;
-      if (q_last < whole) v[u] = LoadRowVec<T>(x, q, C, false);
+      if (q_last < whole) v[u] = LoadVec<kPast>(x + q * Lanes<T>::kN);
       else if (q < all) v[u] = LoadRowVec<T>(x, q, C, true);
     }
   }

@@ -405,6 +405,8 @@ inline unsigned long long __ballot(int predicate) {
   }
   return ((unsigned long long)r[1] << 32) | r[0];
 }
+inline int __popc(unsigned v) { return __builtin_popcount(v); }
+inline int __ffs(int v) { return __builtin_ffs(v); }
 inline int __popcll(unsigned long long v) { return __builtin_popcountll(v); }
 // v_mbcnt: how many bits of the mask's half are below this lane, plus a
 inline unsigned __builtin_amdgcn_mbcnt_lo(unsigned mask, unsigned a) {

@@ -49,6 +49,10 @@ TOKEN_ROWS_EDITS = [
     ("return static_cast<float>(__builtin_bit_cast(_Float16, u));", "return __half2float(__half{u});", 1),
     ("return __builtin_bit_cast(unsigned short, static_cast<_Float16>(f));", "return hip_threads_to_half(f);", 1),
     ("return __builtin_bit_cast(unsigned short, static_cast<__bf16>(f));", "return hip_threads_to_bf16(f);", 1),
+    # 16 bytes at any address, as an integer vector, and accesses past the caches
+    ("typedef unsigned VecAnywhere __attribute__((ext_vector_type(4), aligned(2)));", "typedef struct { unsigned x, y, z, w; } VecAnywhere;", 1),
+    ("const VecAnywhere w = __builtin_nontemporal_load(static_cast<const VecAnywhere *>(p));", "VecAnywhere w; __builtin_memcpy(&w, p, 16);", 1),
+    ("__builtin_nontemporal_store(w, static_cast<VecAnywhere *>(p));", "__builtin_memcpy(p, &w, 16);", 1),
     # an empty statement that only hides a value from the compiler
     ('asm volatile("" : "+v"(v));', ";", 1),
 ]
