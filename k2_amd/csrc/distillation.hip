@@ -349,70 +349,79 @@ struct RowGrad {
   __device__ __forceinline__ float Listed(float x, float q, float c) const { return g * (share * Exp2((x - m) * c) - q); }
 };
 
-// The elements of the vectors that a group of lanes holds.
-template <bool kPast, typename T, int U, int W, int L, bool kRest>
-__device__ __forceinline__ void WriteUnlisted(RowPart<T, U, W, L> &part, T *dx, int C, int first, int wave, int lane,
-                                              const RowGrad<kRest> &f, float c, bool there) {
-  constexpr int kN = Lanes<T>::kN;
-  const int whole = C / kN, all = there ? VecsOf<T>(C) : 0;
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int q = part.Vector(u, first, wave, lane);
-    if (q >= all) continue;
-    float g[kN];
-#pragma unroll
-    for (int e = 0; e < kN; ++e) g[e] = f.skipped ? 0.0f : f.Unlisted(ElementOf<T>(part.v[u], e), c);
-    if (q < whole) {
-      StoreVec<kPast>(dx + (size_t)q * kN, PackOf<T>(g));
-    } else {  // the incomplete last vector, element by element
-      const int base = VecBase<T>(q, C);
-#pragma unroll
-      for (int e = 0; e < kN; ++e)
-        if (base + e >= q * kN && base + e < C) FromFloat(g[e], &dx[base + e]);
-    }
-  }
-}
-
-// The listed elements of columns [begin, end), over what is there: entry j by work-item j mod n.
+// The listed columns of [begin, end) over what is at `to` (column `begin` first), entry j by work-item j mod n; x_first: the
+// logit of its first entry.
 template <typename T, bool kRest>
-__device__ __forceinline__ void WriteListed(const T *x, T *dx, const int *token, const float *q, int K, int begin, int end, int i,
-                                            int n, const RowGrad<kRest> &f, float c) {
+__device__ __forceinline__ void WriteListed(const T *x, T *to, const int *token, const float *q, int K, int begin, int end, int i,
+                                            int n, float x_first, const RowGrad<kRest> &f, float c) {
   for (int j = i; j < K; j += n) {
     const int at = token[j];
     if (at < begin || at >= end) continue;
     float sum = 0.0f;  // a token that is listed twice takes both
     for (int l = 0; l < K; ++l)
       if (token[l] == at) sum += q[l];
-    FromFloat(f.Listed(ToFloat(x[at]), sum, c), &dx[at]);
+    FromFloat(f.Listed(j == i ? x_first : ToFloat(x[at]), sum, c), &to[at - begin]);
   }
 }
 
 template <typename T, int U, bool kRest>
 __global__ __launch_bounds__(kThreads) void DistillShortGradKernel(const T *__restrict__ logits, T *__restrict__ logits_grad,
                                                                    long long row0, long long rows, BackwardArgs a) {
+  constexpr int kStage = StagedVecs<U>();
+  __shared__ Vec stages[kStage > 0 ? kShortRows * kStage : 1];
   HIP_DYNAMIC_SHARED(float, lists)
   const int lane = threadIdx.x % kShort, group = threadIdx.x / kShort;
   // the last row first: of a batch larger than the 256 MB memory-side cache it is the tail that the forward pass left there
   const long long from_last = (long long)blockIdx.x * kShortRows + group;
   if ((from_last & ~3ll) >= rows) return;  // (the wavefront's first row)
   const bool there = from_last < rows;
-  const size_t row = row0 + (there ? rows - 1 - from_last : 0);
+  const size_t row = row0 + (there ? rows - 1 - from_last : 0);  // (a group without a row follows along and writes nothing)
   const T *x = logits + row * a.row_stride;
   T *dx = logits_grad + row * (size_t)a.C;
-  const RowGrad<kRest> f(*reinterpret_cast<const float4 *>(a.records + 4 * row), a.scale.At(row), a.c);
+  // asked for together: the record, the list; then the row and the first listed logits
+  const float4 record = *reinterpret_cast<const float4 *>(a.records + 4 * row);
+  const float scale = a.scale.At(row);
+  int64_t given = -1;
+  float teacher = 0.0f;
+  if (lane < a.K) {
+    given = a.top_tokens[row * a.K + lane];
+    teacher = a.top_logprobs[row * a.K + lane];
+  }
+  const RowGrad<kRest> f(record, scale, a.c);
+  const bool live = there && !f.skipped;
   RowPart<T, U, 1, kShort> part;
-  part.Load(x, f.skipped ? 0 : a.C, 0, 0, lane);
+  part.Load(x, live ? a.C : 0, 0, 0, lane);
+  const bool usable = live && given >= 0 && given < a.C;
+  const float x_first = usable ? ToFloat(x[given]) : 0.0f;
   int *token = reinterpret_cast<int *>(lists) + (size_t)group * 2 * a.K;
   float *q = lists + (size_t)group * 2 * a.K + a.K;
-  for (int j = lane; j < a.K; j += kShort) {
-    const int64_t given = a.top_tokens[row * a.K + j];
-    token[j] = given >= 0 && given < a.C && there && !f.skipped ? (int)given : -1;
+  if (lane < a.K) {
+    token[lane] = usable ? (int)given : -1;
+    q[lane] = expf(teacher - f.lse);
+  }
+  for (int j = lane + kShort; j < a.K; j += kShort) {
+    given = a.top_tokens[row * a.K + j];
+    token[j] = live && given >= 0 && given < a.C ? (int)given : -1;
     q[j] = expf(a.top_logprobs[row * a.K + j] - f.lse);
   }
-  WriteUnlisted<false>(part, dx, a.C, 0, 0, lane, f, a.c, there);
-  // (the stores above, and the list, are before what follows for every lane of the wavefront)
+  const int all = live ? VecsOf<T>(a.C) : 0;
+  T *to = kStage > 0 ? reinterpret_cast<T *>(stages + group * kStage) : dx;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int at = part.Vector(u, 0, 0, lane);
+    if (at < all) WriteVec<false>(to, part.v[u], at, a.C, [&](float xi) { return f.Unlisted(xi, a.c); });
+    else if (there && at < VecsOf<T>(a.C)) StoreZeros<false>(dx, at, a.C);
+  }
+  // (what is written above, and the list, are before what follows for every lane of the wavefront)
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  WriteListed(x, dx, token, q, a.K, 0, a.C, lane, kShort, f, a.c);
+  WriteListed(x, to, token, q, live ? a.K : 0, 0, a.C, lane, kShort, x_first, f, a.c);
+  if (kStage == 0) return;
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int at = part.Vector(u, 0, 0, lane);
+    if (at < all) StoreStaged(to, dx, at, a.C);
+  }
 }
 
 template <typename T, int U, int W, bool kRest, bool kPast>
@@ -423,7 +432,7 @@ __global__ __launch_bounds__(W *kWave) void DistillLongGradKernel(const T *__res
   __shared__ float q[kMaxTeacher];
   const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x / kWave));
   const size_t row = row0 + rows - 1 - blockIdx.x;  // (the last row first, as above)
-  const int first = (int)blockIdx.y * (U * W * kWave);
+  const int first = (int)blockIdx.y * (U * W * kWave), all = VecsOf<T>(a.C);
   const T *x = logits + row * a.row_stride;
   T *dx = logits_grad + row * (size_t)a.C;
   const RowGrad<kRest> f(*reinterpret_cast<const float4 *>(a.records + 4 * row), a.scale.At(row), a.c);
@@ -434,10 +443,18 @@ __global__ __launch_bounds__(W *kWave) void DistillLongGradKernel(const T *__res
     token[j] = given >= 0 && given < a.C && !f.skipped ? (int)given : -1;
     q[j] = expf(a.top_logprobs[row * a.K + j] - f.lse);
   }
-  WriteUnlisted<kPast>(part, dx, a.C, first, wave, lane, f, a.c, true);
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int at = part.Vector(u, first, wave, lane);
+    if (at >= all) continue;
+    if (f.skipped) StoreZeros<kPast>(dx, at, a.C);
+    else WriteVec<kPast>(dx, part.v[u], at, a.C, [&](float xi) { return f.Unlisted(xi, a.c); });
+  }
   __syncthreads();
-  const long long end = (long long)(first + U * W * kWave) * kN;
-  WriteListed(x, dx, token, q, a.K, first * kN, (int)min((long long)a.C, end), (int)threadIdx.x, W * kWave, f, a.c);
+  const int i = threadIdx.x, begin = first * kN, end = (int)min((long long)a.C, (long long)(first + U * W * kWave) * kN);
+  const int mine = i < a.K ? token[i] : -1;
+  WriteListed(x, dx + begin, token, q, a.K, begin, end, i, W * kWave, mine >= begin && mine < end ? ToFloat(x[mine]) : 0.0f, f,
+              a.c);
 }
 
 // ---- sums, masks and launches -----------------------------------------------------------------------

@@ -588,51 +588,30 @@ __device__ __forceinline__ SoftmaxGrad RowGradOf(const BackwardArgs &a, size_t r
   return f;
 }
 
-// The softmax part of the elements that a group of lanes holds; zeros for rows that do not count.
-template <bool kPast, typename T, int U, int W, int L>
-__device__ __forceinline__ void WriteSoftmaxPart(const RowPart<T, U, W, L> &part, T *dx, int C, int first, int wave, int lane,
-                                                 const SoftmaxGrad &f, bool there, bool live) {
-  constexpr int kN = Lanes<T>::kN;
-  const int whole = C / kN, all = there ? VecsOf<T>(C) : 0;
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int q = part.Vector(u, first, wave, lane);
-    if (q >= all) continue;
-    float g[kN];
-#pragma unroll
-    for (int e = 0; e < kN; ++e) g[e] = live ? f.At(ElementOf<T>(part.v[u], e)) : 0.0f;
-    if (q < whole) {
-      StoreVec<kPast>(dx + (size_t)q * kN, PackOf<T>(g));
-    } else {  // the incomplete last vector, element by element
-      const int base = VecBase<T>(q, C);
-#pragma unroll
-      for (int e = 0; e < kN; ++e)
-        if (base + e >= q * kN && base + e < C) FromFloat(g[e], &dx[base + e]);
-    }
-  }
-}
-
-// The entries' own elements of columns [begin, end), over what is there.
+// The entries' columns of [begin, end) over what is at `to` (column `begin` first), entry by entry of the n work-items.
 template <typename T>
-__device__ __forceinline__ void WriteEntries(const T *x, T *dx, const int *entry, const float *entry_grad, int entries, int begin,
-                                             int end, int i, int n, const SoftmaxGrad &f, float inv_tau) {
+__device__ __forceinline__ void WriteEntries(const T *x, T *to, const int *entry, const float *entry_grad, int entries,
+                                             int begin, int end, int i, int n, const SoftmaxGrad &f, float inv_tau) {
   for (; i < entries; i += n) {
     const int token = entry[i];
     if (token < begin || token >= end) continue;
+    const float xi = ToFloat(x[token]);
     float own = 0.0f;  // a token that is listed twice takes both gradients
     for (int j = 0; j < entries; ++j)
       if (entry[j] == token) own += entry_grad[j];
-    FromFloat(f.At(ToFloat(x[token])) + own * inv_tau, &dx[token]);
+    FromFloat(f.At(xi) + own * inv_tau, &to[token - begin]);
   }
 }
 
-__device__ __forceinline__ int EntriesOf(const BackwardArgs &a) {
+__host__ __device__ __forceinline__ int EntriesOf(const BackwardArgs &a) {
   return (a.logprobs_grad != nullptr ? a.n : 0) + (a.top_grad != nullptr ? a.k : 0);
 }
 
 template <typename T, int U>
 __global__ __launch_bounds__(kThreads) void TokenShortGradKernel(const T *__restrict__ logits, T *__restrict__ logits_grad,
                                                                  long long row0, long long rows, BackwardArgs a) {
+  constexpr int kStage = StagedVecs<U>();
+  __shared__ Vec stages[kStage > 0 ? kShortRows * kStage : 1];
   HIP_DYNAMIC_SHARED(float, entries_lds)
   const int lane = threadIdx.x % kShort, in_block = threadIdx.x / kShort, entries = EntriesOf(a);
   // the last row first: of a batch larger than the 256 MB memory-side cache it is the tail that the forward pass left there
@@ -645,14 +624,28 @@ __global__ __launch_bounds__(kThreads) void TokenShortGradKernel(const T *__rest
   T *dx = logits_grad + row * (size_t)a.C;
   float *entry_grad = entries_lds + (size_t)in_block * 2 * entries;
   int *entry = reinterpret_cast<int *>(entry_grad + entries);
-  const float sum = GroupSum<kShort>(ReadEntries(a, row, lane, kShort, live ? entries : 0, entry, entry_grad, true));
+  const float part_sum = ReadEntries(a, row, lane, kShort, live ? entries : 0, entry, entry_grad, true);
   RowPart<T, U, 1, kShort> part;
   part.Load(x, live ? a.C : 0, 0, 0, lane);
-  const SoftmaxGrad f = RowGradOf(a, row, sum);
-  WriteSoftmaxPart<false>(part, dx, a.C, 0, 0, lane, f, there, live);
-  // (the stores above, and the list, are before what follows for every lane of the wavefront)
+  const SoftmaxGrad f = RowGradOf(a, row, GroupSum<kShort>(part_sum));
+  const int all = live ? VecsOf<T>(a.C) : 0;
+  T *to = kStage > 0 ? reinterpret_cast<T *>(stages + in_block * kStage) : dx;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int at = part.Vector(u, 0, 0, lane);
+    if (at < all) WriteVec<false>(to, part.v[u], at, a.C, [&](float xi) { return f.At(xi); });
+    else if (there && at < VecsOf<T>(a.C)) StoreZeros<false>(dx, at, a.C);
+  }
+  // (what is written above, and the list, are before what follows for every lane of the wavefront)
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  WriteEntries(x, dx, entry, entry_grad, live ? entries : 0, 0, a.C, lane, kShort, f, a.inv_tau);
+  WriteEntries(x, to, entry, entry_grad, live ? entries : 0, 0, a.C, lane, kShort, f, a.inv_tau);
+  if (kStage == 0) return;
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int at = part.Vector(u, 0, 0, lane);
+    if (at < all) StoreStaged(to, dx, at, a.C);
+  }
 }
 
 // Longer rows: W wavefronts take U vectors a lane of the stretch of a row that blockIdx.y counts.
@@ -665,24 +658,31 @@ __global__ __launch_bounds__(W *kWave) void TokenLongGradKernel(const T *__restr
   const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x / kWave));
   const int entries = EntriesOf(a);
   const size_t row = row0 + rows - 1 - blockIdx.x;  // (the last row first, as above)
-  const int first = (int)blockIdx.y * (U * W * kWave);
-  const bool live = a.mask == nullptr || a.mask[row] != 0;
+  const int first = (int)blockIdx.y * (U * W * kWave), all = VecsOf<T>(a.C);
   const T *x = logits + row * a.row_stride;
   T *dx = logits_grad + row * (size_t)a.C;
-  RowPart<T, U, W> part;
-  SoftmaxGrad f{0.0f, 0.0f, 0.0f, 0.0f};
-  if (live) {
-    // (every wavefront needs the sum; the first leaves the list)
-    const float sum = WaveSumF(ReadEntries(a, row, lane, kWave, entries, entry, entry_grad, wave == 0));
-    part.template Load<kPast>(x, a.C, first, wave, lane);
-    f = RowGradOf(a, row, sum);
+  if (a.mask != nullptr && a.mask[row] == 0) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int at = RowPart<T, U, W>::Vector(u, first, wave, lane);
+      if (at < all) StoreZeros<kPast>(dx, at, a.C);
+    }
+    return;
   }
-  WriteSoftmaxPart<kPast>(part, dx, a.C, first, wave, lane, f, true, live);
-  if (!live || entries == 0) return;
+  // (every wavefront needs the sum; the first leaves the list)
+  const float sum = WaveSumF(ReadEntries(a, row, lane, kWave, entries, entry, entry_grad, wave == 0));
+  RowPart<T, U, W> part;
+  part.template Load<kPast>(x, a.C, first, wave, lane);
+  const SoftmaxGrad f = RowGradOf(a, row, sum);
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int at = part.Vector(u, first, wave, lane);
+    if (at < all) WriteVec<kPast>(dx, part.v[u], at, a.C, [&](float xi) { return f.At(xi); });
+  }
+  if (entries == 0) return;
   __syncthreads();
-  const long long end = (long long)(first + U * W * kWave) * kN;
-  WriteEntries(x, dx, entry, entry_grad, entries, first * kN, (int)min((long long)a.C, end), (int)threadIdx.x, W * kWave, f,
-               a.inv_tau);
+  const int begin = first * kN, end = (int)min((long long)a.C, (long long)(first + U * W * kWave) * kN);
+  WriteEntries(x, dx + begin, entry, entry_grad, entries, begin, end, (int)threadIdx.x, W * kWave, f, a.inv_tau);
 }
 
 // ---- launches ---------------------------------------------------------------------------------------
@@ -748,12 +748,12 @@ template <typename T>
 int Backward(const void *logits_v, void *grad_v, long long rows, const BackwardArgs &a, hipStream_t stream) {
   const T *logits = static_cast<const T *>(logits_v);
   T *grad = static_cast<T *>(grad_v);
-  const int vecs = VecsOf<T>(a.C), entries = (a.logprobs_grad != nullptr ? a.n : 0) + (a.top_grad != nullptr ? a.k : 0);
+  const int vecs = VecsOf<T>(a.C);
   for (long long done = 0; done < rows; done += kRowsPerLaunch) {
     const long long n = rows - done < kRowsPerLaunch ? rows - done : kRowsPerLaunch, row0 = rows - done - n;
     const dim3 short_grid((unsigned)((n + kShortRows - 1) / kShortRows)), block(kThreads);
     const dim3 grid((unsigned)n, (unsigned)((vecs + 16 * kWave - 1) / (16 * kWave)));
-    const size_t lds = (size_t)kShortRows * 2 * entries * sizeof(float);
+    const size_t lds = (size_t)kShortRows * 2 * EntriesOf(a) * sizeof(float);
     if (vecs <= 2 * kShort) hipLaunchKernelGGL((TokenShortGradKernel<T, 2>), short_grid, block, lds, stream, logits, grad, row0, n, a);
     else if (vecs <= 4 * kShort) hipLaunchKernelGGL((TokenShortGradKernel<T, 4>), short_grid, block, lds, stream, logits, grad, row0, n, a);
     else if (vecs <= 8 * kShort) hipLaunchKernelGGL((TokenShortGradKernel<T, 8>), short_grid, block, lds, stream, logits, grad, row0, n, a);
