@@ -9,6 +9,7 @@
 //   * the GIL is released around the launches;
 //   * CPU tensors are rejected: this library has no CPU path.
 #include <torch/extension.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 
 // PyTorch-ROCm names its HIP devices "cuda"; these are the guard and stream types that go with it
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
@@ -862,7 +863,9 @@ class BoundaryRead {
 namespace {
 
 // ---------------------------------------------------------------------------------------------
-// Rows of output logits (k2_amd/token_loss.py); no counterpart in the reference.
+// Rows of output logits (k2_amd/token_loss.py); no counterpart in the reference.  These functions run without the GIL (the
+// module's definitions release it around them), for they are called by the autograd nodes at their end too, whose backward
+// passes run on torch's own threads: a node in Python would have to wait there for the interpreter.
 
 typedef torch::optional<torch::Tensor> OptionalTensor;
 
@@ -958,14 +961,11 @@ std::tuple<OptionalTensor, OptionalTensor, OptionalTensor, OptionalTensor, Optio
   torch::Tensor scratch;
   if (bytes > 0) scratch = torch::empty({static_cast<int64_t>(bytes)}, r.x.options().dtype(torch::kUInt8));
   void *stream = StreamOf(logits);
-  {
-    pybind11::gil_scoped_release release;
-    Check(k2amd_token_logprobs_forward(r.x.data_ptr(), r.stride, I64(tokens), MaskPtr(mask), FloatPtr(logprobs),
+  Check(k2amd_token_logprobs_forward(r.x.data_ptr(), r.stride, I64(tokens), MaskPtr(mask), FloatPtr(logprobs),
                                        FloatPtr(entropy), FloatPtr(top_logprobs),
                                        Given(top_tokens) ? top_tokens->data_ptr<int64_t>() : nullptr, FloatPtr(stats), r.rows,
                                        Int(r.C), Int(n), Int(num_top), static_cast<float>(temperature), r.dtype,
                                        bytes > 0 ? scratch.data_ptr() : nullptr, bytes, stream));
-  }
   return std::make_tuple(logprobs, entropy, top_logprobs, top_tokens, stats);
 }
 
@@ -988,13 +988,10 @@ torch::Tensor TokenLogprobsBackward(torch::Tensor logits, OptionalTensor tokens,
   c10::hip::HIPGuardMasqueradingAsCUDA guard(dev);
   torch::Tensor grad = torch::empty(logits.sizes(), r.x.options());
   void *stream = StreamOf(logits);
-  {
-    pybind11::gil_scoped_release release;
-    Check(k2amd_token_logprobs_backward(r.x.data_ptr(), r.stride, I64(tokens), MaskPtr(mask), stats.data_ptr<float>(),
+  Check(k2amd_token_logprobs_backward(r.x.data_ptr(), r.stride, I64(tokens), MaskPtr(mask), stats.data_ptr<float>(),
                                         FloatPtr(entropy), I64(top_tokens), FloatPtr(logprobs_grad), FloatPtr(entropy_grad),
                                         FloatPtr(top_grad), grad.data_ptr(), r.rows, Int(r.C), Int(n), Int(k),
                                         static_cast<float>(temperature), r.dtype, stream));
-  }
   return grad;
 }
 
@@ -1020,13 +1017,10 @@ std::tuple<torch::Tensor, OptionalTensor> DistillationForward(torch::Tensor logi
   torch::Tensor scratch;
   if (bytes > 0) scratch = torch::empty({static_cast<int64_t>(bytes)}, r.x.options().dtype(torch::kUInt8));
   void *stream = StreamOf(logits);
-  {
-    pybind11::gil_scoped_release release;
-    Check(k2amd_distillation_forward(r.x.data_ptr(), r.stride, top_logprobs.data_ptr<float>(), I64(top_tokens), MaskPtr(mask),
+  Check(k2amd_distillation_forward(r.x.data_ptr(), r.stride, top_logprobs.data_ptr<float>(), I64(top_tokens), MaskPtr(mask),
                                      losses.data_ptr<float>(), FloatPtr(records), r.rows, Int(r.C), Int(K), bucket ? 1 : 0,
                                      static_cast<float>(temperature), r.dtype, bytes > 0 ? scratch.data_ptr() : nullptr, bytes,
                                      stream));
-  }
   return std::make_tuple(losses, records);
 }
 
@@ -1046,12 +1040,9 @@ std::tuple<torch::Tensor, OptionalTensor> DistillationSum(torch::Tensor losses, 
   torch::Tensor scratch;
   if (bytes > 0) scratch = torch::empty({static_cast<int64_t>(bytes)}, losses.options().dtype(torch::kUInt8));
   void *stream = StreamOf(losses);
-  {
-    pybind11::gil_scoped_release release;
-    Check(k2amd_distillation_sum(losses.data_ptr<float>(), MaskPtr(mask), out.data_ptr<float>(), FloatPtr(inverse_count), sums,
+  Check(k2amd_distillation_sum(losses.data_ptr<float>(), MaskPtr(mask), out.data_ptr<float>(), FloatPtr(inverse_count), sums,
                                  per_sum, mean ? 1 : 0, static_cast<float>(factor), bytes > 0 ? scratch.data_ptr() : nullptr,
                                  bytes, stream));
-  }
   return std::make_tuple(out, inverse_count);
 }
 
@@ -1070,15 +1061,124 @@ torch::Tensor DistillationBackward(torch::Tensor logits, torch::Tensor top_logpr
   c10::hip::HIPGuardMasqueradingAsCUDA guard(dev);
   torch::Tensor grad = torch::empty(logits.sizes(), r.x.options());
   void *stream = StreamOf(logits);
-  {
-    pybind11::gil_scoped_release release;
-    Check(k2amd_distillation_backward(r.x.data_ptr(), r.stride, top_logprobs.data_ptr<float>(), I64(top_tokens),
+  Check(k2amd_distillation_backward(r.x.data_ptr(), r.stride, top_logprobs.data_ptr<float>(), I64(top_tokens),
                                       records.data_ptr<float>(), loss_grad.data_ptr<float>(),
                                       std::max<int64_t>(r.rows / std::max<int64_t>(losses, 1), 1), FloatPtr(inverse_count),
                                       static_cast<float>(factor), grad.data_ptr(), r.rows, Int(r.C), Int(K), bucket ? 1 : 0,
                                       static_cast<float>(temperature), r.dtype, stream));
-  }
   return grad;
+}
+
+// What a backward pass returns where it is itself recorded (create_graph): it cannot be differentiated again, and says so
+// when that is tried.
+torch::Tensor OnceDifferentiable(torch::Tensor grad) {
+  if (!at::GradMode::is_enabled()) return grad;
+  grad = grad.detach();
+  grad.set_requires_grad(true);
+  auto refuse = std::make_shared<torch::autograd::DelayedError>(
+      "k2_amd: trying to differentiate twice a function that is differentiable once", 1);
+  return (*refuse)({grad})[0];
+}
+torch::Tensor Dense(const torch::Tensor &t) { return t.defined() ? t.contiguous() : t; }
+OptionalTensor Maybe(const torch::Tensor &t) { return t.defined() ? OptionalTensor(t) : OptionalTensor(); }
+torch::Tensor Undefined(const OptionalTensor &t) { return Given(t) ? *t : torch::Tensor(); }
+
+struct TokenLogprobsNode : public torch::autograd::Function<TokenLogprobsNode> {
+  // outputs: those of logprobs, entropy, top_logprobs and top_tokens that were asked for
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext *ctx, const torch::Tensor &logits,
+                                                const OptionalTensor &tokens, const OptionalTensor &mask, double temperature,
+                                                int64_t num_top, bool return_entropy) {
+    auto out = TokenLogprobsForward(logits, tokens, mask, temperature, num_top, return_entropy, true);
+    const torch::Tensor entropy = Undefined(std::get<1>(out)), top_tokens = Undefined(std::get<3>(out));
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({logits, Undefined(tokens), Undefined(mask), Undefined(std::get<4>(out)), entropy, top_tokens});
+    ctx->saved_data["temperature"] = temperature;
+    torch::autograd::variable_list results;
+    for (const auto &t : {std::get<0>(out), std::get<1>(out), std::get<2>(out), std::get<3>(out)})
+      if (Given(t)) results.push_back(*t);
+    if (top_tokens.defined()) ctx->mark_non_differentiable({top_tokens});
+    return results;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const torch::Tensor &tokens = saved[1], &entropy = saved[4], &top_tokens = saved[5];
+    size_t next = 0;
+    torch::Tensor logprobs_grad, entropy_grad, top_grad;
+    if (tokens.defined()) logprobs_grad = Dense(grads[next++]);
+    // (the entropy is saved where it was asked for, and only there is it an output)
+    if (entropy.defined()) entropy_grad = Dense(grads[next++]);
+    if (top_tokens.defined()) top_grad = Dense(grads[next++]);
+    torch::autograd::variable_list result(6);
+    if (logprobs_grad.defined() || entropy_grad.defined() || top_grad.defined())
+      result[0] = OnceDifferentiable(TokenLogprobsBackward(saved[0], Maybe(tokens), Maybe(saved[2]), saved[3], Maybe(entropy),
+                                                           Maybe(top_tokens), Maybe(logprobs_grad), Maybe(entropy_grad),
+                                                           Maybe(top_grad), ctx->saved_data["temperature"].toDouble()));
+    return result;
+  }
+};
+
+// get_token_logprobs: (logprobs, entropy, top_logprobs, top_tokens)
+std::tuple<OptionalTensor, OptionalTensor, OptionalTensor, OptionalTensor> TokenLogprobs(
+    const torch::Tensor &logits, const OptionalTensor &tokens, const OptionalTensor &mask, double temperature, int64_t num_top,
+    bool return_entropy) {
+  if (!at::GradMode::is_enabled() || !logits.requires_grad()) {
+    auto out = TokenLogprobsForward(logits, tokens, mask, temperature, num_top, return_entropy, false);
+    return std::make_tuple(std::get<0>(out), std::get<1>(out), std::get<2>(out), std::get<3>(out));
+  }
+  const auto results = TokenLogprobsNode::apply(logits, tokens, mask, temperature, num_top, return_entropy);
+  size_t next = 0;
+  OptionalTensor out[4];
+  if (Given(tokens)) out[0] = results[next++];
+  if (return_entropy) out[1] = results[next++];
+  if (num_top > 0) {
+    out[2] = results[next++];
+    out[3] = results[next++];
+  }
+  return std::make_tuple(out[0], out[1], out[2], out[3]);
+}
+
+// What a distillation loss is reduced to: sums == 0 leaves the rows, n makes n sums of equally many rows each, as a scalar
+// where `scalar`; mean divides by the number of rows that count, factor multiplies the sums.
+torch::Tensor ReduceLosses(const torch::Tensor &rows, const OptionalTensor &mask, int64_t sums, bool mean, double factor,
+                           bool scalar, OptionalTensor *inverse_count) {
+  if (sums == 0) return rows;
+  auto reduced = DistillationSum(rows, mask, sums, mean, factor);
+  *inverse_count = std::get<1>(reduced);
+  return scalar ? std::get<0>(reduced).reshape({}) : std::get<0>(reduced);
+}
+
+struct DistillationNode : public torch::autograd::Function<DistillationNode> {
+  static torch::Tensor forward(torch::autograd::AutogradContext *ctx, const torch::Tensor &logits,
+                               const torch::Tensor &top_logprobs, const torch::Tensor &top_tokens, const OptionalTensor &mask,
+                               double temperature, bool bucket, int64_t sums, bool mean, double factor, bool scalar) {
+    auto out = DistillationForward(logits, top_logprobs, top_tokens, mask, temperature, bucket, true);
+    OptionalTensor inverse_count;
+    torch::Tensor loss = ReduceLosses(std::get<0>(out), mask, sums, mean, factor, scalar, &inverse_count);
+    ctx->save_for_backward({logits, top_logprobs, top_tokens, Undefined(std::get<1>(out)), Undefined(inverse_count)});
+    ctx->saved_data["temperature"] = temperature;
+    ctx->saved_data["bucket"] = bucket;
+    ctx->saved_data["factor"] = factor;
+    return loss;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    torch::autograd::variable_list result(10);
+    result[0] = OnceDifferentiable(DistillationBackward(saved[0], saved[1], saved[2], saved[3], Dense(grads[0]), Maybe(saved[4]),
+                                                        ctx->saved_data["factor"].toDouble(),
+                                                        ctx->saved_data["temperature"].toDouble(),
+                                                        ctx->saved_data["bucket"].toBool()));
+    return result;
+  }
+};
+
+torch::Tensor Distillation(const torch::Tensor &logits, const torch::Tensor &top_logprobs, const torch::Tensor &top_tokens,
+                           const OptionalTensor &mask, double temperature, bool bucket, int64_t sums, bool mean, double factor,
+                           bool scalar) {
+  if (at::GradMode::is_enabled() && logits.requires_grad())
+    return DistillationNode::apply(logits, top_logprobs, top_tokens, mask, temperature, bucket, sums, mean, factor, scalar);
+  auto out = DistillationForward(logits, top_logprobs, top_tokens, mask, temperature, bucket, false);
+  OptionalTensor inverse_count;
+  return ReduceLosses(std::get<0>(out), mask, sums, mean, factor, scalar, &inverse_count);
 }
 
 torch::Tensor PrunedMask(torch::Tensor ranges, torch::Tensor boundary) {
@@ -1090,12 +1190,9 @@ torch::Tensor PrunedMask(torch::Tensor ranges, torch::Tensor boundary) {
   c10::hip::HIPGuardMasqueradingAsCUDA guard(dev);
   torch::Tensor mask = torch::empty(ranges.sizes(), ranges.options().dtype(torch::kBool));
   void *stream = StreamOf(ranges);
-  {
-    pybind11::gil_scoped_release release;
-    Check(k2amd_rnnt_pruned_mask(ranges.data_ptr<int64_t>(), boundary.data_ptr<int64_t>(),
+  Check(k2amd_rnnt_pruned_mask(ranges.data_ptr<int64_t>(), boundary.data_ptr<int64_t>(),
                                  static_cast<uint8_t *>(mask.data_ptr()), Int(ranges.size(0)), Int(ranges.size(1)),
                                  Int(ranges.size(2)), stream));
-  }
   return mask;
 }
 
@@ -1143,10 +1240,13 @@ PYBIND11_MODULE(_k2_amd, m) {
   m.def("prune_gather_backward", &PruneGatherBackward);
   m.def("pruned_ranges_to_lattice", &PrunedRangesToLattice, pybind11::arg("ranges"),
         pybind11::arg("frames"), pybind11::arg("symbols"), pybind11::arg("logits"));
-  m.def("token_logprobs_forward", &TokenLogprobsForward);
-  m.def("token_logprobs_backward", &TokenLogprobsBackward);
-  m.def("distillation_forward", &DistillationForward);
-  m.def("distillation_sum", &DistillationSum);
-  m.def("distillation_backward", &DistillationBackward);
-  m.def("pruned_mask", &PrunedMask);
+  const auto without_gil = pybind11::call_guard<pybind11::gil_scoped_release>();
+  m.def("token_logprobs", &TokenLogprobs, without_gil);
+  m.def("distillation", &Distillation, without_gil);
+  m.def("token_logprobs_forward", &TokenLogprobsForward, without_gil);
+  m.def("token_logprobs_backward", &TokenLogprobsBackward, without_gil);
+  m.def("distillation_forward", &DistillationForward, without_gil);
+  m.def("distillation_sum", &DistillationSum, without_gil);
+  m.def("distillation_backward", &DistillationBackward, without_gil);
+  m.def("pruned_mask", &PrunedMask, without_gil);
 }

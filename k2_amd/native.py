@@ -314,6 +314,22 @@ def pruned_ranges_to_lattice(ranges, frames, symbols, logits):
 MAX_TOKENS, MAX_TOP, MAX_TEACHER = capi.MAX_TOKENS, capi.MAX_TOP, capi.MAX_TEACHER
 
 
+def token_logprobs(logits, tokens, mask, temperature, num_top, return_entropy):
+    """The extension's own autograd node (its backward pass runs without the interpreter), or None without the extension."""
+    _require_device(logits)
+    if _ext is None:
+        return None
+    return _ext.token_logprobs(logits, tokens, mask, temperature, num_top, return_entropy)
+
+
+def distillation(logits, top_logprobs, top_tokens, mask, temperature, bucket, sums, mean, factor, scalar):
+    """Likewise."""
+    _require_device(logits)
+    if _ext is None:
+        return None
+    return _ext.distillation(logits, top_logprobs, top_tokens, mask, temperature, bucket, sums, mean, factor, scalar)
+
+
 def token_logprobs_forward(logits, tokens, mask, temperature, num_top, return_entropy, keep):
     _require_device(logits)
     if _ext is not None:

@@ -28,6 +28,8 @@ class TokenLogprobs(NamedTuple):
 
 
 class _TokenLogprobs(torch.autograd.Function):
+    """The node of the ctypes host; the extension has its own (csrc/pybind.cpp)."""
+
     @staticmethod
     def forward(ctx, logits, tokens, mask, temperature, num_top, return_entropy):
         logprobs, entropy, top_logprobs, top_tokens, stats = native.token_logprobs_forward(
@@ -51,8 +53,8 @@ class _TokenLogprobs(torch.autograd.Function):
 
 
 class _Distillation(torch.autograd.Function):
-    """The loss of each row, or sums of them: ``sums`` 0 leaves the rows, n makes n sums of equally many rows each.
-    ``mean``: divided by the number of rows that count.  ``factor`` multiplies the sums."""
+    """The node of the ctypes host, as above.  The loss of each row, or sums of them: ``sums`` 0 leaves the rows, n makes n
+    sums of equally many rows each.  ``mean``: divided by the number of rows that count.  ``factor`` multiplies the sums."""
 
     @staticmethod
     def forward(ctx, logits, top_logprobs, top_tokens, mask, temperature, bucket, sums, mean, factor):
@@ -124,9 +126,21 @@ def get_token_logprobs(
     num_top = int(num_top)
     assert 0 <= num_top <= native.MAX_TOP, num_top
     args = (logits, tokens, mask, float(temperature), num_top, bool(return_entropy))
-    if torch.is_grad_enabled() and logits.requires_grad:
-        return TokenLogprobs(*_TokenLogprobs.apply(*args))
-    return TokenLogprobs(*native.token_logprobs_forward(*args, False)[:4])
+    results = native.token_logprobs(*args)
+    if results is None:
+        if torch.is_grad_enabled() and logits.requires_grad:
+            results = _TokenLogprobs.apply(*args)
+        else:
+            results = native.token_logprobs_forward(*args, False)[:4]
+    return TokenLogprobs(*results)
+
+
+def _distill(args, sums, mean, factor, scalar):
+    loss = native.distillation(*args, sums, mean, factor, scalar)
+    if loss is None:
+        loss = _Distillation.apply(*args, sums, mean, factor)
+        loss = loss.reshape(()) if scalar else loss
+    return loss
 
 
 def _distillation_args(logits, top_logprobs, top_tokens, mask, temperature, rest, reduction):
@@ -140,8 +154,8 @@ def _distillation_args(logits, top_logprobs, top_tokens, mask, temperature, rest
         raise ValueError(f"rest should be ('renormalise' | 'bucket'), given {rest}")
     if reduction not in ("none", "mean", "sum"):
         raise ValueError(f"reduction should be ('none' | 'mean' | 'sum'), given {reduction}")
-    return (logits, top_logprobs.to(device=logits.device, dtype=torch.float32).contiguous(), _dev_i64(top_tokens, logits),
-            mask, float(temperature), rest == "bucket")
+    return (logits, top_logprobs.to(device=logits.device, dtype=torch.float32).contiguous(), _dev_i64(top_tokens, logits), mask,
+            float(temperature), rest == "bucket")
 
 
 def distillation_loss(
@@ -170,8 +184,9 @@ def distillation_loss(
     Gradients scale with 1 / temperature; multiply the loss by temperature ** 2 to keep them comparable across
     temperatures."""
     args = _distillation_args(logits, top_logprobs, top_tokens, mask, temperature, rest, reduction)
-    loss = _Distillation.apply(*args, 0 if reduction == "none" else 1, reduction == "mean", 1.0)
-    return loss if reduction == "none" else loss.reshape(())
+    if reduction == "none":
+        return _distill(args, 0, False, 1.0, False)
+    return _distill(args, 1, reduction == "mean", 1.0, True)
 
 
 def get_pruned_mask(ranges: Tensor, boundary: Tensor) -> Tensor:
@@ -203,5 +218,5 @@ def rnnt_distillation_loss_pruned(
     mask = None if boundary is None else get_pruned_mask(ranges, boundary)
     args = _distillation_args(logits, top_logprobs, top_tokens, mask, temperature, rest, reduction)
     if reduction == "none":
-        return _Distillation.apply(*args, B, False, 1.0)
-    return _Distillation.apply(*args, 1, False, 1.0 if reduction == "sum" else 1.0 / max(B, 1)).reshape(())
+        return _distill(args, B, False, 1.0, False)
+    return _distill(args, 1, False, 1.0 if reduction == "sum" else 1.0 / max(B, 1), True)
