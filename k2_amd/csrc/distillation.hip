@@ -96,11 +96,17 @@ __device__ __forceinline__ bool MarkListed(const List &list, int lane, unsigned 
 
 template <typename T, int U, int W, int L>
 __device__ __forceinline__ void DropListed(RowPart<T, U, W, L> &part, int C, int lane, const unsigned *bits) {
+  constexpr int kN = Lanes<T>::kN;
+  const unsigned *own = bits + lane * kN / 32;  // a round of L vectors is whole words of marks
+  const int shift = lane * kN % 32;
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const int q = part.VectorAnew(u, 0, 0, lane);
-    const unsigned marked = q < VecsOf<T>(C) ? MarksOf<T>(bits, VecBase<T>(q, C), 0) : 0u;
-    if (__ballot(marked != 0) != 0) DropMarked<T>(&part.v[u], marked);
+    unsigned marked = own[u * (L * kN / 32)] >> shift & ((1u << kN) - 1);
+    if ((u + 1) * L * kN > C) {  // the round with the row's last vector: read to end with the row
+      const int q = part.VectorAnew(u, 0, 0, lane);
+      marked = q < VecsOf<T>(C) ? MarksOf<T>(bits, VecBase<T>(q, C), 0) : 0u;
+    }
+    DropMarked<T>(&part.v[u], marked);
   }
 }
 
@@ -150,13 +156,13 @@ __device__ __forceinline__ void FinishRow(List list, ListState state, unsigned r
     at = GroupMax<L>(at);
   } else {
     float sum = 0.0f;
-    for (int j = lane; j < list.K; j += L) sum += expf(list.a[j] - a_max);
-    lse = a_max + logf(GroupSum<L>(sum));
+    for (int j = lane; j < list.K; j += L) sum += Exp(list.a[j] - a_max);
+    lse = a_max + kLn2 * Log2(GroupSum<L>(sum));
   }
   float others = 0.0f, loss = 0.0f;
   for (int j = lane; j < list.K; j += L) {
     const float a = list.a[j];
-    const float q = a > Real<float>::NegInf() ? expf(a - lse) : 0.0f;
+    const float q = a > Real<float>::NegInf() ? Exp(a - lse) : 0.0f;
     if (-(float)j != at) others += q;
     if (q > 0.0f) loss += q * ((a - lse) - LogProb(list.x[j], m, ls, inv_tau));
   }
@@ -166,11 +172,11 @@ __device__ __forceinline__ void FinishRow(List list, ListState state, unsigned r
     others = GroupSum<L>(others);
     // 1 - sum q, the largest by expm1: exact where the list holds nearly everything
     if (rest.s != 0.0f) q0 = fmaxf(0.0f, -expm1f(a_max) - others);
-    mass = others + expf(a_max) + q0;
+    mass = others + Exp(a_max) + q0;
     if (rest.s != 0.0f) {
       const float log_p0 = (rest.m - m) * inv_tau + kLn2 * (Log2(rest.s) - ls);
-      p0 = expf(log_p0);
-      if (q0 > 0.0f) loss += q0 * (logf(q0) - log_p0);
+      p0 = Exp(log_p0);
+      if (q0 > 0.0f) loss += q0 * (kLn2 * Log2(q0) - log_p0);
     }
   }
   if (lane != 0) return;
@@ -223,7 +229,8 @@ __global__ __launch_bounds__(kThreads) void DistillShortKernel(const T *__restri
   if (state != kUsable) list.K = 0;
   const T *x = logits + row * a.row_stride;
   RowPart<T, U, 1, kShort> part;
-  part.Load(x, state == kUsable ? a.C : 0, 0, 0, lane);
+  // (all four rows or none: a load that some lanes skip is a branch for each vector)
+  part.Load(x, __ballot(state == kUsable) != 0 ? a.C : 0, 0, 0, lane);
   const float x_first = ListedLogit(x, list, lane);
   unsigned repeated = 0;
   if (kRest) {
@@ -390,19 +397,19 @@ __global__ __launch_bounds__(kThreads) void DistillShortGradKernel(const T *__re
   const RowGrad<kRest> f(record, scale, a.c);
   const bool live = there && !f.skipped;
   RowPart<T, U, 1, kShort> part;
-  part.Load(x, live ? a.C : 0, 0, 0, lane);
+  part.Load(x, __ballot(live) != 0 ? a.C : 0, 0, 0, lane);
   const bool usable = live && given >= 0 && given < a.C;
   const float x_first = usable ? ToFloat(x[given]) : 0.0f;
   int *token = reinterpret_cast<int *>(lists) + (size_t)group * 2 * a.K;
   float *q = lists + (size_t)group * 2 * a.K + a.K;
   if (lane < a.K) {
     token[lane] = usable ? (int)given : -1;
-    q[lane] = expf(teacher - f.lse);
+    q[lane] = Exp(teacher - f.lse);
   }
   for (int j = lane + kShort; j < a.K; j += kShort) {
     given = a.top_tokens[row * a.K + j];
     token[j] = live && given >= 0 && given < a.C ? (int)given : -1;
-    q[j] = expf(a.top_logprobs[row * a.K + j] - f.lse);
+    q[j] = Exp(a.top_logprobs[row * a.K + j] - f.lse);
   }
   const int all = live ? VecsOf<T>(a.C) : 0;
   T *to = kStage > 0 ? reinterpret_cast<T *>(stages + group * kStage) : dx;
@@ -441,7 +448,7 @@ __global__ __launch_bounds__(W *kWave) void DistillLongGradKernel(const T *__res
   for (int j = threadIdx.x; j < a.K; j += W * kWave) {
     const int64_t given = a.top_tokens[row * a.K + j];
     token[j] = given >= 0 && given < a.C && !f.skipped ? (int)given : -1;
-    q[j] = expf(a.top_logprobs[row * a.K + j] - f.lse);
+    q[j] = Exp(a.top_logprobs[row * a.K + j] - f.lse);
   }
 #pragma unroll
   for (int u = 0; u < U; ++u) {
@@ -459,10 +466,11 @@ __global__ __launch_bounds__(W *kWave) void DistillLongGradKernel(const T *__res
 
 // ---- sums, masks and launches -----------------------------------------------------------------------
 
-// Sums of rows_per_sum values each, and how many rows count, in a fixed order and in double: a workgroup of 1024 a chunk of
-// kChunk values, eight of them on their way at a time in each work-item; where a sum has several chunks, a wavefront joins
-// them.  (A sum of one chunk, as of most batches of sequences, is one launch.)
-constexpr int kChunk = 16384, kSumThreads = 1024;
+// Sums of rows_per_sum values each, and how many rows count, in a fixed order and in double, eight values on their way at a time
+// in each work-item.  Up to kOneChunk of them are one workgroup's (4.9 us at 8192); more are cut into chunks of kChunk, for a
+// workgroup each, which a wavefront joins in a second launch (80000 in chunks of 16384 took 14.4 us, five workgroups going
+// twice to memory).
+constexpr int kOneChunk = 16384, kChunk = 2048, kSumThreads = 1024, kChunkThreads = kChunk / 8;
 
 struct SumOutput {
   float *sums, *inverse_count;
@@ -479,15 +487,15 @@ __global__ __launch_bounds__(kSumThreads) void RowChunkSumKernel(const float *__
                                                                  const uint8_t *__restrict__ mask, int rows_per_sum,
                                                                  double *__restrict__ partial, SumOutput out) {
   __shared__ double lds[2 * kSumThreads / kWave];
-  const int first = (int)blockIdx.x * kChunk, last = min(rows_per_sum, first + kChunk);
+  const int first = (int)blockIdx.x * kChunk, last = gridDim.x == 1 ? rows_per_sum : min(rows_per_sum, first + kChunk);
   const size_t base = (size_t)blockIdx.y * rows_per_sum;
   double sum = 0, count = 0;
-  for (int i = first + (int)threadIdx.x; i < last; i += 8 * kSumThreads) {
+  for (int i = first + (int)threadIdx.x; i < last; i += 8 * (int)blockDim.x) {
     float v[8];
     uint8_t m[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const int at = i + j * kSumThreads;
+      const int at = i + j * (int)blockDim.x;
       v[j] = at < last ? values[base + at] : 0.0f;
       m[j] = at < last ? (mask != nullptr ? mask[base + at] : 1) : 0;
     }
@@ -509,7 +517,7 @@ __global__ __launch_bounds__(kSumThreads) void RowChunkSumKernel(const float *__
   }
   __syncthreads();
   if (threadIdx.x != 0) return;
-  for (int w = 1; w < kSumThreads / kWave; ++w) {
+  for (int w = 1; w < (int)blockDim.x / kWave; ++w) {
     sum += lds[2 * w];
     count += lds[2 * w + 1];
   }
@@ -600,7 +608,7 @@ int Backward(const void *logits, void *grad, long long rows, int rest, const Bac
   return rest ? BackwardOf<T, true>(x, dx, rows, a, stream) : BackwardOf<T, false>(x, dx, rows, a, stream);
 }
 
-long long SumChunks(long long rows_per_sum) { return (rows_per_sum + kChunk - 1) / kChunk; }
+long long SumChunks(long long rows_per_sum) { return rows_per_sum <= kOneChunk ? 1 : (rows_per_sum + kChunk - 1) / kChunk; }
 
 }  // namespace
 }  // namespace k2amd
@@ -668,13 +676,13 @@ int k2amd_distillation_sum(const float *row_losses, const uint8_t *mask, float *
   if (num_sums > 65535 || rows_per_sum >= (1ll << 31)) return K2AMD_ERR_UNSUPPORTED;
   if (num_sums == 0) return K2AMD_OK;
   if (sums == nullptr || (rows_per_sum > 0 && row_losses == nullptr)) return K2AMD_ERR_INVALID_ARGUMENT;
-  const int chunks = rows_per_sum > 0 ? (int)SumChunks(rows_per_sum) : 1;
+  const int chunks = (int)SumChunks(rows_per_sum);
   if (chunks > 1 && (scratch == nullptr || Misaligned(scratch) ||
                      scratch_bytes < k2amd_distillation_sum_scratch_bytes(num_sums, rows_per_sum)))
     return K2AMD_ERR_WORKSPACE;
   hipStream_t st = static_cast<hipStream_t>(stream);
   const SumOutput out{sums, inverse_count, mean, factor};
-  hipLaunchKernelGGL(RowChunkSumKernel, dim3((unsigned)chunks, (unsigned)num_sums), dim3(kSumThreads), 0, st, row_losses, mask,
+  hipLaunchKernelGGL(RowChunkSumKernel, dim3((unsigned)chunks, (unsigned)num_sums), dim3(chunks == 1 ? kSumThreads : kChunkThreads), 0, st, row_losses, mask,
                      (int)rows_per_sum, static_cast<double *>(scratch), out);
   if (chunks > 1)
     hipLaunchKernelGGL(RowSumKernel, dim3((unsigned)num_sums), dim3(kWave), 0, st, static_cast<const double *>(scratch), chunks,

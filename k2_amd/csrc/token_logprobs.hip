@@ -202,10 +202,13 @@ constexpr int kThreads = kShort * kShortRows;
 
 template <int U>
 __device__ __forceinline__ int RowGroupsReaching(const float (&group)[U], float v) {
-  float n = 0.0f;
+  int n = 0;
 #pragma unroll
-  for (int u = 0; u < U; ++u) n += group[u] >= v ? 1.0f : 0.0f;
-  return (int)GroupSum<kShort>(n);
+  for (int u = 0; u < U; ++u) n += group[u] >= v ? 1 : 0;
+  n += __builtin_amdgcn_update_dpp(0, n, 0xb1, 0xf, 0xf, false);  // (the moves of GroupSum)
+  n += __builtin_amdgcn_update_dpp(0, n, 0x4e, 0xf, 0xf, false);
+  n += __builtin_amdgcn_update_dpp(0, n, 0x141, 0xf, 0xf, false);
+  return n + __builtin_amdgcn_update_dpp(0, n, 0x140, 0xf, 0xf, false);
 }
 
 // as Threshold above, for each of the wavefront's rows
@@ -248,7 +251,8 @@ __global__ __launch_bounds__(kThreads) void TokenShortKernel(const T *__restrict
   const bool live = there && masked != 0;
   const T *x = logits + row * a.row_stride;
   RowPart<T, U, 1, kShort> part;
-  part.Load(x, live ? a.C : 0, 0, 0, lane);
+  // (all four rows or none: a load that some lanes skip is a branch for each vector)
+  part.Load(x, __ballot(live) != 0 ? a.C : 0, 0, 0, lane);
   float x_token = live && token >= 0 && token < a.C ? ToFloat(x[token]) : 0.0f;
   float group[U], high = Real<float>::NegInf();
 #pragma unroll
@@ -468,21 +472,15 @@ __global__ __launch_bounds__(kStreamWaves *kWave) void TokenStreamKernel(const T
   WriteRow(a, row, lane, sums, token, token >= 0 && token < a.C ? ToFloat(x[token]) : 0.0f);
 }
 
-// How many of the n keys at `keys`, the largest first, are larger than `key` (n <= 64).
-__device__ __forceinline__ int LargerKeys(const unsigned long long *keys, int n, unsigned long long key) {
-  int larger = 0;
-#pragma unroll
-  for (int step = 64; step > 0; step >>= 1)
-    if (larger + step <= n && keys[larger + step - 1] > key) larger += step;
-  return larger;
-}
-
 // Joins the parts of a row: a workgroup a row.  The keys of a part are in order, so a key's place among all is its place in
-// its own part and, in every other part, the number of larger ones, by bisection.
-constexpr int kJoinThreads = 256;
+// its own part and, in every other part, the number of larger ones, by bisection.  A work-item searches four parts side by
+// side for a key: steps of a search wait for one another, and it is their latency that counts where there is one row (one
+// after the other the 16 parts of 131072 columns took 14 us, counted one by one 41).
+constexpr int kJoinThreads = 512;
 template <typename T>
 __global__ __launch_bounds__(kJoinThreads) void TokenJoinKernel(const T *__restrict__ logits, long long row0, ForwardArgs a) {
   HIP_DYNAMIC_SHARED(unsigned long long, keys)
+  int *places = reinterpret_cast<int *>(keys + a.parts * a.k);
   const size_t row = row0 + blockIdx.x;
   if (a.mask != nullptr && a.mask[row] == 0) return;
   const int i = threadIdx.x, lane = i & (kWave - 1), all = a.parts * a.k;
@@ -497,37 +495,42 @@ __global__ __launch_bounds__(kJoinThreads) void TokenJoinKernel(const T *__restr
     const float4 v = a.part_sums[row * a.parts + lane];
     sums = Sums{v.x, v.y, v.z};
   }
-  for (int j = i; j < all; j += kJoinThreads) keys[j] = a.part_keys[row * all + j];
+  for (int j = i; j < all; j += kJoinThreads) {
+    keys[j] = a.part_keys[row * all + j];
+    places[j] = j % a.k;
+  }
   sums = JoinLanes(sums, a.c);
   if (i < kWave) WriteRow(a, row, i, sums, token, x_token);
   if (a.k == 0) return;
   __syncthreads();
   const float ls = Log2(sums.s);
+  int highest = 1;
+  while (2 * highest <= a.k) highest *= 2;
+  for (int task = i; task < all * ((a.parts + 3) / 4); task += kJoinThreads) {
+    const int j = task % all, first = 4 * (task / all), own = j / a.k;
+    const unsigned long long key = keys[j];
+    int larger[4] = {0, 0, 0, 0}, place = 0;
+    for (int step = highest; step > 0; step >>= 1)
+#pragma unroll
+      for (int p = 0; p < 4; ++p) {
+        const unsigned long long *part = keys + min(first + p, a.parts - 1) * a.k;
+        if (larger[p] + step <= a.k && part[larger[p] + step - 1] > key) larger[p] += step;
+      }
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+      if (first + p >= a.parts || first + p == own) continue;
+      // (0, past the last of its part: behind every key, in the order of the parts)
+      place += key == 0 && first + p < own ? a.k : larger[p];
+    }
+    atomicAdd(&places[j], place);
+  }
+  __syncthreads();
   for (int j = i; j < all; j += kJoinThreads) {
     const unsigned long long key = keys[j];
-    const int part = j / a.k;
-    int place = j - part * a.k;
-    if (key != 0) {
-#pragma unroll 4
-      for (int p = 0; p < a.parts; ++p) {
-        const int larger = LargerKeys(keys + p * a.k, a.k, key);
-        place += p != part ? larger : 0;
-      }
-      if (place < a.k) {
-        a.top_tokens[row * a.k + place] = IndexOf(key);
-        a.top_logprobs[row * a.k + place] = LogProb(LogitOf(key), sums.m, ls, a.inv_tau);
-      }
-      continue;
-    }
-    // past the last of its part: behind every key, in the order of the parts' ends
-    for (int p = 0; p < a.parts; ++p) {
-      if (p == part) continue;
-      place += p < part ? a.k : LargerKeys(keys + p * a.k, a.k, 0ull);
-    }
-    if (place < a.k) {
-      a.top_tokens[row * a.k + place] = -1;
-      a.top_logprobs[row * a.k + place] = Real<float>::NegInf();
-    }
+    const int place = places[j];
+    if (place >= a.k) continue;
+    a.top_tokens[row * a.k + place] = key != 0 ? (int64_t)IndexOf(key) : -1;
+    a.top_logprobs[row * a.k + place] = key != 0 ? LogProb(LogitOf(key), sums.m, ls, a.inv_tau) : Real<float>::NegInf();
   }
 }
 
@@ -626,7 +629,7 @@ __global__ __launch_bounds__(kThreads) void TokenShortGradKernel(const T *__rest
   int *entry = reinterpret_cast<int *>(entry_grad + entries);
   const float part_sum = ReadEntries(a, row, lane, kShort, live ? entries : 0, entry, entry_grad, true);
   RowPart<T, U, 1, kShort> part;
-  part.Load(x, live ? a.C : 0, 0, 0, lane);
+  part.Load(x, __ballot(live) != 0 ? a.C : 0, 0, 0, lane);
   const SoftmaxGrad f = RowGradOf(a, row, GroupSum<kShort>(part_sum));
   const int all = live ? VecsOf<T>(a.C) : 0;
   T *to = kStage > 0 ? reinterpret_cast<T *>(stages + in_block * kStage) : dx;
@@ -706,7 +709,7 @@ void LaunchHeld(const T *logits, long long rows, bool entropy, const ForwardArgs
     else hipLaunchKernelGGL((TokenHeldKernel<T, U, W, false>), grid, block, 0, stream, logits, row0, a);
     if (a.parts > 1)
       hipLaunchKernelGGL(TokenJoinKernel<T>, dim3((unsigned)n), dim3(kJoinThreads),
-                         (size_t)a.parts * a.k * sizeof(unsigned long long), stream, logits, row0, a);
+                         (size_t)a.parts * a.k * (sizeof(unsigned long long) + sizeof(int)), stream, logits, row0, a);
   }
 }
 

@@ -241,6 +241,7 @@ constexpr int StagedVecs() { return U <= 8 ? U * 16 : 0; }
 
 __device__ __forceinline__ float Exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float Log2(float x) { return __builtin_amdgcn_logf(x); }
+__device__ __forceinline__ float Exp(float x) { return Exp2(x * 1.44269504088896341f); }  // |x| 2^-23 off, relative
 
 // Reductions over a wavefront: within rows of 16 lanes by DPP moves, across the four rows through scalar registers.  Every
 // lane gets the result.
@@ -372,15 +373,11 @@ __device__ __forceinline__ Sums SumsOf(RowPart<T, U, W, L> &part, float high, fl
 // -inf in the place of a vector's elements that are marked
 template <typename T>
 __device__ __forceinline__ void DropMarked(Vec *v, unsigned marked) {
+  auto all_if = [&](int bit) { return (unsigned)((int)(marked << (31 - bit)) >> 31); };
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    unsigned &w = v->w[i];
-    if (sizeof(T) == 4) {
-      if (marked >> i & 1u) w = Lanes<T>::kNegInf;
-    } else {
-      if (marked >> (2 * i) & 1u) w = (w & 0xffff0000u) | (Lanes<T>::kNegInf & 0xffffu);
-      if (marked >> (2 * i + 1) & 1u) w = (w & 0xffffu) | (Lanes<T>::kNegInf & 0xffff0000u);
-    }
+    const unsigned gone = sizeof(T) == 4 ? all_if(i) : (all_if(2 * i) & 0xffffu) | (all_if(2 * i + 1) & 0xffff0000u);
+    v->w[i] = (gone & Lanes<T>::kNegInf) | (~gone & v->w[i]);
   }
 }
 // the marks of the elements of a vector that is read from column `base` on; bit 0 of `bits` is column `begin` (`base` is

@@ -211,11 +211,11 @@ def test_entry_points_refuse_before_launching():
     assert back(0) == 1 and back(1, None) == 1
     assert lib.k2amd_token_logprobs_backward(one, 8, None, None, one, None, None, one, None, None, one, 1, 8, 1, 0, 1.0, 0, None) == 1
     assert lib.k2amd_token_logprobs_backward(one, 8, one, None, one, None, None, None, one, None, one, 1, 8, 1, 0, 1.0, 0, None) == 1
-    assert lib.k2amd_distillation_sum(one, None, one, None, 1, 20000, 0, 1.0, ok, 31, None) == 3
-    assert lib.k2amd_distillation_sum(one, None, one, None, 1, 20000, 0, 1.0, one, 32, None) == 3
+    assert lib.k2amd_distillation_sum(one, None, one, None, 1, 20000, 0, 1.0, ok, 159, None) == 3
+    assert lib.k2amd_distillation_sum(one, None, one, None, 1, 20000, 0, 1.0, one, 160, None) == 3
     assert lib.k2amd_distillation_sum(one, None, one, None, 1, -1, 0, 1.0, one, 8, None) == 1
     assert lib.k2amd_distillation_sum(None, None, None, None, 0, 0, 0, 1.0, None, 0, None) == 0
-    assert lib.k2amd_distillation_sum_scratch_bytes(2, 10) == 0 and lib.k2amd_distillation_sum_scratch_bytes(2, 20000) == 64
+    assert lib.k2amd_distillation_sum_scratch_bytes(2, 10) == 0 and lib.k2amd_distillation_sum_scratch_bytes(2, 20000) == 2 * 160
     assert lib.k2amd_rnnt_pruned_mask(None, None, None, 0, 3, 3, None) == 0
     assert lib.k2amd_rnnt_pruned_mask(None, None, None, 1, 3, 3, None) == 1
     assert lib.k2amd_rnnt_pruned_mask(one, one, one, 1 << 20, 1 << 11, 1, None) == 2
