@@ -328,8 +328,9 @@ __device__ __forceinline__ Sums JoinLanes(const Sums &a, float c) {
 
 // m, s and t (kEntropy) of what a group of lanes holds, from its largest logit.  The inner loop is one fused multiply-add,
 // one exponential and one addition an element: d = x c - M with M = m c rounded, which leaves every exponent off by the same
-// M - m c, exactly known, and that is taken out of the sums at the end.  Logits beyond 1e30 (the lowest of a type) would
-// overflow there: rows with a largest logit of that size take the difference first.
+// M - m c, exactly known and below a half, and that is taken out of the sums at the end.  Rows whose m c is beyond kFar (a
+// type's lowest value everywhere, a temperature of nearly 0) take the difference first.
+constexpr float kFar = 1.0e6f;
 template <bool kEntropy, typename T, int U, int W, int L>
 __device__ __forceinline__ Sums SumsOf(RowPart<T, U, W, L> &part, float high, float c) {
   constexpr int kN = Lanes<T>::kN;
@@ -337,8 +338,7 @@ __device__ __forceinline__ Sums SumsOf(RowPart<T, U, W, L> &part, float high, fl
   float s[4] = {0, 0, 0, 0}, t[4] = {0, 0, 0, 0};
 #pragma unroll
   for (int u = 0; u < U; ++u) part.Packed(u);  // (here, and not in the two branches: each would get registers of its own)
-  const bool can_overflow = sizeof(T) == 4 || Lanes<T>::kNegInf != 0xfc00fc00u;  // (halves end at 65504)
-  const bool far = can_overflow && __ballot(fabsf(r.m) > 1e30f) != 0;
+  const bool far = __ballot(!(fabsf(r.m * c) <= kFar)) != 0;
   const float shift = far ? 0.0f : -(r.m * c);
   if (far) {
 #pragma unroll
@@ -437,7 +437,7 @@ __device__ __forceinline__ Sums StreamSums(const T *x, int C, int first, int end
     r.m = fmaxf(high[0], high[1]);
     const float before = reference;
     reference = r.m == Real<float>::NegInf() ? 0.0f : r.m * c;
-    far |= fabsf(r.m) > 1e30f && r.m != Real<float>::NegInf();
+    far |= !(fabsf(reference) <= kFar);
     const float down = fminf(before - reference, 0.0f), scale = Exp2(down);  // (the first reference may be below 0: s is 0 then)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -453,7 +453,7 @@ __device__ __forceinline__ Sums StreamSums(const T *x, int C, int first, int end
         if (kEntropy) t[e & 3] += fmaxf(d, kNothing) * p;
       }
   }
-  if (__ballot(far) != 0) {  // logits at the end of the type's range: differences first, no reference (as in SumsOf)
+  if (__ballot(far) != 0) {  // differences first, as in SumsOf
 #pragma unroll
     for (int i = 0; i < 4; ++i) s[i] = t[i] = 0.0f;
     r.m = WaveMaxF(r.m);

@@ -73,6 +73,53 @@ def test_ties_and_masked_vocabularies(device, dtype, C):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("C", [60, 700, 5000, 40001])
+def test_far_from_zero(device, dtype, C):
+    """Rows that lie anywhere in the type's range, and temperatures that take the logits far apart or close together: the
+    budgets are those of differences of logits, wherever the logits are."""
+    import k2_amd as k2
+    x = orc.logits_case(C, 8, C, torch.float32, device)
+    offsets = [0.0, 300.0, -3000.0, 4.0e4, -6.0e4] + ([2.0e6, -1.0e9, 3.0e20] if dtype != torch.float16 else [100.0, -100.0, 1.0e3])
+    x = (x + torch.tensor(offsets, device=device).unsqueeze(1)).to(dtype).requires_grad_()
+    tokens = torch.randint(0, C, (8, 1), device=device)
+    for temperature in (1.0, 0.01, 1.0e-9, 1.0e6):
+        got = k2.get_token_logprobs(x, tokens, temperature=temperature, num_top=4, return_entropy=True)
+        orc.check_token_logprobs(x.detach(), tokens, None, temperature, 4, k2.TokenLogprobs(*(u.detach() for u in got)))
+        up = torch.ones_like(got.logprobs)
+        (grad,) = torch.autograd.grad(got.logprobs, x, up)
+        if temperature >= 0.01:  # (beyond, the gradient itself leaves float16)
+            orc.check_token_grad(x.detach(), tokens, None, temperature, (up, None, None), None, grad)
+        without = k2.get_token_logprobs(x.detach(), tokens, temperature=temperature, return_entropy=True)
+        orc.check_token_logprobs(x.detach(), tokens, None, temperature, 0, without)
+    a, t = orc.teacher_case(1, x.detach(), 5, 1.0)
+    for bucket in (False, True):
+        loss = k2.distillation_loss(x, a, t, rest="bucket" if bucket else "renormalise", reduction="none")
+        (grad,) = torch.autograd.grad(loss, x, torch.ones_like(loss))
+        orc.check_distillation(x.detach(), a, t, None, 1.0, bucket, loss.detach(), torch.ones_like(loss), grad)
+
+
+def test_more_rows_than_a_launch_takes(device):
+    """Calls beyond 2^20 rows are several launches; the gradient's go from the last rows to the first."""
+    import k2_amd as k2
+    rows, C = (1 << 20) + 1037, 9
+    x = orc.logits_case(4, rows, C, torch.float16, device).requires_grad_()
+    tokens = torch.randint(0, C, (rows, 1), device=device)
+    mask = _mask(1, rows, device)
+    got = k2.get_token_logprobs(x, tokens, mask=mask, num_top=2, return_entropy=True)
+    orc.check_token_logprobs(x.detach(), tokens, mask, 1.0, 2, k2.TokenLogprobs(*(u.detach() for u in got)))
+    up = torch.randn(rows, 1, device=device)
+    (grad,) = torch.autograd.grad(got.logprobs, x, up)
+    orc.check_token_grad(x.detach(), tokens, mask, 1.0, (up, None, None), None, grad)
+    a, t = orc.teacher_case(2, x.detach(), 3, 1.0)
+    loss = k2.distillation_loss(x, a, t, mask=mask, rest="bucket", reduction="none")
+    up = torch.randn(rows, device=device)
+    (grad,) = torch.autograd.grad(loss, x, up)
+    orc.check_distillation(x.detach(), a, t, mask, 1.0, True, loss.detach(), up, grad)
+    total = k2.distillation_loss(x, a, t, mask=mask, rest="bucket", reduction="sum")
+    assert abs(total.double() - loss.double().sum()) <= 1e-6 * loss.double().abs().sum()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_not_numbers(device, dtype):
     """NaN and +inf make their row's results NaN and no other's; a NaN is listed before every number; rows masked out may
     hold anything."""
@@ -495,4 +542,4 @@ def test_refusals_on_the_device(device):
         got = k2.get_token_logprobs(x, torch.zeros(4, dtype=torch.int64, device=device)).logprobs
         (g,) = torch.autograd.grad(got.sum(), x, create_graph=True)
         g.sum().backward()
-    assert not math.isnan(float(k2.get_token_logprobs(x, torch.zeros(4, dtype=torch.int64)).logprobs.sum()))  # tokens move
+    assert not math.isnan(float(k2.get_token_logprobs(x.detach(), torch.zeros(4, dtype=torch.int64)).logprobs.sum()))  # tokens move
