@@ -5,6 +5,12 @@
 //   dx_i = 1/tau [ sum_{j: c_j = i} g_j - p_i sum_j g_j - gH p_i (log p_i + H) ]
 //
 // with c_j the given tokens and the alternatives together and g_j what reaches their log-probs.
+//
+// Measured on an MI355X, kernel times: 80000 x 500 float32, four fifths of the rows, 8 alternatives, 45 us (20 us to read them;
+// the arithmetic, half of it the selection, keeps the vector units busy for 27); 4096 x 32000 bfloat16 with 64 alternatives
+// 102 us (41 to read; the selection is two thirds of the instructions); 6553 of 8191 x 32000 bfloat16 with entropy 86 us
+// (4.9 TB/s), and their gradient 159 us (419 MB read, 524 MB written: 5.9 TB/s); one row of 131072 with 20 alternatives
+// 8.4 us in 16 parts and 7.3 us for their join.
 #include "token_rows.h"
 
 namespace k2amd {
@@ -192,7 +198,8 @@ __device__ __forceinline__ void WriteRow(const ForwardArgs &a, size_t row, int i
   }
 }
 
-// Short rows: 16 lanes each, four rows a wavefront.  What a row depends on (mask, tokens) is asked for first and together, then
+// Short rows: 16 lanes each, four rows a wavefront (a wavefront a row took the same 47 us as this at first, and the selection
+// four times the instructions a row).  What a row depends on (mask, tokens) is asked for first and together, then
 // the row.  Every vector of a row is a group of the threshold's; each row has a threshold of its own, so that the counting is
 // done in the 16 lanes of the row.  A lane collects which of its elements reach it in bits and then lists them one after the
 // other, reading each again (it is in the nearest cache): the list's code is run as often as the busiest lane has elements in
