@@ -144,8 +144,8 @@ __device__ __forceinline__ int VecBase(int q, int C) {
   return max(0, min(q * kN, C - kN));
 }
 
-// Vector q of row x (q < VecsOf(C)), elements that belong to the vector in front of it as -inf.  `ragged`: uniform, whether
-// q may be the incomplete last vector.
+// Vector q of row x (q < VecsOf(C)), elements that belong to the vector in front of it as -inf.  `ragged`: whether q may be the
+// row's incomplete last vector.
 template <typename T>
 __device__ __forceinline__ Vec LoadRowVec(const T *x, int q, int C, bool ragged) {
   constexpr int kN = Lanes<T>::kN;

@@ -106,7 +106,7 @@ def get_token_logprobs(
       logits: [..., C].
       tokens: int64, the shape of the rows ([...]: one token a row) or [..., n] with n <= 64.  A negative token (padding)
         has log-prob 0 and adds nothing to the gradient; one of C and above is a mistake and gives NaN.
-      mask: bool [...]; rows with False are not read: log-prob 0, entropy 0, no alternatives, gradient 0.
+      mask: bool [...]; rows with False do not count, whatever they hold: log-prob 0, entropy 0, no alternatives, gradient 0.
       temperature: positive.
       num_top: how many alternatives to list, at most 64: the largest logits of each row in falling order, the lower index
         first where two are equal.
@@ -174,7 +174,7 @@ def distillation_loss(
       top_logprobs: [..., K] with K <= 256, the teacher's log-probs at the same temperature; no gradient flows to them.
       top_tokens: int64 [..., K]; a negative one is no entry, one of C and above is a mistake and gives NaN.  A token listed
         twice counts with both entries.
-      mask: bool [...]; rows with False are not read and have loss 0 and gradient 0.
+      mask: bool [...]; rows with False do not count, whatever they hold: loss 0, gradient 0.
       rest: "renormalise" scales the listed probabilities to sum to one; "bucket" leaves them as they are and compares what
         they leave of one with the student's total outside the list, as one more outcome (a row whose student has nothing
         outside the list has no such outcome).

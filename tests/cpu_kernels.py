@@ -6,9 +6,9 @@ numpy buffers (or CPU tensors, through the product's own Python layer).  Most fi
 but plain HIP (LDS, barriers, wavefront shuffles, atomics); rnnt_simple.hip and joiner.hip besides
 that the two matrix instructions (fp32 and bfloat16 operands), which the stand-in computes from
 their documented operand layouts, mi_wave.hip two DPP lane shifts, readlane and agent-scope
-atomics.  Two files are compiled from copies in which the lines that the host compiler cannot
-parse are replaced, and not a character else (EDITS below): joiner.hip (three spellings) and
-mi_fast.hip, the pipelined mutual-information kernels and the single launch, whose inline assembly
+atomics.  Four files are compiled from copies in which the lines that the host compiler cannot
+parse are replaced, and not a character else (EDITS below): joiner.hip (three spellings),
+token_logprobs.hip and distillation.hip (what token_rows.h spells of 16-bit types) and mi_fast.hip, the pipelined mutual-information kernels and the single launch, whose inline assembly
 (two DPP arithmetic instructions, buffer loads, coherent loads and stores, wait counts) gives way
 to calls that do what the instructions do.  The ctypes signatures are k2_amd/capi.py's own table,
 so a wrong entry there shows up here as well.
@@ -58,7 +58,7 @@ TOKEN_ROWS_EDITS = [
 ]
 
 
-# Two sources hold lines that the host compiler cannot parse; the host build compiles copies in
+# Four sources hold lines that the host compiler cannot parse; the host build compiles copies in
 # which exactly these are replaced and not a character else.  (old, new, count): a literal that
 # must be found `count` times (None: at least once); a compiled pattern replaces every match.
 EDITS = {
