@@ -207,35 +207,32 @@ __device__ __forceinline__ void WriteRow(const ForwardArgs &a, size_t row, int i
 constexpr int kShort = 16, kShortRows = 16;
 constexpr int kThreads = kShort * kShortRows;
 
-template <int U>
-__device__ __forceinline__ int RowGroupsReaching(const float (&group)[U], float v) {
-  int n = 0;
-#pragma unroll
-  for (int u = 0; u < U; ++u) n += group[u] >= v ? 1 : 0;
-  n += __builtin_amdgcn_update_dpp(0, n, 0xb1, 0xf, 0xf, false);  // (the moves of GroupSum)
+__device__ __forceinline__ int RowSum(int n) {  // (the moves of GroupSum)
+  n += __builtin_amdgcn_update_dpp(0, n, 0xb1, 0xf, 0xf, false);
   n += __builtin_amdgcn_update_dpp(0, n, 0x4e, 0xf, 0xf, false);
   n += __builtin_amdgcn_update_dpp(0, n, 0x141, 0xf, 0xf, false);
   return n + __builtin_amdgcn_update_dpp(0, n, 0x140, 0xf, 0xf, false);
 }
 
-// as Threshold above, for each of the wavefront's rows
-template <int U>
-__device__ __forceinline__ float RowThreshold(const float (&group)[U], float high, int k) {
+// as Threshold above, for each of the wavefront's rows; reaching(v): how many of a row's groups (or elements) reach v
+template <typename Reaching>
+__device__ __forceinline__ float RowThreshold(float high, int k, const Reaching &reaching) {
   float lo = high, hi = high;
-  bool found = RowGroupsReaching(group, high) >= k, done = found;
-#pragma unroll
+  bool found = reaching(high) >= k, done = found;
+#pragma unroll 1
   for (int i = 0; i < 3; ++i) {
     if (__ballot(!found) == 0) continue;
     const float v = high - (i == 0 ? 8.0f : i == 1 ? 64.0f : 4096.0f);
-    const bool reached = RowGroupsReaching(group, v) >= k;
+    const bool reached = reaching(v) >= k;
     if (!found) (reached ? lo : hi) = v;
     found |= reached;
   }
   if (!found) lo = Real<float>::NegInf();
   done |= !found;
+#pragma unroll 1
   for (int step = 0; step < 24 && __ballot(!done) != 0; ++step) {
     const float mid = 0.5f * (lo + hi);
-    const int n = RowGroupsReaching(group, mid);
+    const int n = reaching(mid);
     if (!done) (n >= k ? lo : hi) = mid;
     done |= n >= k && n <= k + (k >> 1) + 2;
   }
@@ -287,7 +284,32 @@ __global__ __launch_bounds__(kThreads) void TokenShortKernel(const T *__restrict
   unsigned long long *list = lists[in_block];
   if (lane == 0) listed[in_block] = 0;
   const bool odd = sums.s != sums.s;  // a NaN or +inf among them
-  const float threshold = RowThreshold<U>(group, live && !odd ? high : Real<float>::NegInf(), live && !odd ? a.k : 0);
+  const float from = live && !odd ? high : Real<float>::NegInf();
+  const int wanted = live && !odd ? a.k : 0;
+  float threshold;
+  if (2 * a.k <= VecsOf<T>(a.C)) {
+    threshold = RowThreshold(from, wanted, [&](float v) {
+      int n = 0;
+#pragma unroll
+      for (int u = 0; u < U; ++u) n += group[u] >= v ? 1 : 0;
+      return RowSum(n);
+    });
+  } else {
+    // so many that the k-th largest of the groups' maxima says little: the elements themselves are counted (64000 x 500
+    // bfloat16 with 64 alternatives by groups listed more than there is room for in nearly every row, and took 1019 us)
+    threshold = RowThreshold(from, wanted, [&](float v) {
+      int n = 0;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        Vec x;  // (a copy: the branch must not get vectors of its own)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x.w[i] = Anew(part.v[u].w[i]);
+#pragma unroll
+        for (int e = 0; e < kN; ++e) n += ElementOf<T>(x, e) >= v ? 1 : 0;
+      }
+      return RowSum(n);
+    });
+  }
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   constexpr int kPerWord = 32 / kN;  // vectors whose elements share a word of bits
 #pragma unroll
@@ -301,10 +323,11 @@ __global__ __launch_bounds__(kThreads) void TokenShortKernel(const T *__restrict
       unsigned of_vector = 0;
 #pragma unroll
       for (int e = 0; e < kN; ++e) of_vector |= ElementOf<T>(v, e) >= threshold ? 1u << e : 0u;
-      // (the -inf that pads a row is no element of it)
-      const int q = part.VectorAnew(u, 0, 0, lane), base = VecBase<T>(q, a.C);
-      of_vector &= q < VecsOf<T>(a.C) ? ((1u << kN) - 1) << min(kN, q * kN - base) : 0u;
-      if (base + kN > a.C) of_vector &= (1u << (a.C - base)) - 1;
+      if ((u + 1) * kShort * kN > a.C) {  // the round with the row's end: the -inf that pads a row is no element of it
+        const int q = part.VectorAnew(u, 0, 0, lane), base = VecBase<T>(q, a.C);
+        of_vector &= q < VecsOf<T>(a.C) ? ((1u << kN) - 1) << min(kN, q * kN - base) : 0u;
+        if (base + kN > a.C) of_vector &= (1u << (a.C - base)) - 1;
+      }
       bits |= of_vector << (i * kN);
     }
     if (!live || odd) bits = 0;
