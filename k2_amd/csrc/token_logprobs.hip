@@ -580,6 +580,7 @@ struct BackwardArgs {
 // dx of an element that is no entry: -p (G + gH (log p + H)) / tau, with 1 / (s tau) in the coefficients
 struct SoftmaxGrad {
   float m, c, flat, slope;
+  float entry;  // what an entry's own gradient is multiplied by: 1 / tau
   __device__ __forceinline__ float At(float x) const {
     const float d = (x - m) * c;
     return Exp2(d) * (flat + slope * fmaxf(d, kNothing));
@@ -610,8 +611,9 @@ __device__ __forceinline__ SoftmaxGrad RowGradOf(const BackwardArgs &a, size_t r
   const float s = a.stats[2 * row + 1];
   const float h = a.entropy_grad != nullptr ? a.entropy[row] : 0.0f;
   const float gh = a.entropy_grad != nullptr ? a.entropy_grad[row] : 0.0f;
-  SoftmaxGrad f{a.stats[2 * row], a.c, 0.0f, 0.0f};
-  if (s != 0.0f) {  // (a row without any mass: every p is 0)
+  SoftmaxGrad f{a.stats[2 * row], a.c, 0.0f, 0.0f, 0.0f};
+  if (s != 0.0f) {  // (a row without any mass: every p is 0, and no logit moves a log-prob)
+    f.entry = a.inv_tau;
     const float inv_s = a.inv_tau / s;
     f.flat = -inv_s * (sum + gh * (h - kLn2 * Log2(s)));
     f.slope = -inv_s * gh * kLn2;
@@ -624,7 +626,7 @@ __device__ __forceinline__ SoftmaxGrad RowGradOf(const BackwardArgs &a, size_t r
 // The entries' columns of [begin, end) over what is at `to` (column `begin` first), entry by entry of the n work-items.
 template <typename T>
 __device__ __forceinline__ void WriteEntries(const T *x, T *to, const int *entry, const float *entry_grad, int entries,
-                                             int begin, int end, int i, int n, const SoftmaxGrad &f, float inv_tau) {
+                                             int begin, int end, int i, int n, const SoftmaxGrad &f) {
   for (; i < entries; i += n) {
     const int token = entry[i];
     if (token < begin || token >= end) continue;
@@ -632,7 +634,7 @@ __device__ __forceinline__ void WriteEntries(const T *x, T *to, const int *entry
     float own = 0.0f;  // a token that is listed twice takes both gradients
     for (int j = 0; j < entries; ++j)
       if (entry[j] == token) own += entry_grad[j];
-    FromFloat(f.At(xi) + own * inv_tau, &to[token - begin]);
+    FromFloat(f.At(xi) + (f.entry != 0.0f ? own * f.entry : 0.0f), &to[token - begin]);
   }
 }
 
@@ -671,7 +673,7 @@ __global__ __launch_bounds__(kThreads) void TokenShortGradKernel(const T *__rest
   }
   // (what is written above, and the list, are before what follows for every lane of the wavefront)
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  WriteEntries(x, to, entry, entry_grad, live ? entries : 0, 0, a.C, lane, kShort, f, a.inv_tau);
+  WriteEntries(x, to, entry, entry_grad, live ? entries : 0, 0, a.C, lane, kShort, f);
   if (kStage == 0) return;
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
@@ -715,7 +717,7 @@ __global__ __launch_bounds__(W *kWave) void TokenLongGradKernel(const T *__restr
   if (entries == 0) return;
   __syncthreads();
   const int begin = first * kN, end = (int)min((long long)a.C, (long long)(first + U * W * kWave) * kN);
-  WriteEntries(x, dx + begin, entry, entry_grad, entries, begin, end, (int)threadIdx.x, W * kWave, f, a.inv_tau);
+  WriteEntries(x, dx + begin, entry, entry_grad, entries, begin, end, (int)threadIdx.x, W * kWave, f);
 }
 
 // ---- launches ---------------------------------------------------------------------------------------

@@ -177,6 +177,23 @@ def test_nothing_outside_the_tensors_is_touched(lib, at, dtype, code, C):
         assert inv.a[0] == 0.5 and out.intact() and inv.intact() and scratch.intact()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("C", [1, 40, 700, 2300])
+def test_rows_of_nothing_get_no_gradient(host, C, dtype):
+    """A row of nothing but -inf: log-probs that no logit moves, whichever of them are asked for."""
+    import k2_amd as k2
+    x = orc.logits_case(C, 3, C, dtype, CPU)
+    x[1] = NEG
+    x.requires_grad_()
+    got = k2.get_token_logprobs(x, torch.tensor([[0, C - 1]] * 3), num_top=2, return_entropy=True)
+    assert got.logprobs[1].eq(NEG).all() and got.entropy[1] == 0 and got.top_logprobs[1].eq(NEG).all()
+    ups = [torch.full_like(u, 3.0) for u in (got.logprobs, got.entropy, got.top_logprobs)]
+    ups[0][1, 0] = float("inf")  # what a loss of exp(-logprob) would send back
+    (grad,) = torch.autograd.grad([got.logprobs, got.entropy, got.top_logprobs], x, ups)
+    assert grad[1].eq(0).all()
+    assert C == 1 or (grad[0].ne(0).any() and grad[2].ne(0).any())
+
+
 def test_entry_points_refuse_before_launching():
     """On the library itself: wrong arguments come back as codes; pointers are never looked at."""
     import ctypes

@@ -255,6 +255,21 @@ def test_gradients_of_log_probs_entropy_and_alternatives(device, dtype, C, n, k)
         assert grad[5].eq(0).all()
 
 
+@pytest.mark.parametrize("C", [5, 500, 4999, 131072])
+def test_rows_of_nothing_get_no_gradient(device, C):
+    """A row of nothing but -inf: log-probs that no logit moves, whatever is sent back through them."""
+    import k2_amd as k2
+    for dtype in DTYPES:
+        x = orc.logits_case(C, 3, C, dtype, device)
+        x[1] = NEG
+        x.requires_grad_()
+        got = k2.get_token_logprobs(x, torch.tensor([[0, C - 1]] * 3, device=device), num_top=2, return_entropy=True)
+        ups = [torch.full_like(u, 3.0) for u in (got.logprobs, got.entropy, got.top_logprobs)]
+        ups[0][1, 0] = float("inf")
+        (grad,) = torch.autograd.grad([got.logprobs, got.entropy, got.top_logprobs], x, ups)
+        assert grad[1].eq(0).all() and grad[0].ne(0).any() and grad[2].ne(0).any()
+
+
 def test_gradients_against_differences(device):
     """Central differences of the operators themselves along random directions: f(x + h v) - f(x - h v) over 2 h.  The two
     values are each at most E off (the forward budgets: some 1e-5 for sums of a few rows) and the third derivative of a
