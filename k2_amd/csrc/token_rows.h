@@ -504,6 +504,7 @@ __device__ __forceinline__ float LogitOf(unsigned long long key) {
 inline bool RowsOk(long long rows, long long row_stride, int C, float temperature, int dtype) {
   if (rows < 0 || C < 1 || row_stride < 0) return false;
   if (!(temperature > 0.0f) || temperature - temperature != 0.0f) return false;
+  if (!(kLog2E / (double)temperature <= 3.40282346e38)) return false;  // (c of the kernels would be infinite)
   return dtype == K2AMD_F32 || dtype == K2AMD_F16 || dtype == K2AMD_BF16;
 }
 inline bool RowsServed(long long rows, int C) { return rows < (1ll << 31) && C <= kMaxColumns; }

@@ -107,7 +107,7 @@ def get_token_logprobs(
       tokens: int64, the shape of the rows ([...]: one token a row) or [..., n] with n <= 64.  A negative token (padding)
         has log-prob 0 and adds nothing to the gradient; one of C and above is a mistake and gives NaN.
       mask: bool [...]; rows with False do not count, whatever they hold: log-prob 0, entropy 0, no alternatives, gradient 0.
-      temperature: positive.
+      temperature: positive; it and log2(e) / temperature have to be float32 numbers.
       num_top: how many alternatives to list, at most 64: the largest logits of each row in falling order, the lower index
         first where two are equal.
       return_entropy: whether to return the entropy of each row.

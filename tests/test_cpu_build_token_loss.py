@@ -194,6 +194,19 @@ def test_rows_of_nothing_get_no_gradient(host, C, dtype):
     assert C == 1 or (grad[0].ne(0).any() and grad[2].ne(0).any())
 
 
+@pytest.mark.parametrize("temperature", [1e-50, 1e-40, 4e-39, 1e39])
+def test_temperatures_out_of_range(host, temperature):
+    """log2 e / temperature has to be a float32 number."""
+    import k2_amd as k2
+    x = torch.randn(3, 9)
+    with pytest.raises(Exception, match="invalid argument"):
+        k2.get_token_logprobs(x, torch.zeros(3, dtype=torch.int64), temperature=temperature)
+    with pytest.raises(Exception, match="invalid argument"):
+        k2.distillation_loss(x, torch.zeros(3, 2), torch.zeros(3, 2, dtype=torch.int64), temperature=temperature)
+    got = k2.get_token_logprobs(x, temperature=5e-39, num_top=1, return_entropy=True)
+    assert got.top_logprobs.eq(0).all() and got.entropy.eq(0).all()
+
+
 def test_entry_points_refuse_before_launching():
     """On the library itself: wrong arguments come back as codes; pointers are never looked at."""
     import ctypes
