@@ -460,7 +460,7 @@ K2AMD_API int k2amd_token_logprobs_backward(const void *logits, long long row_st
                                             long long rows, int C, int n, int k, float temperature, int dtype, void *stream);
 
 /* Distillation from a teacher's list of K <= 256 tokens a row: top_tokens [rows][K] int64 (negative: no entry; past the
- * vocabulary: the row's loss is NaN), top_logprobs [rows][K].  rest == 0: the list is renormalised (q = softmax of its
+ * vocabulary: the row's loss and gradient are NaN), top_logprobs [rows][K] (NaN or +inf at a token: likewise NaN).  rest == 0: the list is renormalised (q = softmax of its
  * log-probs); rest != 0: q = exp(log-probs) and what they leave of 1 is one more outcome, the student's counterpart of
  * which is everything that is not listed (a row without any student mass there has no such outcome).
  * scratch: as above, k2amd_distillation_scratch_bytes(...) bytes.

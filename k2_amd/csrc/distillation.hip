@@ -41,7 +41,8 @@ struct List {
 };
 enum ListState { kNone, kUsable, kWrong };
 
-// The tokens and the teacher's log-probs.
+// The tokens and the teacher's log-probs.  A log-prob of NaN or +inf (a teacher whose logits overflowed) is as wrong as a
+// token past the vocabulary: the comparisons that follow would take it for an entry without weight.
 template <int L>
 __device__ __forceinline__ ListState ReadList(int C, const float *top_logprobs, const int64_t *top_tokens, const List &list,
                                               int lane, bool live) {
@@ -51,7 +52,7 @@ __device__ __forceinline__ ListState ReadList(int C, const float *top_logprobs, 
       const int64_t given = top_tokens[j];
       const float a = top_logprobs[j];
       const int token = given >= 0 && given < C ? (int)given : -1;
-      wrong |= given >= C;
+      wrong |= given >= C || (token >= 0 && !(a < -Real<float>::NegInf()));
       present |= token >= 0;
       list.token[j] = token;
       list.a[j] = token >= 0 ? a : Real<float>::NegInf();
@@ -186,8 +187,8 @@ __device__ __forceinline__ void FinishRow(List list, ListState state, unsigned r
     }
   }
   if (lane != 0) return;
-  // no list (without a rest, one of impossible tokens alone is none): nothing to learn; an index past the vocabulary is a
-  // mistake of the caller's and shows as NaN
+  // no list (without a rest, one of impossible tokens alone is none): nothing to learn; an index past the vocabulary or a
+  // log-prob that is none is a mistake of the caller's and shows as NaN
   const bool skipped = !live || state == kNone || (state == kUsable && !kRest && a_max == Real<float>::NegInf());
   const float nan = __uint_as_float(0x7fc00000u);
   *loss_out = skipped ? 0.0f : state == kWrong ? nan : loss;

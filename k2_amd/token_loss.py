@@ -171,7 +171,9 @@ def distillation_loss(
 
     Args:
       logits: the student's, [..., C]; its distribution is softmax(logits / temperature).
-      top_logprobs: [..., K] with K <= 256, the teacher's log-probs at the same temperature; no gradient flows to them.
+      top_logprobs: [..., K] with K <= 256, the teacher's log-probs at the same temperature; no gradient flows to them.  NaN or
+        +inf at a token (what a teacher row gives that overflowed its type) makes its row's loss and gradient NaN; -inf is
+        probability 0.
       top_tokens: int64 [..., K]; a negative one is no entry, one of C and above is a mistake and gives NaN.  A token listed
         twice counts with both entries.
       mask: bool [...]; rows with False do not count, whatever they hold: loss 0, gradient 0.

@@ -1,0 +1,46 @@
+"""Calls of k2_amd/token_loss.py at the edges of what it takes, on the host build of the kernels through both host layers: lists
+with values that are no log-probs."""
+import pytest
+import torch
+
+import token_oracle as orc
+from test_cpu_build_host_layer import host_on_cpu  # noqa: F401  (a fixture)
+from test_cpu_build_token_loss import host  # noqa: F401  (a fixture)
+
+CPU = torch.device("cpu")
+NEG, INF, NAN = float("-inf"), float("inf"), float("nan")
+
+
+# (short rows; rows that wavefronts read along; rows in two parts)
+@pytest.mark.parametrize("C,dtype", [(40, torch.float32), (700, torch.bfloat16), (1100, torch.float32), (4200, torch.float32)])
+def test_lists_that_hold_no_log_probs(host, C, dtype):  # noqa: F811
+    """NaN or +inf at a listed token makes its row's loss and gradient NaN and no other's; at a token that is absent, and in a
+    row that is masked out, it says nothing.  -inf is probability 0."""
+    import k2_amd as k2
+    x = orc.logits_case(C, 7, C, dtype, CPU).requires_grad_()
+    a, t = orc.teacher_case(1, x.detach(), 4, 1.0)
+    a[0, 1] = NAN
+    a[1] = NAN
+    a[2, 3] = INF
+    a[3, 0], t[3, 0] = NAN, -1
+    a[4] = NAN
+    a[5, 2] = NEG
+    mask = torch.tensor([True, True, True, True, False, True, True])
+    wrong = torch.tensor([True, True, True, False, False, False, False])
+    for bucket in (False, True):
+        loss = k2.distillation_loss(x, a, t, mask=mask, rest="bucket" if bucket else "renormalise", reduction="none")
+        (grad,) = torch.autograd.grad(loss, x, torch.ones_like(loss))
+        assert torch.equal(loss.isnan(), wrong), loss
+        assert grad[wrong].isnan().all() and torch.isfinite(grad[~wrong]).all()
+        a0 = torch.where(t < 0, torch.full_like(a, NEG), a)
+        orc.check_distillation(x.detach()[~wrong], a0[~wrong], t[~wrong], mask[~wrong], 1.0, bucket, loss.detach()[~wrong],
+                               torch.ones(4), grad[~wrong])
+        for reduction in ("sum", "mean"):
+            assert k2.distillation_loss(x, a, t, mask=mask, rest="bucket" if bucket else "renormalise", reduction=reduction).isnan()
+    # from a teacher's row that overflowed, as its labelling lists it
+    teacher = x.detach().clone()
+    teacher[6, 5] = INF
+    labels = k2.get_token_logprobs(teacher, num_top=4)
+    assert labels.top_tokens[6].ge(0).all()
+    loss = k2.distillation_loss(x, labels.top_logprobs, labels.top_tokens, reduction="none")
+    assert loss[6].isnan() and torch.isfinite(loss[:6]).all()

@@ -1,0 +1,45 @@
+"""Calls of k2_amd/token_loss.py at the edges of what it takes, on the GPU: lists with values that are no log-probs."""
+import pytest
+import torch
+
+import token_oracle as orc
+
+pytestmark = pytest.mark.gpu
+DTYPES = [torch.float32, torch.float16, torch.bfloat16]
+NEG, INF, NAN = float("-inf"), float("inf"), float("nan")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("C", [40, 500, 1237, 5000, 40001])
+def test_lists_that_hold_no_log_probs(device, dtype, C):
+    """NaN or +inf at a listed token makes its row's loss and gradient NaN and no other's; at a token that is absent, and in a
+    row that is masked out, it says nothing."""
+    import k2_amd as k2
+    rows, K = 9, 6
+    x = orc.logits_case(C, rows, C, dtype, device).requires_grad_()
+    a, t = orc.teacher_case(1, x.detach(), K, 1.0)
+    a[0, 1] = NAN
+    a[1] = NAN
+    a[2, 3] = INF
+    a[3, 0], t[3, 0] = NAN, -1
+    a[4] = NAN
+    a[5, 2] = NEG
+    mask = torch.ones(rows, dtype=torch.bool, device=device)
+    mask[4] = False
+    wrong = torch.zeros_like(mask)
+    wrong[:3] = True
+    a0 = torch.where(t < 0, torch.full_like(a, NEG), a)
+    for rest in ("renormalise", "bucket"):
+        loss = k2.distillation_loss(x, a, t, mask=mask, rest=rest, reduction="none")
+        (grad,) = torch.autograd.grad(loss, x, torch.ones_like(loss))
+        assert torch.equal(loss.isnan(), wrong)
+        assert grad[wrong].isnan().all()
+        keep = ~wrong
+        orc.check_distillation(x.detach()[keep], a0[keep], t[keep], mask[keep], 1.0, rest == "bucket", loss.detach()[keep],
+                               torch.ones(rows - 3, device=device), grad[keep])
+        assert k2.distillation_loss(x, a, t, mask=mask, rest=rest).isnan()
+    teacher = x.detach().clone()
+    teacher[6, 5] = INF
+    labels = k2.get_token_logprobs(teacher, num_top=4)
+    loss = k2.distillation_loss(x, labels.top_logprobs, labels.top_tokens, reduction="none")
+    assert loss[6].isnan() and int(loss.isnan().sum()) == 1
