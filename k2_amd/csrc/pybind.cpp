@@ -1117,10 +1117,20 @@ struct TokenLogprobsNode : public torch::autograd::Function<TokenLogprobsNode> {
   }
 };
 
+// Whether a tensor carries a tangent of forward-mode differentiation, which these operators do not have: where no gradient
+// is asked for either, the kernels would run without their node and drop it.
+bool CarriesTangent(const torch::Tensor &t) {
+  return c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined();
+}
+void RefuseTangent(const torch::Tensor &t, const char *name) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!CarriesTangent(t), "k2_amd: ", name, " carry a tangent: there is no forward-mode derivative");
+}
+
 // get_token_logprobs: (logprobs, entropy, top_logprobs, top_tokens)
 std::tuple<OptionalTensor, OptionalTensor, OptionalTensor, OptionalTensor> TokenLogprobs(
     const torch::Tensor &logits, const OptionalTensor &tokens, const OptionalTensor &mask, double temperature, int64_t num_top,
     bool return_entropy) {
+  RefuseTangent(logits, "logits");
   if (!at::GradMode::is_enabled() || !logits.requires_grad()) {
     auto out = TokenLogprobsForward(logits, tokens, mask, temperature, num_top, return_entropy, false);
     return std::make_tuple(std::get<0>(out), std::get<1>(out), std::get<2>(out), std::get<3>(out));
@@ -1174,6 +1184,8 @@ struct DistillationNode : public torch::autograd::Function<DistillationNode> {
 torch::Tensor Distillation(const torch::Tensor &logits, const torch::Tensor &top_logprobs, const torch::Tensor &top_tokens,
                            const OptionalTensor &mask, double temperature, bool bucket, int64_t sums, bool mean, double factor,
                            bool scalar) {
+  RefuseTangent(logits, "logits");
+  RefuseTangent(top_logprobs, "top_logprobs");
   if (at::GradMode::is_enabled() && logits.requires_grad())
     return DistillationNode::apply(logits, top_logprobs, top_tokens, mask, temperature, bucket, sums, mean, factor, scalar);
   auto out = DistillationForward(logits, top_logprobs, top_tokens, mask, temperature, bucket, false);

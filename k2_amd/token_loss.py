@@ -4,7 +4,8 @@ from a teacher's listed log-probs, on any batch of rows and on the pruned lattic
 
 No counterpart in the reference.  Each is one fused HIP kernel forward and one backward (k2_amd/csrc/token_logprobs.hip,
 k2_amd/csrc/distillation.hip) behind a torch.autograd.Function.  Logits are float32, float16 or bfloat16 device tensors,
-[..., C], any strides; sums and results are float32, gradients have the logits' type.
+[..., C], any strides; sums and results are float32, gradients have the logits' type.  There are no second derivatives, and no
+forward-mode ones: a tensor that carries a tangent is refused (NotImplementedError).
 """
 import math
 from typing import NamedTuple, Optional
@@ -33,7 +34,7 @@ class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, tokens, mask, temperature, num_top, return_entropy):
         logprobs, entropy, top_logprobs, top_tokens, stats = native.token_logprobs_forward(
-            logits, tokens, mask, temperature, num_top, return_entropy, True)
+            logits, tokens, mask, temperature, num_top, return_entropy, ctx.needs_input_grad[0])
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(logits, tokens, mask, stats, entropy, top_tokens)
         ctx.temperature = temperature
@@ -128,10 +129,7 @@ def get_token_logprobs(
     args = (logits, tokens, mask, float(temperature), num_top, bool(return_entropy))
     results = native.token_logprobs(*args)
     if results is None:
-        if torch.is_grad_enabled() and logits.requires_grad:
-            results = _TokenLogprobs.apply(*args)
-        else:
-            results = native.token_logprobs_forward(*args, False)[:4]
+        results = _TokenLogprobs.apply(*args)
     return TokenLogprobs(*results)
 
 

@@ -1,5 +1,5 @@
 """Calls of k2_amd/token_loss.py at the edges of what it takes, on the host build of the kernels through both host layers: lists
-with values that are no log-probs."""
+with values that are no log-probs, forward-mode tangents."""
 import pytest
 import torch
 
@@ -44,3 +44,26 @@ def test_lists_that_hold_no_log_probs(host, C, dtype):  # noqa: F811
     assert labels.top_tokens[6].ge(0).all()
     loss = k2.distillation_loss(x, labels.top_logprobs, labels.top_tokens, reduction="none")
     assert loss[6].isnan() and torch.isfinite(loss[:6]).all()
+
+
+@pytest.mark.parametrize("requires_grad", [False, True])
+@pytest.mark.parametrize("grad_mode", [False, True])
+def test_forward_mode_is_refused(host, requires_grad, grad_mode):  # noqa: F811
+    """A tangent is never dropped: with or without a gradient besides, in logits and in the teacher's log-probs."""
+    import k2_amd as k2
+    import torch.autograd.forward_ad as fw
+    x = torch.randn(3, 9).requires_grad_(requires_grad)
+    tokens, a, t = torch.zeros(3, dtype=torch.int64), torch.full((3, 2), -1.0), torch.tensor([[1, 2]] * 3)
+    lattice = (torch.arange(3).reshape(1, 1, 3), torch.tensor([[0, 0, 2, 1]]))
+    with torch.set_grad_enabled(grad_mode), fw.dual_level():
+        dual = fw.make_dual(x, torch.ones(3, 9))
+        listed = fw.make_dual(a, torch.ones(3, 2))
+        for call in (lambda: k2.get_token_logprobs(dual, tokens), lambda: k2.get_token_logprobs(dual, return_entropy=True, num_top=2),
+                     lambda: k2.distillation_loss(dual, a, t), lambda: k2.distillation_loss(x, listed, t, reduction="none"),
+                     lambda: k2.rnnt_distillation_loss_pruned(dual.view(1, 1, 3, 9), a.view(1, 1, 3, 2), t.view(1, 1, 3, 2), *lattice)):
+            with pytest.raises(NotImplementedError):
+                call()
+        # the primal alone is as good as any tensor, and so is a level that nothing was made dual in
+        assert torch.equal(k2.get_token_logprobs(fw.unpack_dual(dual).primal, tokens).logprobs,
+                           k2.get_token_logprobs(x, tokens).logprobs)
+    assert k2.get_token_logprobs(x, tokens).logprobs.requires_grad == requires_grad

@@ -1,4 +1,4 @@
-"""Calls of k2_amd/token_loss.py at the edges of what it takes, on the GPU: lists with values that are no log-probs."""
+"""Calls of k2_amd/token_loss.py at the edges of what it takes, on the GPU: lists with values that are no log-probs, forward-mode tangents."""
 import pytest
 import torch
 
@@ -43,3 +43,18 @@ def test_lists_that_hold_no_log_probs(device, dtype, C):
     labels = k2.get_token_logprobs(teacher, num_top=4)
     loss = k2.distillation_loss(x, labels.top_logprobs, labels.top_tokens, reduction="none")
     assert loss[6].isnan() and int(loss.isnan().sum()) == 1
+
+
+@pytest.mark.parametrize("requires_grad", [False, True])
+def test_forward_mode_is_refused(device, requires_grad):
+    """A tangent is never dropped, whether or not a gradient is asked for besides."""
+    import k2_amd as k2
+    import torch.autograd.forward_ad as fw
+    x = torch.randn(3, 9, device=device).requires_grad_(requires_grad)
+    a, t = torch.full((3, 2), -1.0, device=device), torch.tensor([[1, 2]] * 3, device=device)
+    with fw.dual_level():
+        dual, listed = fw.make_dual(x, torch.ones(3, 9, device=device)), fw.make_dual(a, torch.ones(3, 2, device=device))
+        for call in (lambda: k2.get_token_logprobs(dual, num_top=2), lambda: k2.distillation_loss(dual, a, t),
+                     lambda: k2.distillation_loss(x, listed, t)):
+            with pytest.raises(NotImplementedError):
+                call()
