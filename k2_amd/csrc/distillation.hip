@@ -494,15 +494,17 @@ __global__ __launch_bounds__(kSumThreads) void RowChunkSumKernel(const float *__
                                                                  const uint8_t *__restrict__ mask, int rows_per_sum,
                                                                  double *__restrict__ partial, SumOutput out) {
   __shared__ double lds[2 * kSumThreads / kWave];
-  const int first = (int)blockIdx.x * kChunk, last = gridDim.x == 1 ? rows_per_sum : min(rows_per_sum, first + kChunk);
+  // (64 bits: up to 2^31 - 1 rows, and the end of the last chunk and the step past it lie beyond them)
+  const long long first = (long long)blockIdx.x * kChunk;
+  const long long last = gridDim.x == 1 ? rows_per_sum : min((long long)rows_per_sum, first + kChunk);
   const size_t base = (size_t)blockIdx.y * rows_per_sum;
   double sum = 0, count = 0;
-  for (int i = first + (int)threadIdx.x; i < last; i += 8 * (int)blockDim.x) {
+  for (long long i = first + threadIdx.x; i < last; i += 8 * (int)blockDim.x) {
     float v[8];
     uint8_t m[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const int at = i + j * (int)blockDim.x;
+      const long long at = i + j * (int)blockDim.x;
       v[j] = at < last ? values[base + at] : 0.0f;
       m[j] = at < last ? (mask != nullptr ? mask[base + at] : 1) : 0;
     }

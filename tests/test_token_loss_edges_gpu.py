@@ -1,4 +1,5 @@
-"""Calls of k2_amd/token_loss.py at the edges of what it takes, on the GPU: lists with values that are no log-probs, forward-mode tangents."""
+"""Calls of k2_amd/token_loss.py at the edges of what it takes, on the GPU: lists with values that are no log-probs, forward-mode
+tangents, sums of as many rows as are served."""
 import pytest
 import torch
 
@@ -58,3 +59,18 @@ def test_forward_mode_is_refused(device, requires_grad):
                      lambda: k2.distillation_loss(x, listed, t)):
             with pytest.raises(NotImplementedError):
                 call()
+
+
+@pytest.mark.parametrize("rows", [(1 << 31) - 1, (1 << 31) - 1000, (1 << 31) - 2048])
+def test_sum_of_as_many_rows_as_are_served(device, rows):
+    """The losses next to the 2^31st row: the whole numbers here add up exactly, in double, to far less than 2^24."""
+    from k2_amd import native
+    losses = torch.zeros(rows, device=device)
+    at = torch.tensor([0, 2047, 2048, 16384, 1 << 30, rows - 2500, rows - 2049, rows - 2048, rows - 1048, rows - 2, rows - 1], device=device)
+    losses[at] = torch.arange(1.0, 12.0, device=device)
+    total, _ = native.distillation_sum(losses, None, 1, False, 0.5)
+    assert total.item() == 33.0
+    mask = torch.zeros(rows, dtype=torch.bool, device=device)
+    mask[at] = True
+    mean, inverse = native.distillation_sum(losses, mask, 1, True, 1.0)
+    assert mean.item() == 6.0 and inverse.item() == torch.tensor(1.0 / 11).item()
