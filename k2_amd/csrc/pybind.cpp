@@ -1147,11 +1147,11 @@ std::tuple<OptionalTensor, OptionalTensor, OptionalTensor, OptionalTensor> Token
   return std::make_tuple(out[0], out[1], out[2], out[3]);
 }
 
-// What a distillation loss is reduced to: sums == 0 leaves the rows, n makes n sums of equally many rows each, as a scalar
+// What a distillation loss is reduced to: sums < 0 leaves the rows, n >= 0 makes n sums of equally many rows each, as a scalar
 // where `scalar`; mean divides by the number of rows that count, factor multiplies the sums.
 torch::Tensor ReduceLosses(const torch::Tensor &rows, const OptionalTensor &mask, int64_t sums, bool mean, double factor,
                            bool scalar, OptionalTensor *inverse_count) {
-  if (sums == 0) return rows;
+  if (sums < 0) return rows;
   auto reduced = DistillationSum(rows, mask, sums, mean, factor);
   *inverse_count = std::get<1>(reduced);
   return scalar ? std::get<0>(reduced).reshape({}) : std::get<0>(reduced);

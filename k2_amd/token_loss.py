@@ -54,14 +54,14 @@ class _TokenLogprobs(torch.autograd.Function):
 
 
 class _Distillation(torch.autograd.Function):
-    """The node of the ctypes host, as above.  The loss of each row, or sums of them: ``sums`` 0 leaves the rows, n makes n
-    sums of equally many rows each.  ``mean``: divided by the number of rows that count.  ``factor`` multiplies the sums."""
+    """The node of the ctypes host, as above.  The loss of each row, or sums of them: ``sums`` -1 leaves the rows, n >= 0
+    makes n sums of equally many rows each.  ``mean``: divided by the number of rows that count.  ``factor`` multiplies the sums."""
 
     @staticmethod
     def forward(ctx, logits, top_logprobs, top_tokens, mask, temperature, bucket, sums, mean, factor):
         rows, records = native.distillation_forward(logits, top_logprobs, top_tokens, mask, temperature, bucket,
                                                     ctx.needs_input_grad[0])
-        loss, inverse_count = (rows, None) if sums == 0 else native.distillation_sum(rows, mask, sums, mean, factor)
+        loss, inverse_count = (rows, None) if sums < 0 else native.distillation_sum(rows, mask, sums, mean, factor)
         if records is not None:
             ctx.save_for_backward(logits, top_logprobs, top_tokens, records, inverse_count if mean else None)
             ctx.meta = (temperature, bucket, factor)
@@ -185,7 +185,7 @@ def distillation_loss(
     temperatures."""
     args = _distillation_args(logits, top_logprobs, top_tokens, mask, temperature, rest, reduction)
     if reduction == "none":
-        return _distill(args, 0, False, 1.0, False)
+        return _distill(args, -1, False, 1.0, False)
     return _distill(args, 1, reduction == "mean", 1.0, True)
 
 

@@ -1,5 +1,5 @@
 """Calls of k2_amd/token_loss.py at the edges of what it takes, on the host build of the kernels through both host layers: lists
-with values that are no log-probs, forward-mode tangents."""
+with values that are no log-probs, forward-mode tangents, lattices without rows."""
 import pytest
 import torch
 
@@ -67,3 +67,22 @@ def test_forward_mode_is_refused(host, requires_grad, grad_mode):  # noqa: F811
         assert torch.equal(k2.get_token_logprobs(fw.unpack_dual(dual).primal, tokens).logprobs,
                            k2.get_token_logprobs(x, tokens).logprobs)
     assert k2.get_token_logprobs(x, tokens).logprobs.requires_grad == requires_grad
+
+
+@pytest.mark.parametrize("B,T,R", [(0, 4, 3), (2, 0, 3), (0, 0, 3)])
+def test_lattices_without_rows(host, B, T, R):  # noqa: F811
+    """One loss a sequence, however many sequences and rows of each there are."""
+    import k2_amd as k2
+    x = torch.zeros(B, T, R, 9, requires_grad=True)
+    a, t = torch.zeros(B, T, R, 2), torch.zeros(B, T, R, 2, dtype=torch.int64)
+    ranges, boundary = torch.zeros(B, T, R, dtype=torch.int64), torch.zeros(B, 4, dtype=torch.int64)
+    for box in (None, boundary):
+        for logits in (x, x.detach()):
+            for reduction in ("none", "sum", "mean"):
+                loss = k2.rnnt_distillation_loss_pruned(logits, a, t, ranges, box, reduction=reduction)
+                assert loss.shape == ((B,) if reduction == "none" else ()) and loss.eq(0).all()
+                assert loss.requires_grad == logits.requires_grad
+                if logits.requires_grad:
+                    (grad,) = torch.autograd.grad(loss, x, torch.ones_like(loss))
+                    assert grad.shape == x.shape
+    assert k2.distillation_loss(x, a, t, reduction="none").shape == (B, T, R)

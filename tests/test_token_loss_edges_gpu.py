@@ -1,5 +1,5 @@
 """Calls of k2_amd/token_loss.py at the edges of what it takes, on the GPU: lists with values that are no log-probs, forward-mode
-tangents, sums of as many rows as are served."""
+tangents, sums of as many rows as are served, lattices without rows."""
 import pytest
 import torch
 
@@ -74,3 +74,16 @@ def test_sum_of_as_many_rows_as_are_served(device, rows):
     mask[at] = True
     mean, inverse = native.distillation_sum(losses, mask, 1, True, 1.0)
     assert mean.item() == 6.0 and inverse.item() == torch.tensor(1.0 / 11).item()
+
+
+@pytest.mark.parametrize("B,T", [(0, 4), (2, 0)])
+def test_lattices_without_rows(device, B, T):
+    """One loss a sequence, however many sequences and rows of each there are."""
+    import k2_amd as k2
+    x = torch.zeros(B, T, 3, 9, device=device, requires_grad=True)
+    a, t = torch.zeros(B, T, 3, 2, device=device), torch.zeros(B, T, 3, 2, dtype=torch.int64, device=device)
+    ranges, boundary = torch.zeros(B, T, 3, dtype=torch.int64, device=device), torch.zeros(B, 4, dtype=torch.int64, device=device)
+    for reduction in ("none", "sum", "mean"):
+        loss = k2.rnnt_distillation_loss_pruned(x, a, t, ranges, boundary, reduction=reduction)
+        assert loss.shape == ((B,) if reduction == "none" else ()) and loss.eq(0).all()
+        assert torch.autograd.grad(loss, x, torch.ones_like(loss))[0].shape == x.shape
