@@ -247,7 +247,8 @@ __global__ __launch_bounds__(kThreads) void DistillShortKernel(const T *__restri
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     DropListed(part, a.C, lane, listed[group]);
   }
-  const Sums sums = SumsOf<false>(part, HighOf(part), a.c);
+  const float high = HighOf(part);
+  const Sums sums = SumsOf<false>(part, state == kUsable ? high : Real<float>::NegInf(), a.c);
   ReadLogits<T, kShort>(x, list, lane, x_first);
   // (lane 0 of a group writes: one without a row is given another)
   FinishRow<kShort, kRest>(list, state, repeated, sums, there ? lane : lane + kShort, a.c, a.inv_tau, live, a.row_losses + row,

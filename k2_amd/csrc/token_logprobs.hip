@@ -268,7 +268,7 @@ __global__ __launch_bounds__(kThreads) void TokenShortKernel(const T *__restrict
     high = fmaxf(high, group[u]);
   }
   high = GroupMax<kShort>(high);
-  const Sums sums = SumsOf<kEntropy>(part, high, a.c);
+  const Sums sums = SumsOf<kEntropy>(part, live ? high : Real<float>::NegInf(), a.c);
   if (there && !live) {
     for (int i = lane; i < max(max(a.n, a.k), 1); i += kShort) WriteSkippedRow(a, row, i);
   } else if (there) {

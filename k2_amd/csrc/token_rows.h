@@ -333,18 +333,35 @@ __device__ __forceinline__ Sums JoinLanes(const Sums &a, float c) {
 // m, s and t (kEntropy) of what a group of lanes holds, from its largest logit.  The inner loop is one fused multiply-add,
 // one exponential and one addition an element: d = x c - M with M = m c rounded, which leaves every exponent off by the same
 // M - m c, exactly known and below a half, and that is taken out of the sums at the end.  Rows whose m c is beyond kFar (a
-// type's lowest value everywhere, a temperature of nearly 0) take the difference first.
+// type's lowest value everywhere, a temperature of nearly 0) take the difference first.  Each row chooses for itself: where the
+// rows of a wavefront differ, both forms are computed, so that no row's bits depend on what lies next to it.  (Rows that do
+// not count come with -inf as their largest logit: whatever they hold, they never ask for the second form.)
 constexpr float kFar = 1.0e6f;
 template <bool kEntropy, typename T, int U, int W, int L>
 __device__ __forceinline__ Sums SumsOf(RowPart<T, U, W, L> &part, float high, float c) {
   constexpr int kN = Lanes<T>::kN;
   Sums r{high == Real<float>::NegInf() ? 0.0f : high, 0.0f, 0.0f};
-  float s[4] = {0, 0, 0, 0}, t[4] = {0, 0, 0, 0};
 #pragma unroll
   for (int u = 0; u < U; ++u) part.Packed(u);  // (here, and not in the two branches: each would get registers of its own)
-  const bool far = __ballot(!(fabsf(r.m * c) <= kFar)) != 0;
-  const float shift = far ? 0.0f : -(r.m * c);
-  if (far) {
+  const bool far = !(fabsf(r.m * c) <= kFar);
+  if (__ballot(!far) != 0) {
+    const float shift = -(r.m * c);
+    float s[4] = {0, 0, 0, 0}, t[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int e = 0; e < kN; ++e) {
+        const float d = __builtin_fmaf(ElementOf<T>(part.v[u], e), c, shift), p = Exp2(d);
+        s[e & 3] += p;
+        if (kEntropy) t[e & 3] += fmaxf(d, kNothing) * p;
+      }
+    const float off = __builtin_fmaf(r.m, c, shift), scale = Exp2(-off);
+    r.s = GroupSum<L>((s[0] + s[1]) + (s[2] + s[3]));
+    if (kEntropy) r.t = (GroupSum<L>((t[0] + t[1]) + (t[2] + t[3])) - off * r.s) * scale;
+    r.s *= scale;
+  }
+  if (__ballot(far) != 0) {
+    float s[4] = {0, 0, 0, 0}, t[4] = {0, 0, 0, 0};
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       Vec v;
@@ -357,20 +374,13 @@ __device__ __forceinline__ Sums SumsOf(RowPart<T, U, W, L> &part, float high, fl
         if (kEntropy) t[e & 3] += fmaxf(d, kNothing) * p;
       }
     }
-  } else {
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int e = 0; e < kN; ++e) {
-        const float d = __builtin_fmaf(ElementOf<T>(part.v[u], e), c, shift), p = Exp2(d);
-        s[e & 3] += p;
-        if (kEntropy) t[e & 3] += fmaxf(d, kNothing) * p;
-      }
+    const float s_far = GroupSum<L>((s[0] + s[1]) + (s[2] + s[3]));
+    const float t_far = kEntropy ? GroupSum<L>((t[0] + t[1]) + (t[2] + t[3])) : 0.0f;
+    if (far) {
+      r.s = s_far;
+      r.t = t_far;
+    }
   }
-  const float off = far ? 0.0f : __builtin_fmaf(r.m, c, shift), scale = Exp2(-off);
-  r.s = GroupSum<L>((s[0] + s[1]) + (s[2] + s[3]));
-  if (kEntropy) r.t = (GroupSum<L>((t[0] + t[1]) + (t[2] + t[3])) - off * r.s) * scale;
-  r.s *= scale;
   return r;
 }
 

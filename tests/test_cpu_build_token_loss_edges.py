@@ -1,5 +1,5 @@
 """Calls of k2_amd/token_loss.py at the edges of what it takes, on the host build of the kernels through both host layers: lists
-with values that are no log-probs, forward-mode tangents, lattices without rows."""
+with values that are no log-probs, forward-mode tangents, lattices without rows, rows next to others."""
 import pytest
 import torch
 
@@ -86,3 +86,33 @@ def test_lattices_without_rows(host, B, T, R):  # noqa: F811
                     (grad,) = torch.autograd.grad(loss, x, torch.ones_like(loss))
                     assert grad.shape == x.shape
     assert k2.distillation_loss(x, a, t, reduction="none").shape == (B, T, R)
+
+
+@pytest.mark.parametrize("C,dtype", [(37, torch.float32), (300, torch.bfloat16), (500, torch.float32)])
+def test_rows_do_not_see_their_neighbours(host, C, dtype):  # noqa: F811
+    """Four short rows share a wavefront: whatever three of them hold, masked out or not, the fourth's bits are the same."""
+    import k2_amd as k2
+    rows = 8
+    x = orc.logits_case(C, rows, C, dtype, CPU)
+    x[6] = 3.0e7 * torch.sign(x[6].float()).to(dtype)  # (one that takes differences first)
+    a, t = orc.teacher_case(1, x, 4, 1.0, repeat=True)
+    keep = torch.tensor([True, False, False, True, False, False, True, False])
+    others = torch.randn(int((~keep).sum()), C)
+    fillings = [others, others * 1e30, torch.full_like(others, torch.finfo(dtype).min), torch.full_like(others, NAN),
+                torch.full_like(others, NEG), torch.full_like(others, INF)]
+    for mask in (keep, None):
+        want = None
+        for filling in fillings:
+            y = x.clone()
+            y[~keep] = filling.to(dtype)
+            y.requires_grad_()
+            got = k2.get_token_logprobs(y, t[:, 0].clamp(min=0), mask=mask, num_top=3, return_entropy=True)
+            (grad,) = torch.autograd.grad([got.logprobs, got.entropy], y, [torch.ones(rows)] * 2)
+            results = [*got, grad]
+            for rest in ("renormalise", "bucket"):
+                loss = k2.distillation_loss(y, a, t, mask=mask, rest=rest, reduction="none")
+                results += [loss, torch.autograd.grad(loss.sum(), y)[0]]
+            results = [u.detach()[keep] for u in results]
+            want = want or results
+            for u, w in zip(results, want):
+                assert torch.equal(u, w)

@@ -1,5 +1,5 @@
 """Calls of k2_amd/token_loss.py at the edges of what it takes, on the GPU: lists with values that are no log-probs, forward-mode
-tangents, sums of as many rows as are served, lattices without rows."""
+tangents, sums of as many rows as are served, lattices without rows, rows next to others."""
 import pytest
 import torch
 
@@ -87,3 +87,43 @@ def test_lattices_without_rows(device, B, T):
         loss = k2.rnnt_distillation_loss_pruned(x, a, t, ranges, boundary, reduction=reduction)
         assert loss.shape == ((B,) if reduction == "none" else ()) and loss.eq(0).all()
         assert torch.autograd.grad(loss, x, torch.ones_like(loss))[0].shape == x.shape
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("C", [9, 37, 300, 500, 1000, 1237])
+def test_rows_do_not_see_their_neighbours(device, dtype, C):
+    """Short rows share a wavefront: whatever the others hold, masked out or not, a row's bits are the same, and the same at
+    every place in the batch."""
+    import k2_amd as k2
+    rows = 64
+    x = orc.logits_case(C, rows, C, dtype, device)
+    if dtype != torch.float16:
+        x[6] = 3.0e7 * torch.sign(x[6].float()).to(dtype)  # (one that takes differences first)
+    a, t = orc.teacher_case(1, x, 4, 1.0, repeat=True)
+    gen = torch.Generator(device=device).manual_seed(C)
+    keep = torch.rand(rows, generator=gen, device=device) < 0.4
+    keep[6] = True
+    others = torch.randn(int((~keep).sum()), C, generator=gen, device=device)
+    fillings = [others, others * 1e4, others * 1e30, torch.full_like(others, torch.finfo(dtype).min),
+                torch.full_like(others, NAN), torch.full_like(others, NEG), torch.full_like(others, INF)]
+
+    def results(y, mask, a=a, t=t):
+        y = y.requires_grad_()
+        got = k2.get_token_logprobs(y, t[:, 0].clamp(min=0), mask=mask, num_top=3, return_entropy=True)
+        (grad,) = torch.autograd.grad([got.logprobs, got.entropy], y, [torch.ones(len(y), device=device)] * 2)
+        out = [*got, grad]
+        for rest in ("renormalise", "bucket"):
+            loss = k2.distillation_loss(y, a, t, mask=mask, rest=rest, reduction="none")
+            out += [loss, torch.autograd.grad(loss.sum(), y)[0]]
+        return [u.detach() for u in out]
+
+    want = [u[keep] for u in results(x.clone(), None)]
+    for mask in (keep, None):
+        for filling in fillings:
+            y = x.clone()
+            y[~keep] = filling.to(dtype)
+            for u, w in zip(results(y, mask), want):
+                assert torch.equal(u[keep], w)
+    order = torch.randperm(rows, generator=gen, device=device)
+    for u, w in zip(results(x[order].clone(), None, a[order], t[order]), results(x.clone(), None)):
+        assert torch.equal(u, w[order])
