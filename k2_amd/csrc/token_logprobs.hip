@@ -588,16 +588,21 @@ struct SoftmaxGrad {
 };
 
 // A row's entries in LDS, lane by lane of the n that share it; returns this lane's part of the sum of their gradients.
+// *wrong: whether a token of this lane's is past the vocabulary.
 __device__ __forceinline__ float ReadEntries(const BackwardArgs &a, size_t row, int i, int n, int entries, int *entry,
-                                             float *entry_grad, bool write) {
+                                             float *entry_grad, bool write, bool *wrong) {
   const int used = a.logprobs_grad != nullptr ? a.n : 0;
   float sum = 0.0f;
+  *wrong = false;
   for (; i < entries; i += n) {
     const bool given = i < used;
     const int64_t token = given ? a.tokens[row * a.n + i] : a.top_tokens[row * a.k + (i - used)];
     float g = given ? a.logprobs_grad[row * a.n + i] : a.top_grad[row * a.k + (i - used)];
     if (token < 0) g = 0.0f;
-    if (token >= a.C) g = __uint_as_float(0x7fc00000u);
+    if (token >= a.C) {
+      g = __uint_as_float(0x7fc00000u);
+      *wrong = true;
+    }
     sum += g;
     if (write) {
       entry[i] = token < 0 || token >= a.C ? -1 : (int)token;
@@ -607,18 +612,21 @@ __device__ __forceinline__ float ReadEntries(const BackwardArgs &a, size_t row, 
   return sum;
 }
 
-__device__ __forceinline__ SoftmaxGrad RowGradOf(const BackwardArgs &a, size_t row, float sum) {
+// wrong: whether one of the row's tokens is past the vocabulary
+__device__ __forceinline__ SoftmaxGrad RowGradOf(const BackwardArgs &a, size_t row, float sum, bool wrong) {
   const float s = a.stats[2 * row + 1];
   const float h = a.entropy_grad != nullptr ? a.entropy[row] : 0.0f;
   const float gh = a.entropy_grad != nullptr ? a.entropy_grad[row] : 0.0f;
   SoftmaxGrad f{a.stats[2 * row], a.c, 0.0f, 0.0f, 0.0f};
-  if (s != 0.0f) {  // (a row without any mass: every p is 0, and no logit moves a log-prob)
+  if (s != 0.0f) {
     f.entry = a.inv_tau;
     const float inv_s = a.inv_tau / s;
     f.flat = -inv_s * (sum + gh * (h - kLn2 * Log2(s)));
     f.slope = -inv_s * gh * kLn2;
-  } else if (sum != sum) {
-    f.flat = sum;
+  } else if (wrong) {
+    // (a row without any mass: every p is 0, and no logit moves a log-prob, whatever is sent back through it, NaN included;
+    // a wrong token shows all the same)
+    f.flat = __uint_as_float(0x7fc00000u);
   }
   return f;
 }
@@ -659,10 +667,11 @@ __global__ __launch_bounds__(kThreads) void TokenShortGradKernel(const T *__rest
   T *dx = logits_grad + row * (size_t)a.C;
   float *entry_grad = entries_lds + (size_t)in_block * 2 * entries;
   int *entry = reinterpret_cast<int *>(entry_grad + entries);
-  const float part_sum = ReadEntries(a, row, lane, kShort, live ? entries : 0, entry, entry_grad, true);
+  bool wrong;
+  const float part_sum = ReadEntries(a, row, lane, kShort, live ? entries : 0, entry, entry_grad, true, &wrong);
   RowPart<T, U, 1, kShort> part;
   part.Load(x, __ballot(live) != 0 ? a.C : 0, 0, 0, lane);
-  const SoftmaxGrad f = RowGradOf(a, row, GroupSum<kShort>(part_sum));
+  const SoftmaxGrad f = RowGradOf(a, row, GroupSum<kShort>(part_sum), GroupBallot<kShort>(wrong) != 0);
   const int all = live ? VecsOf<T>(a.C) : 0;
   T *to = kStage > 0 ? reinterpret_cast<T *>(stages + in_block * kStage) : dx;
 #pragma unroll
@@ -705,10 +714,11 @@ __global__ __launch_bounds__(W *kWave) void TokenLongGradKernel(const T *__restr
     return;
   }
   // (every wavefront needs the sum; the first leaves the list)
-  const float sum = WaveSumF(ReadEntries(a, row, lane, kWave, entries, entry, entry_grad, wave == 0));
+  bool wrong;
+  const float sum = WaveSumF(ReadEntries(a, row, lane, kWave, entries, entry, entry_grad, wave == 0, &wrong));
   RowPart<T, U, W> part;
   part.template Load<kPast>(x, a.C, first, wave, lane);
-  const SoftmaxGrad f = RowGradOf(a, row, sum);
+  const SoftmaxGrad f = RowGradOf(a, row, sum, __ballot(wrong) != 0);
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const int at = part.Vector(u, first, wave, lane);

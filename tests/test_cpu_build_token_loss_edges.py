@@ -1,5 +1,6 @@
 """Calls of k2_amd/token_loss.py at the edges of what it takes, on the host build of the kernels through both host layers: lists
-with values that are no log-probs, forward-mode tangents, lattices without rows, rows next to others."""
+with values that are no log-probs, forward-mode tangents, lattices without rows, rows next to others,
+rows of nothing."""
 import pytest
 import torch
 
@@ -116,3 +117,24 @@ def test_rows_do_not_see_their_neighbours(host, C, dtype):  # noqa: F811
             want = want or results
             for u, w in zip(results, want):
                 assert torch.equal(u, w)
+
+
+@pytest.mark.parametrize("C,dtype", [(1, torch.float32), (40, torch.bfloat16), (700, torch.float32), (2300, torch.float16)])
+@pytest.mark.parametrize("up", [[NAN, 0.0], [INF, NEG], [INF, INF], [1.0, NAN]])
+def test_rows_of_nothing_whatever_is_sent_back(host, C, dtype, up):  # noqa: F811
+    """A row of nothing but -inf has gradient 0, and a token past the vocabulary shows in it all the same."""
+    import k2_amd as k2
+    x = orc.logits_case(C, 4, C, dtype, CPU)
+    x[1:3] = NEG
+    x.requires_grad_()
+    tokens = torch.tensor([[0, C - 1]] * 4)
+    tokens[2, 1] = C
+    got = k2.get_token_logprobs(x, tokens, num_top=2, return_entropy=True)
+    ups = [torch.full_like(u, 3.0) for u in (got.logprobs, got.entropy, got.top_logprobs)]
+    for u in ups[0], ups[2]:
+        u[1] = torch.tensor(up)
+    ups[1][1] = up[0]
+    (grad,) = torch.autograd.grad([got.logprobs, got.entropy, got.top_logprobs], x, ups, retain_graph=True)
+    assert grad[1].eq(0).all() and grad[2].isnan().all() and torch.isfinite(grad[[0, 3]]).all()
+    (grad,) = torch.autograd.grad(got.logprobs, x, ups[0])
+    assert grad[1].eq(0).all() and grad[2].isnan().all()

@@ -1,5 +1,6 @@
 """Calls of k2_amd/token_loss.py at the edges of what it takes, on the GPU: lists with values that are no log-probs, forward-mode
-tangents, sums of as many rows as are served, lattices without rows, rows next to others."""
+tangents, sums of as many rows as are served, lattices without rows, rows next to others,
+rows of nothing."""
 import pytest
 import torch
 
@@ -127,3 +128,23 @@ def test_rows_do_not_see_their_neighbours(device, dtype, C):
     order = torch.randperm(rows, generator=gen, device=device)
     for u, w in zip(results(x[order].clone(), None, a[order], t[order]), results(x.clone(), None)):
         assert torch.equal(u, w[order])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("C", [5, 500, 1237, 4999, 131072])
+def test_rows_of_nothing_whatever_is_sent_back(device, dtype, C):
+    """A row of nothing but -inf has gradient 0, and a token past the vocabulary shows in it all the same."""
+    import k2_amd as k2
+    x = orc.logits_case(C, 4, C, dtype, device)
+    x[1:3] = NEG
+    x.requires_grad_()
+    tokens = torch.tensor([[0, C - 1]] * 4, device=device)
+    tokens[2, 1] = C
+    got = k2.get_token_logprobs(x, tokens, num_top=2, return_entropy=True)
+    for up in ([NAN, 0.0], [INF, NEG], [INF, INF], [1.0, NAN]):
+        ups = [torch.full_like(u, 3.0) for u in (got.logprobs, got.entropy, got.top_logprobs)]
+        for u in ups[0], ups[2]:
+            u[1] = torch.tensor(up, device=device)
+        ups[1][1] = up[0]
+        (grad,) = torch.autograd.grad([got.logprobs, got.entropy, got.top_logprobs], x, ups, retain_graph=True)
+        assert grad[1].eq(0).all() and grad[2].isnan().all() and torch.isfinite(grad[[0, 3]]).all()
