@@ -796,7 +796,7 @@ _LOGITS_DTYPES = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
 
 def _logits_rows(logits):
     """(logits, rows, row stride, C, dtype code) of logits [..., C]: as they are where their rows lie at one distance from
-    each other, else a dense copy."""
+    each other, else a dense copy (also of what torch only marks as negated: the kernels read the memory itself)."""
     if not isinstance(logits, torch.Tensor) or logits.dtype not in _LOGITS_DTYPES:
         raise RuntimeError("k2_amd: logits must be a float32, float16 or bfloat16 tensor")
     if not _on_device(logits):
@@ -805,6 +805,7 @@ def _logits_rows(logits):
         raise RuntimeError(f"k2_amd: logits must be [..., C] with C >= 1, got {list(logits.shape)}")
     C = logits.shape[-1]
     rows = logits.numel() // C
+    logits = logits.resolve_neg()
     if logits.is_contiguous():
         return logits, rows, C, C, _LOGITS_DTYPES[logits.dtype]
     stride, expected = C, None

@@ -869,7 +869,8 @@ namespace {
 
 typedef torch::optional<torch::Tensor> OptionalTensor;
 
-// logits [..., C] as rows: as they are where their rows lie at one distance from each other, else a dense copy
+// logits [..., C] as rows: as they are where their rows lie at one distance from each other, else a dense copy (also of what
+// torch only marks as negated: the kernels read the memory itself)
 struct LogitsRows {
   torch::Tensor x;
   int64_t rows, stride, C;
@@ -888,17 +889,18 @@ struct LogitsRows {
     rows = logits.numel() / C;
     lead.assign(logits.sizes().begin(), logits.sizes().end() - 1);
     stride = C;
-    if (logits.is_contiguous()) return;
-    bool uniform = logits.stride(-1) == 1 || C == 1;
+    if (logits.is_neg()) x = logits.resolve_neg();
+    if (x.is_contiguous()) return;
+    bool uniform = x.stride(-1) == 1 || C == 1;
     int64_t expected = -1;
-    for (int64_t d = logits.dim() - 2; d >= 0; --d) {
-      if (logits.size(d) == 1) continue;
-      if (expected < 0) stride = logits.stride(d);
-      else if (logits.stride(d) != expected) uniform = false;
-      expected = logits.stride(d) * logits.size(d);
+    for (int64_t d = x.dim() - 2; d >= 0; --d) {
+      if (x.size(d) == 1) continue;
+      if (expected < 0) stride = x.stride(d);
+      else if (x.stride(d) != expected) uniform = false;
+      expected = x.stride(d) * x.size(d);
     }
     if (!uniform) {
-      x = logits.contiguous();
+      x = x.contiguous();
       stride = C;
     }
   }
@@ -1079,7 +1081,7 @@ torch::Tensor OnceDifferentiable(torch::Tensor grad) {
       "k2_amd: trying to differentiate twice a function that is differentiable once", 1);
   return (*refuse)({grad})[0];
 }
-torch::Tensor Dense(const torch::Tensor &t) { return t.defined() ? t.contiguous() : t; }
+torch::Tensor Dense(const torch::Tensor &t) { return t.defined() ? t.resolve_neg().contiguous() : t; }
 OptionalTensor Maybe(const torch::Tensor &t) { return t.defined() ? OptionalTensor(t) : OptionalTensor(); }
 torch::Tensor Undefined(const OptionalTensor &t) { return Given(t) ? *t : torch::Tensor(); }
 

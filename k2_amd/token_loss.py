@@ -72,13 +72,13 @@ class _Distillation(torch.autograd.Function):
     def backward(ctx, loss_grad):
         logits, top_logprobs, top_tokens, records, inverse_count = ctx.saved_tensors
         temperature, bucket, factor = ctx.meta
-        grad = native.distillation_backward(logits, top_logprobs, top_tokens, records, loss_grad.contiguous(), inverse_count,
+        grad = native.distillation_backward(logits, top_logprobs, top_tokens, records, _dense(loss_grad), inverse_count,
                                             factor, temperature, bucket)
         return (grad,) + (None,) * 8
 
 
 def _dense(t: Optional[Tensor]) -> Optional[Tensor]:
-    return None if t is None else t.contiguous()
+    return None if t is None else t.resolve_neg().contiguous()
 
 
 def _check_logits(logits: Tensor, mask: Optional[Tensor], temperature: float) -> Optional[Tensor]:
@@ -152,7 +152,7 @@ def _distillation_args(logits, top_logprobs, top_tokens, mask, temperature, rest
         raise ValueError(f"rest should be ('renormalise' | 'bucket'), given {rest}")
     if reduction not in ("none", "mean", "sum"):
         raise ValueError(f"reduction should be ('none' | 'mean' | 'sum'), given {reduction}")
-    return (logits, top_logprobs.to(device=logits.device, dtype=torch.float32).contiguous(), _dev_i64(top_tokens, logits), mask,
+    return (logits, _dense(top_logprobs.to(device=logits.device, dtype=torch.float32)), _dev_i64(top_tokens, logits), mask,
             float(temperature), rest == "bucket")
 
 
