@@ -1,6 +1,6 @@
 """Calls of k2_amd/token_loss.py at the edges of what it takes, on the host build of the kernels through both host layers: lists
 with values that are no log-probs, forward-mode tangents, lattices without rows, rows next to others,
-rows of nothing, tensors marked as negated."""
+rows of nothing, tensors marked as negated, long lists on short rows."""
 import pytest
 import torch
 
@@ -162,3 +162,20 @@ def test_tensors_that_are_marked_as_negated(host):  # noqa: F811
                  (x, a, torch._neg_view(-up))):
         for u, w in zip(results(*args), want):
             assert torch.equal(u, w)
+
+
+def test_long_lists_on_short_rows(host):  # noqa: F811
+    """The most that a gradient keeps in LDS beside the rows it stages."""
+    import k2_amd as k2
+    C, rows, K = 300, 3, 256
+    x = orc.logits_case(1, rows, C, torch.float32, CPU).requires_grad_()
+    a, t = orc.teacher_case(1, x.detach(), K, 1.0, repeat=True)
+    for bucket in (False, True):
+        loss = k2.distillation_loss(x, a, t, rest="bucket" if bucket else "renormalise", reduction="none")
+        (grad,) = torch.autograd.grad(loss, x, torch.ones(rows))
+        orc.check_distillation(x.detach(), a, t, None, 1.0, bucket, loss.detach(), torch.ones(rows), grad)
+    tokens = torch.randint(0, C, (rows, 64))
+    got = k2.get_token_logprobs(x, tokens, num_top=64)
+    ups = torch.randn(rows, 64), torch.randn(rows, 64)
+    (grad,) = torch.autograd.grad([got.logprobs, got.top_logprobs], x, ups)
+    orc.check_token_grad(x.detach(), tokens, None, 1.0, (ups[0], None, ups[1]), got.top_tokens, grad)

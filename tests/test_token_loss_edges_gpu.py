@@ -1,6 +1,6 @@
 """Calls of k2_amd/token_loss.py at the edges of what it takes, on the GPU: lists with values that are no log-probs, forward-mode
 tangents, sums of as many rows as are served, lattices without rows, rows next to others,
-rows of nothing."""
+rows of nothing, long lists on short rows."""
 import pytest
 import torch
 
@@ -148,3 +148,34 @@ def test_rows_of_nothing_whatever_is_sent_back(device, dtype, C):
         ups[1][1] = up[0]
         (grad,) = torch.autograd.grad([got.logprobs, got.entropy, got.top_logprobs], x, ups, retain_graph=True)
         assert grad[1].eq(0).all() and grad[2].isnan().all() and torch.isfinite(grad[[0, 3]]).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("C", [70, 300, 500, 512, 1000, 1024])
+def test_long_lists_on_short_rows(device, dtype, C):
+    """The most that a gradient keeps in LDS beside the rows it stages: 256 entries a row of a teacher's list, 64 given tokens
+    and 64 alternatives."""
+    import k2_amd as k2
+    rows = 37
+    for K in (65, 100, 256):
+        x = orc.logits_case(C + K, rows, C, dtype, device).requires_grad_()
+        a, t = orc.teacher_case(K, x.detach(), K, 1.0, holes=True, repeat=True)
+        mask = torch.rand(rows, device=device) < 0.8
+        up = torch.randn(rows, device=device)
+        for bucket in (False, True):
+            loss = k2.distillation_loss(x, a, t, mask=mask, rest="bucket" if bucket else "renormalise", reduction="none")
+            (grad,) = torch.autograd.grad(loss, x, up)
+            orc.check_distillation(x.detach(), a, t, mask, 1.0, bucket, loss, up, grad)
+    for n, k in ((17, 0), (3, 20), (64, 64)):
+        x = orc.logits_case(C + n, rows, C, dtype, device).requires_grad_()
+        tokens = torch.randint(0, C, (rows, n), device=device)
+        tokens[1, 0], tokens[2, 1] = -1, tokens[2, 0]
+        got = k2.get_token_logprobs(x, tokens, mask=mask, num_top=k, return_entropy=True)
+        orc.check_token_logprobs(x.detach(), tokens, mask, 1.0, k,
+                                 k2.TokenLogprobs(*(None if u is None else u.detach() for u in got)))
+        ups = [torch.randn(rows, n, device=device), torch.randn(rows, device=device), torch.randn(rows, k, device=device) if k else None]
+        (grad,) = torch.autograd.grad([u for u in (got.logprobs, got.entropy, got.top_logprobs) if u is not None], x,
+                                      [u for u in ups if u is not None])
+        if k:
+            ups[2][got.top_tokens < 0] = 0.0
+        orc.check_token_grad(x.detach(), tokens, mask, 1.0, (ups[0], ups[1].unsqueeze(1), ups[2]), got.top_tokens, grad)
