@@ -434,7 +434,8 @@ K2AMD_API int k2amd_lattice_fill(const int32_t *ranges, const int32_t *frames,
 /* ------------------------------------------------------------------ rows of output logits
  *
  * No counterpart in the reference.  `logits`: `rows` rows of C elements (dtype K2AMD_F32, K2AMD_F16 or K2AMD_BF16), row r
- * at element r * row_stride, any alignment of the element type; p = softmax(x / temperature) of a row x, temperature > 0 (1.45 / temperature a float).
+ * at element r * row_stride, any alignment of the element type; p = softmax(x / temperature) of a row x, temperature > 0 and
+ * finite, and log2(e) / temperature at most FLT_MAX (else K2AMD_ERR_INVALID_ARGUMENT).
  * `mask` [rows] (one byte a row, 0: the row does not count, whatever it holds) or NULL.  Sums are held in 32 bits or more;
  * results do not depend on the order in which workgroups run.  Served: fewer than 2^31 rows of up to 2^20 columns.
  *

@@ -139,7 +139,7 @@ __device__ __forceinline__ void FinishRow(List list, ListState state, unsigned r
                                           float inv_tau, bool live, float *loss_out, float *record) {
   if (state != kUsable) list.K = 0;
   float a_max = Real<float>::NegInf(), m_set = Real<float>::NegInf();
-  for (int j = lane, r = 0; j < list.K; j += L, ++r) {
+  for (int j = lane; j < list.K; j += L) {
     a_max = fmaxf(a_max, list.a[j]);
     m_set = fmaxf(m_set, list.x[j]);
   }
@@ -357,7 +357,7 @@ template <bool kRest>
 struct RowGrad {
   float from, coefficient, m, share, lse, g;
   bool skipped;
-  __device__ __forceinline__ RowGrad(const float4 &r, float scale, float /*c*/)
+  __device__ __forceinline__ RowGrad(const float4 &r, float scale)
       : from(r.x), coefficient(r.y * scale), m(kRest ? r.z : r.x), share(r.w), lse(kRest ? 0.0f : r.z), g(scale),
         skipped(r.w == kSkipped) {}
   __device__ __forceinline__ float Unlisted(float x, float c) const { return coefficient * Exp2((x - from) * c); }
@@ -402,7 +402,7 @@ __global__ __launch_bounds__(kThreads) void DistillShortGradKernel(const T *__re
     given = a.top_tokens[row * a.K + lane];
     teacher = a.top_logprobs[row * a.K + lane];
   }
-  const RowGrad<kRest> f(record, scale, a.c);
+  const RowGrad<kRest> f(record, scale);
   const bool live = there && !f.skipped;
   RowPart<T, U, 1, kShort> part;
   part.Load(x, __ballot(live) != 0 ? a.C : 0, 0, 0, lane);
@@ -450,7 +450,7 @@ __global__ __launch_bounds__(W *kWave) void DistillLongGradKernel(const T *__res
   const int first = (int)blockIdx.y * (U * W * kWave), all = VecsOf<T>(a.C);
   const T *x = logits + row * a.row_stride;
   T *dx = logits_grad + row * (size_t)a.C;
-  const RowGrad<kRest> f(*reinterpret_cast<const float4 *>(a.records + 4 * row), a.scale.At(row), a.c);
+  const RowGrad<kRest> f(*reinterpret_cast<const float4 *>(a.records + 4 * row), a.scale.At(row));
   RowPart<T, U, W> part;
   part.template Load<kPast>(x, f.skipped ? 0 : a.C, first, wave, lane);
   for (int j = threadIdx.x; j < a.K; j += W * kWave) {

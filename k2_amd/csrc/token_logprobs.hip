@@ -108,7 +108,7 @@ __device__ __forceinline__ int ListByClasses(RowPart<T, U, W> &part, int C, int 
   for (int round = 0; count < k; ++round) {
     // the first class: the NaNs; the second: the largest; then the largest below the last
     float high = Real<float>::NegInf();
-      if (round > 0) {
+    if (round > 0) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const Vec &v = part.Packed(u);
@@ -119,7 +119,7 @@ __device__ __forceinline__ int ListByClasses(RowPart<T, U, W> &part, int C, int 
         }
       }
       high = WaveMaxF(high);
-        }
+    }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (count >= k) continue;
