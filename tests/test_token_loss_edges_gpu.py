@@ -1,6 +1,7 @@
 """Calls of k2_amd/token_loss.py at the edges of what it takes, on the GPU: lists with values that are no log-probs, forward-mode
 tangents, sums of as many rows as are served, lattices without rows, rows next to others,
-rows of nothing, long lists on short rows."""
+rows of nothing, long lists on short rows, the longest rows and the most of them, rows in parts in
+graphs, two threads."""
 import pytest
 import torch
 
@@ -179,3 +180,141 @@ def test_long_lists_on_short_rows(device, dtype, C):
         if k:
             ups[2][got.top_tokens < 0] = 0.0
         orc.check_token_grad(x.detach(), tokens, mask, 1.0, (ups[0], ups[1].unsqueeze(1), ups[2]), got.top_tokens, grad)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("C", [(1 << 20) - 3, 1 << 20])
+@pytest.mark.parametrize("rows", [1, 3, 300])
+def test_the_longest_rows(device, dtype, C, rows):
+    """Rows of as many columns as are served, in up to 64 parts."""
+    import k2_amd as k2
+    pick = torch.arange(rows, device=device)[-2:]
+    x = orc.logits_case(rows, rows, C, dtype, device).requires_grad_()
+    tokens = torch.randint(0, C, (rows, 1), device=device)
+    tokens[-1] = C - 1
+    got = k2.get_token_logprobs(x, tokens, num_top=64, return_entropy=True)
+    orc.check_token_logprobs(x.detach()[pick], tokens[pick], None, 1.0, 64, k2.TokenLogprobs(*(u.detach()[pick] for u in got)))
+    ups = torch.randn(rows, 1, device=device), torch.randn(rows, device=device), torch.randn(rows, 64, device=device)
+    (grad,) = torch.autograd.grad([got.logprobs, got.entropy, got.top_logprobs], x, ups)
+    orc.check_token_grad(x.detach()[pick], tokens[pick], None, 1.0, (ups[0][pick], ups[1][pick].unsqueeze(1), ups[2][pick]),
+                         got.top_tokens[pick], grad[pick])
+    without = k2.get_token_logprobs(x.detach(), tokens, return_entropy=True)
+    orc.check_token_logprobs(x.detach()[pick], tokens[pick], None, 1.0, 0,
+                             k2.TokenLogprobs(without.logprobs[pick], without.entropy[pick], None, None))
+    del got, grad, without
+    a, t = orc.teacher_case(1, x.detach()[pick], 100, 1.0, repeat=True)
+    A, Tt = torch.full((rows, 100), NEG, device=device), torch.full((rows, 100), -1, dtype=torch.int64, device=device)
+    A[pick], Tt[pick] = a, t
+    up = torch.randn(rows, device=device)
+    for rest in ("renormalise", "bucket"):
+        loss = k2.distillation_loss(x, A, Tt, rest=rest, reduction="none")
+        (grad,) = torch.autograd.grad(loss, x, up)
+        orc.check_distillation(x.detach()[pick], a, t, None, 1.0, rest == "bucket", loss.detach()[pick], up[pick], grad[pick])
+
+
+def test_more_long_rows_than_a_launch_takes(device):
+    """Rows of several wavefronts beyond 2^20 of them: the last rows of both launches against the definition."""
+    import k2_amd as k2
+    rows, C = (1 << 20) + 5, 2056
+    pick = torch.tensor([0, (1 << 20) - 1, 1 << 20, rows - 1], device=device)
+    part = orc.logits_case(3, len(pick), C, torch.bfloat16, device)
+    x = torch.zeros(rows, C, dtype=torch.bfloat16, device=device)
+    x[pick] = part
+    x.requires_grad_()
+    tokens = torch.randint(0, C, (rows,), device=device)
+    mask = torch.ones(rows, dtype=torch.bool, device=device)
+    mask[(1 << 20) + 1] = False
+    for k in (0, 2):
+        got = k2.get_token_logprobs(x, tokens, mask=mask, num_top=k, return_entropy=True)
+        orc.check_token_logprobs(part, tokens[pick].unsqueeze(1), None, 1.0, k,
+                                 k2.TokenLogprobs(*(None if u is None else u.detach()[pick] for u in got)))
+        assert got.logprobs[(1 << 20) + 1] == 0 and got.entropy[(1 << 20) + 1] == 0
+    (grad,) = torch.autograd.grad(got.logprobs.sum(), x)
+    orc.check_token_grad(part, tokens[pick].unsqueeze(1), None, 1.0, (torch.ones(len(pick), 1, device=device), None, None), None,
+                         grad[pick])
+    assert grad[(1 << 20) + 1].eq(0).all()
+    del grad, got
+    a, t = orc.teacher_case(4, part, 3, 1.0)
+    A, Tt = torch.full((rows, 3), NEG, device=device), torch.full((rows, 3), -1, dtype=torch.int64, device=device)
+    A[pick], Tt[pick] = a, t
+    loss = k2.distillation_loss(x, A, Tt, mask=mask, rest="bucket", reduction="none")
+    (grad,) = torch.autograd.grad(loss.sum(), x)
+    orc.check_distillation(part, a, t, None, 1.0, True, loss.detach()[pick], torch.ones(len(pick), device=device), grad[pick])
+    assert int(grad.ne(0).any(1).sum()) == len(pick) and int(loss.ne(0).sum()) == len(pick)
+
+
+def test_rows_in_parts_in_graphs(device):
+    """Calls that join parts of rows through scratch memory, captured twice and replayed in turn with new inputs."""
+    import k2_amd as k2
+    rows, C, K = 5, 40009, 6
+    x = orc.logits_case(1, rows, C, torch.float32, device)
+    a, t = orc.teacher_case(2, x, K, 1.0)
+    tokens = torch.randint(0, C, (rows,), device=device)
+    mask = torch.tensor([True, True, False, True, True], device=device)
+
+    def step(z):
+        got = k2.get_token_logprobs(z, tokens, mask=mask, num_top=9, return_entropy=True)
+        plain = k2.get_token_logprobs(z, tokens, mask=mask)
+        loss = k2.distillation_loss(z, a, t, mask=mask, rest="bucket")
+        (grad,) = torch.autograd.grad([got.logprobs.sum(), got.entropy.sum(), plain.logprobs.sum(), loss], z)
+        return (*got, plain.logprobs, loss, grad)
+
+    side = torch.cuda.Stream()
+    graphs = []
+    for _ in range(2):
+        inputs = x.clone()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            for _ in range(2):
+                step(inputs.detach().requires_grad_())
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outputs = step(inputs.detach().requires_grad_())
+        graphs.append((graph, inputs, outputs))
+    for turn in range(4):
+        for i, (graph, inputs, outputs) in enumerate(graphs):
+            y = orc.logits_case(10 * turn + i, rows, C, torch.float32, device)
+            eager = [u.detach().clone() for u in step(y.clone().requires_grad_())]
+            inputs.copy_(y)
+            graph.replay()
+            torch.cuda.synchronize()
+            for u, v in zip(eager, outputs):
+                assert torch.equal(u, v), (turn, i)
+
+
+def test_calls_from_two_threads_on_two_streams(device):
+    """The host layers hold no lock and no workspace: forward and backward at once on streams of their own."""
+    import threading
+    import k2_amd as k2
+    rows, C = 64, 33001
+    x = [orc.logits_case(i, rows, C, torch.bfloat16, device) for i in range(2)]
+    lists = [orc.teacher_case(i, x[i], 5, 1.0) for i in range(2)]
+    torch.cuda.synchronize()
+
+    def step(i):
+        z = x[i].detach().requires_grad_()
+        got = k2.get_token_logprobs(z, lists[i][1][:, 0], num_top=9, return_entropy=True)
+        loss = k2.distillation_loss(z, *lists[i], rest="bucket", reduction="sum")
+        (grad,) = torch.autograd.grad([got.logprobs.sum(), got.entropy.sum(), loss], z)
+        return [u.detach() for u in (*got, loss, grad)]
+
+    want, failures = [step(0), step(1)], []
+    torch.cuda.synchronize()
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(20):
+                    got = step(i)
+                    torch.cuda.current_stream().synchronize()
+                    assert all(torch.equal(u, v) for u, v in zip(got, want[i]))
+        except BaseException as error:  # (a thread's failure is not the test's by itself)
+            failures.append(error)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for thread in threads:
+        thread.start()
+    for thread in threads:
+        thread.join()
+    assert not failures, failures
