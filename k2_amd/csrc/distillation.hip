@@ -13,11 +13,11 @@
 // for every element, and the listed elements are then written over it.
 //
 // Measured on an MI355X, kernel times after some hundred passes.  80000 x 500 (four fifths of the rows count), lists of 8, with
-// a rest: forward 46 us in float32 and 29 in bfloat16, backward 56 and 28.  The forward pass of a training loop reads while the 160 MB (80 MB) of the
-// last gradient leave the memory-side cache: with all its arithmetic taken out it took 40 us and 20 us.  8192 x 32000,
-// lists of 20: forward 102 us in bfloat16 (5.1 TB/s) and 188 in float32 (5.6), backward 185 and 369 (5.7 TB/s both).
-// 2048 x 131072, lists of 64, with a rest: forward in two parts 113 us in bfloat16 and 191 in float32 and 8 for their join,
-// backward 181 and 383.
+// a rest: forward 46 us in float32 and 29 in bfloat16, backward 56 and 28.  The forward pass of a training
+// loop reads while the 160 MB (80 MB) of the last gradient leave the memory-side cache: with all its arithmetic taken out it
+// took 40 us and 20 us.  8192 x 32000, lists of 20: forward 102 us in bfloat16 (5.1 TB/s) and 188 in float32 (5.6), backward
+// 185 and 369 (5.7 TB/s both).  2048 x 131072, lists of 64, with a rest: forward in two parts 113 us in bfloat16 and 191 in
+// float32 and 8 for their join, backward 181 and 383.
 #include "token_rows.h"
 
 namespace k2amd {

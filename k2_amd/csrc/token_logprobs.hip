@@ -7,7 +7,7 @@
 // with c_j the given tokens and the alternatives together and g_j what reaches their log-probs.
 //
 // Measured on an MI355X, kernel times after some hundred passes: 80000 x 500 float32, four fifths of the rows, 8 alternatives,
-// 43 us (20 us to read them; the arithmetic, half of it the selection, keeps the vector units busy for 27); 4096 x 32000 with
+// 43 us (20 us to read them; the arithmetic, half of it the selection, keeps the vector units busy for 23); 4096 x 32000 with
 // 64 alternatives 98 us in bfloat16 (41 to read; the selection is two thirds of the instructions) and in float32, whose rows
 // are two parts, 143 and 20 for the join; 6553 of 8191 x 32000 with entropy 83 us in bfloat16 (5.0 TB/s) and 146 in float32
 // (5.8), and their gradient 156 (419 MB read, 524 MB written: 6.0 TB/s) and 331 (5.7); one row of 131072 with 20 alternatives
